@@ -113,7 +113,8 @@ B200MOE_API int b200moe_quant_1x128(const void* x, int64_t M, int64_t K, int64_t
 /* ------------------------------------------------------------------------
  * Weight quantisation: per_block_quant_fp8(w, 128, 128)
  * (phase5_orchestrator.py:35-41). w (E, N, K) bf16 contiguous -> q (E, N, K)
- * fp8 and s (E, N/128, K/128) fp32, s = max(block amax/448, 1e-12).
+ * fp8 and s (E, ceil(N/128), K/128) fp32, s = max(block amax/448, 1e-12). The
+ * last block of an N that is no multiple of 128 covers the rows that exist.
  * ---------------------------------------------------------------------- */
 B200MOE_API int b200moe_quant_block128(const void* w, int64_t E, int64_t N, int64_t K, uint8_t* q, float* s, void* stream);
 
@@ -514,6 +515,53 @@ B200MOE_API int b200moe_experts_fused(const void* hidden, int64_t M, int topk, c
  * sglang_integration/aiter.py:164-177. */
 B200MOE_API int b200moe_combine_reduce(const void* out_pair, const int32_t* slot_pos, int sorted_rows, int64_t M,
                            int topk, int64_t H, void* out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Dense (not expert-grouped) products in the layer's number formats, for the
+ * parts of a MoE block around the routed experts: projections, the shared
+ * expert, dense feed-forward layers. No counterpart in the reference, whose
+ * shared expert is fused as one more routed slot by its serving framework.
+ *
+ * b200moe_linear:
+ *   out[m, n] = sum_kb x_scale[m, kb] * w_scale[n / 128, kb]
+ *               * sum_{k in block kb} x_q[m, k] * w[n, k]  (+ residual[m, n])
+ * in fp32, rounded once to bf16 (out_f32 = 0) or stored as f32 (1).
+ * Activations: either x (M, K) bf16, quantised first as b200moe_quant_1x128
+ * does (into the workspace, b200moe_linear_workspace_size() bytes, 256-byte
+ * aligned), or x_q (M, K) fp8 with x_scale (M, K/128); pass NULL for the other.
+ * ld_x / ld_xs are row strides in elements of x or x_q / x_scale (ld_xs is not
+ * read with bf16 rows). w (N, K) fp8 with row stride ld_w bytes; w_scale
+ * (ceil(N/128), K/128) contiguous. residual (M, N) bf16 or NULL; it may be out
+ * itself (the same address and stride, with bf16 out). Any M >= 0 and N >= 1;
+ * K % 128 == 0. Activation and weight rows start 16-byte aligned.
+ *
+ * b200moe_gate_up: the product with w13 (2I, H), gate/up rows interleaved (row
+ * 2j = gate j, 2j+1 = up j) as in the layer, then silu(gate) * up in fp32,
+ * quantised 1x128 into q (M, I) fp8 and s (M, I/128): the layer's stage 1 on
+ * dense rows. I % 128 == 0; rows of q start 16-byte aligned.
+ *
+ * b200moe_mlp: b200moe_gate_up followed by b200moe_linear with w2 (H, I) on its
+ * result, bit for bit: a dense or shared expert, residual = the routed output
+ * to add to. Weights contiguous; workspace b200moe_mlp_workspace_size() bytes,
+ * 256-byte aligned.
+ *
+ * A pipeline wait that gives up sets B200MOE_DEVERR_TIMEOUT in err_word
+ * (required) and leaves the outputs undefined.
+ * ---------------------------------------------------------------------- */
+B200MOE_API size_t b200moe_linear_workspace_size(int64_t M, int64_t K);
+B200MOE_API int b200moe_linear(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs,
+                               int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ld_w, const float* w_scale,
+                               const void* residual, int64_t ld_res, void* out, int64_t ld_out, int out_f32,
+                               void* workspace, size_t workspace_bytes, int32_t* err_word, void* stream);
+B200MOE_API int b200moe_gate_up(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs,
+                                int64_t M, int64_t H, int64_t I, const uint8_t* w13, int64_t ld_w,
+                                const float* w13_scale, uint8_t* q, int64_t ld_q, float* s, int64_t ld_s,
+                                void* workspace, size_t workspace_bytes, int32_t* err_word, void* stream);
+B200MOE_API size_t b200moe_mlp_workspace_size(int64_t M, int64_t H, int64_t I);
+B200MOE_API int b200moe_mlp(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs,
+                            int64_t M, int64_t H, int64_t I, const uint8_t* w13, const float* w13_scale,
+                            const uint8_t* w2, const float* w2_scale, const void* residual, int64_t ld_res, void* out,
+                            int64_t ld_out, void* workspace, size_t workspace_bytes, int32_t* err_word, void* stream);
 
 /* ------------------------------------------------------------------------
  * Diagnostics.

@@ -1,0 +1,124 @@
+"""Refusals of the dense FP8 products (fp8_block_linear, fp8_gate_up, fp8_mlp):
+checked on the host before anything is launched, so no GPU is needed."""
+import pytest
+import torch
+
+from trials_b200 import _lib, dense, fp8_block_linear, fp8_gate_up, fp8_mlp
+
+P = 256  # a non-null, aligned address that no refused call touches
+FP8 = torch.float8_e4m3fn
+
+
+def linear(x=P, xq=None, xs=None, ld_x=256, ld_xs=2, M=4, N=100, K=256, w=P, ld_w=256, ws=P, res=None, ld_res=0,
+           out=P, ld_out=100, f32=0, work=P, nwork=1 << 20, err=P):
+    return _lib.lib().b200moe_linear(x, xq, xs, ld_x, ld_xs, M, N, K, w, ld_w, ws, res, ld_res, out, ld_out, f32, work,
+                                     nwork, err, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(M=-1), dict(N=0), dict(K=0), dict(w=None), dict(ws=None), dict(err=None), dict(ld_w=128), dict(x=None),
+    dict(xq=P, xs=P), dict(x=None, xq=P), dict(x=None, xq=P, xs=P, ld_xs=1), dict(ld_x=128), dict(out=None),
+    dict(ld_out=99), dict(res=P, ld_res=99)])
+def test_linear_invalid_arguments(kw):
+    assert linear(**kw) == _lib.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("kw", [
+    dict(K=200, ld_x=256, ld_w=256), dict(w=P + 8), dict(ld_w=264), dict(x=P + 8), dict(ld_x=260),
+    dict(x=None, xq=P, xs=P, ld_x=264), dict(out=P + 1), dict(f32=1, out=P + 2), dict(M=(1 << 30) + 1),
+    dict(N=(1 << 24) + 1, ld_out=1 << 25)])
+def test_linear_unsupported_layouts(kw):
+    assert linear(**kw) == _lib.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("kw", [dict(work=None), dict(nwork=100), dict(work=P + 16)])
+def test_linear_workspace(kw):
+    assert linear(**kw) == _lib.ERR_WORKSPACE
+
+
+def test_empty_batches_launch_nothing():
+    L = _lib.lib()
+    assert linear(M=0, x=None, out=None, work=None, nwork=0) == _lib.OK
+    assert L.b200moe_gate_up(None, None, None, 0, 0, 0, 256, 128, P, 256, P, None, 0, None, 0, None, 0, P,
+                             None) == _lib.OK
+    assert L.b200moe_mlp(None, None, None, 0, 0, 0, 256, 128, P, P, P, P, None, 0, None, 0, None, 0, P,
+                         None) == _lib.OK
+    assert L.b200moe_linear_workspace_size(0, 256) == 0 and L.b200moe_mlp_workspace_size(0, 256, 128) == 0
+
+
+def test_gate_up_and_mlp_host_checks():
+    L = _lib.lib()
+
+    def gate_up(I=128, q=P, ld_q=128, s=P, ld_s=1, H=256):
+        return L.b200moe_gate_up(P, None, None, 256, 0, 4, H, I, P, 256, P, q, ld_q, s, ld_s, P, 1 << 20, P, None)
+
+    assert gate_up(I=0) == _lib.ERR_INVALID_ARG
+    assert gate_up(q=None) == _lib.ERR_INVALID_ARG
+    assert gate_up(ld_q=64) == _lib.ERR_INVALID_ARG
+    assert gate_up(I=64, ld_q=64) == _lib.ERR_UNSUPPORTED
+    assert gate_up(q=P + 8) == _lib.ERR_UNSUPPORTED
+    assert gate_up(H=384) == _lib.ERR_INVALID_ARG  # row stride 256 is shorter than a row
+
+    def mlp(I=128, w2=P, out=P, nwork=1 << 20, res=None):
+        return L.b200moe_mlp(P, None, None, 256, 0, 4, 256, I, P, P, w2, P, res, 0, out, 256, P, nwork, P, None)
+
+    assert mlp(I=0) == _lib.ERR_INVALID_ARG
+    assert mlp(I=192) == _lib.ERR_UNSUPPORTED
+    assert mlp(w2=None) == _lib.ERR_INVALID_ARG
+    assert mlp(w2=P + 8) == _lib.ERR_UNSUPPORTED
+    assert mlp(res=P) == _lib.ERR_INVALID_ARG  # residual without a stride
+    assert mlp(nwork=L.b200moe_mlp_workspace_size(4, 256, 128) - 1) == _lib.ERR_WORKSPACE
+
+
+def test_workspace_sizes_cover_codes_and_scales():
+    L = _lib.lib()
+    assert L.b200moe_linear_workspace_size(3, 384) >= 3 * 384 + 3 * 3 * 4
+    assert L.b200moe_mlp_workspace_size(3, 384, 128) >= 3 * 384 + 3 * 3 * 4 + 3 * 128 + 3 * 4
+
+
+def test_python_ops_refuse_cpu_tensors():
+    x = torch.zeros(2, 256, dtype=torch.bfloat16)
+    w = torch.zeros(256, 256).to(FP8)
+    s = torch.ones(2, 2)
+    for call in (lambda: fp8_block_linear(x, w, s), lambda: fp8_gate_up(x, w, s), lambda: fp8_mlp(x, w, s, w, s)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+# The Python checks behind the device check, on CPU tensors.
+def test_python_input_checks():
+    bf, q, s = torch.zeros(3, 256, dtype=torch.bfloat16), torch.zeros(3, 256).to(FP8), torch.ones(3, 2)
+    assert dense._input(bf, None)[0] is bf and dense._input(q, s)[1] is s
+    for bad in ((bf, s), (q, None), (q, s[:2]), (q, s[:, :1]), (bf[0], None)):
+        with pytest.raises(ValueError):
+            dense._input(*bad)
+    for bad in ((bf.float(), None), (bf.half(), None), (q, s.double()), (bf[:, :200], None), (bf[:, :0], None)):
+        with pytest.raises(NotImplementedError):
+            dense._input(*bad)
+    # layouts that the kernels cannot read are copied
+    for odd in (bf.t().contiguous().t(), torch.zeros(3, 260, dtype=torch.bfloat16)[:, :256],
+                torch.zeros(3 * 256 + 1, dtype=torch.bfloat16)[1:].view(3, 256), bf[:1].expand(3, 256)):
+        got = dense._input(odd, None)[0]
+        assert got is not odd and got.is_contiguous() and torch.equal(got, odd)
+    strided = torch.zeros(3, 512, dtype=torch.bfloat16)[:, :256]
+    assert dense._input(strided, None)[0] is strided
+
+
+def test_python_weight_and_output_checks():
+    w, s = torch.zeros(200, 256).to(FP8), torch.ones(2, 2)
+    assert dense._weight(w, s, 256, "weight")[0] == 256
+    for bad in ((w, s[:1]), (w[:, :128], s), (w[:0], s[:0]), (w.view(10, 20, 256), s)):
+        with pytest.raises(ValueError):
+            dense._weight(*bad, 256, "weight")
+    with pytest.raises(ValueError):  # transposed storage
+        dense._weight(torch.zeros(256, 256).to(FP8).t(), s, 256, "weight")
+    for bad in ((w.float(), s), (w, s.double())):
+        with pytest.raises(NotImplementedError):
+            dense._weight(*bad, 256, "weight")
+    out = torch.zeros(3, 5, dtype=torch.bfloat16)
+    assert dense._output(out, out, 3, 5, torch.bfloat16, out.device) == (out, out)
+    for o, r in ((out[:2], None), (out.float(), None), (None, out[:, :4])):
+        with pytest.raises(ValueError):
+            dense._output(o, r, 3, 5, torch.bfloat16, out.device)
+    with pytest.raises(NotImplementedError):
+        dense._output(None, out.float(), 3, 5, torch.bfloat16, out.device)

@@ -4,6 +4,7 @@ Hand-written sm_100a CUDA kernels (TMA + tcgen05/TMEM grouped GEMMs, warp-scan
 routing, fused quantisation) behind a C ABI (include/b200moe.h), with a Python
 surface that mirrors the reference's drop-in calls.
 """
+from .dense import fp8_block_linear, fp8_gate_up, fp8_mlp  # noqa: F401
 from .moe import (  # noqa: F401
     ActivationType,
     QuantType,

@@ -11,6 +11,7 @@
 #include <mutex>
 
 #include "../../include/b200moe.h"
+#include "dense.h"
 #include "launch.h"
 #include "moe_gemm.cuh"
 #include "router.cuh"
@@ -55,13 +56,14 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// 2D byte matrix [rows][cols] (row pitch = cols), box = 128 bytes x box_rows,
-// 128-byte swizzle (the K-major canonical layout of the tcgen05 descriptors).
-int make_tmap_u8(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_rows) {
+// 2D byte matrix [rows][cols] (row pitch = ld bytes, 0: cols), box = 128 bytes
+// x box_rows, 128-byte swizzle (the K-major canonical layout of the tcgen05
+// descriptors).
+int make_tmap_u8(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_rows, int64_t ld = 0) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(B200MOE_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable%s");
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)cols};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld > 0 ? ld : cols)};
   cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1u, 1u};
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
@@ -365,9 +367,9 @@ int b200moe_quant_1x128(const void* x, int64_t M, int64_t K, int64_t ldx, uint8_
 }
 
 int b200moe_quant_block128(const void* w, int64_t E, int64_t N, int64_t K, uint8_t* q, float* s, void* stream) {
-  if (E < 0 || N <= 0 || K <= 0 || N % 128 != 0 || K % 128 != 0 || (E > 0 && (!w || !q || !s)))
+  if (E < 0 || N <= 0 || K <= 0 || K % 128 != 0 || (E > 0 && (!w || !q || !s)))
     return fail(B200MOE_ERR_INVALID_ARG, "b200moe_quant_block128: bad argument%s");
-  if (!aligned16(w) || !aligned16(q) || E > 65535 || N / 128 > 65535)
+  if (!aligned16(w) || !aligned16(q) || E > 65535 || ceil_div(N, 128) > 65535)
     return fail(B200MOE_ERR_UNSUPPORTED, "b200moe_quant_block128: alignment or size%s");
   return cuda_status(launch_quant_block128(w, E, N, K, q, s, (cudaStream_t)stream), "quant_block128");
 }
@@ -1377,6 +1379,181 @@ int b200moe_router_topk(const void* logits, int logits_bf16, int64_t M, int num_
   return cuda_status(launch_router_topk(logits, logits_bf16, M, num_experts, topk, scoring, correction_bias,
                                         renormalize, scaling, topk_weights, topk_ids, (cudaStream_t)stream),
                      "router_topk");
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Dense (not expert-grouped) FP8 block-scaled products.
+// ---------------------------------------------------------------------------
+namespace {
+
+// The activation rows of a dense product: bf16 (quantised into the workspace
+// first) or fp8 with 1x128 scales.
+struct DenseInput {
+  const void* x;
+  const uint8_t* q;
+  const float* s;
+  int64_t ld_x, ld_s;
+};
+
+int check_dense(const char* name, const DenseInput& in, int64_t M, int64_t N, int64_t K, const uint8_t* w,
+                int64_t ld_w, const float* w_scale, const int32_t* err_word) {
+  if (M < 0 || N <= 0 || K <= 0 || !w || !w_scale || !err_word || ld_w < K)
+    return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
+  if (M > 0 && ((in.x != nullptr) == (in.q != nullptr) || (in.q && !in.s)))
+    return fail(B200MOE_ERR_INVALID_ARG, "%s: pass either bf16 rows or fp8 rows with their scales", name);
+  if (M > 0 && (in.ld_x < K || (in.q && in.ld_s < K / 128)))
+    return fail(B200MOE_ERR_INVALID_ARG, "%s: row stride shorter than a row", name);
+  if (K % 128 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "%s: K must be a multiple of 128", name);
+  if (M > (1 << 30) || N > (1 << 24) || K > (1 << 20))
+    return fail(B200MOE_ERR_UNSUPPORTED, "%s: dimension too large", name);
+  if (!aligned16(w) || ld_w % 16 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "%s: weight rows must be 16-byte aligned", name);
+  const bool rows_ok = in.x ? (aligned16(in.x) && in.ld_x % 8 == 0) : (aligned16(in.q) && in.ld_x % 16 == 0);
+  if (M > 0 && !rows_ok) return fail(B200MOE_ERR_UNSUPPORTED, "%s: activation rows must be 16-byte aligned", name);
+  return B200MOE_OK;
+}
+
+size_t dense_quant_bytes(int64_t M, int64_t K) {
+  return (size_t)round_up(M * K, 256) + (size_t)round_up(M * (K / 128) * 4, 256);
+}
+
+// bf16 rows -> fp8 rows in ws (dense_quant_bytes); fp8 rows stay as they are.
+int dense_quantise(DenseInput& in, int64_t M, int64_t K, uint8_t* ws, void* stream) {
+  if (!in.x) return B200MOE_OK;
+  uint8_t* q = ws;
+  float* s = reinterpret_cast<float*>(ws + round_up(M * K, 256));
+  const int st = b200moe_quant_1x128(in.x, M, K, in.ld_x, q, K, s, K / 128, 1, stream);
+  if (st) return st;
+  in = DenseInput{nullptr, q, s, K, K / 128};
+  return B200MOE_OK;
+}
+
+// One product of quantised rows; the output fields of p are set by the caller.
+int run_dense(const char* name, int epi, const DenseInput& in, int64_t M, int64_t N, int64_t K, const uint8_t* w,
+              int64_t ld_w, const float* w_scale, DenseParams p, int32_t* err_word, void* stream) {
+  const DensePlan pl = dense_plan(epi, M, N, K);
+  CUtensorMap tm_x, tm_w;
+  int st = make_tmap_u8(&tm_x, in.q, M, K, pl.x_box_rows, in.ld_x);
+  if (st) return st;
+  st = make_tmap_u8(&tm_w, w, N, K, pl.w_box_rows, ld_w);
+  if (st) return st;
+  p.xs = in.s;
+  p.ld_xs = in.ld_s;
+  p.ws = w_scale;
+  p.M = (int)M;
+  p.N = (int)N;
+  p.K = (int)K;
+  p.err = err_word;
+  p.timeout_ns = kTimeoutNs;
+  return cuda_status(launch_dense(epi, pl, tm_x, tm_w, p, (cudaStream_t)stream), name);
+}
+
+int check_dense_out(const char* name, int64_t M, int64_t N, const void* residual, int64_t ld_res, const void* out,
+                    int64_t ld_out, int out_f32, DenseParams& p) {
+  if (M > 0 && (!out || ld_out < N || (residual && ld_res < N)))
+    return fail(B200MOE_ERR_INVALID_ARG, "%s: bad output or residual", name);
+  const int64_t esize = out_f32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(out) % esize != 0 || (reinterpret_cast<uintptr_t>(residual) & 1) != 0)
+    return fail(B200MOE_ERR_UNSUPPORTED, "%s: misaligned output or residual", name);
+  p.out = const_cast<void*>(out);
+  p.ld_out = ld_out;
+  p.out_f32 = out_f32 ? 1 : 0;
+  p.residual = residual;
+  p.ld_res = ld_res;
+  p.vec = N % 8 == 0 && aligned16(out) && (ld_out * esize) % 16 == 0 &&
+          (!residual || (aligned16(residual) && ld_res % 8 == 0));
+  return B200MOE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t b200moe_linear_workspace_size(int64_t M, int64_t K) { return M > 0 && K > 0 ? dense_quant_bytes(M, K) : 0; }
+
+int b200moe_linear(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs, int64_t M,
+                   int64_t N, int64_t K, const uint8_t* w, int64_t ld_w, const float* w_scale, const void* residual,
+                   int64_t ld_res, void* out, int64_t ld_out, int out_f32, void* workspace, size_t workspace_bytes,
+                   int32_t* err_word, void* stream) {
+  DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
+  int st = check_dense("b200moe_linear", in, M, N, K, w, ld_w, w_scale, err_word);
+  if (st) return st;
+  DenseParams p{};
+  st = check_dense_out("b200moe_linear", M, N, residual, ld_res, out, ld_out, out_f32, p);
+  if (st) return st;
+  if (M == 0) return B200MOE_OK;
+  if (x && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
+            workspace_bytes < dense_quant_bytes(M, K)))
+    return fail(B200MOE_ERR_WORKSPACE, "b200moe_linear: workspace too small or not 256-byte aligned%s");
+  st = dense_quantise(in, M, K, static_cast<uint8_t*>(workspace), stream);
+  if (st) return st;
+  return run_dense("b200moe_linear", DENSE_OUT, in, M, N, K, w, ld_w, w_scale, p, err_word, stream);
+}
+
+int b200moe_gate_up(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs, int64_t M,
+                    int64_t H, int64_t I, const uint8_t* w13, int64_t ld_w, const float* w13_scale, uint8_t* q,
+                    int64_t ld_q, float* s, int64_t ld_s, void* workspace, size_t workspace_bytes, int32_t* err_word,
+                    void* stream) {
+  DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
+  if (I <= 0 || I > (1 << 23)) return fail(B200MOE_ERR_INVALID_ARG, "b200moe_gate_up: bad argument%s");
+  int st = check_dense("b200moe_gate_up", in, M, 2 * I, H, w13, ld_w, w13_scale, err_word);
+  if (st) return st;
+  if (M > 0 && (!q || !s || ld_q < I || ld_s < I / 128))
+    return fail(B200MOE_ERR_INVALID_ARG, "b200moe_gate_up: bad output%s");
+  if (I % 128 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "b200moe_gate_up: I must be a multiple of 128%s");
+  if (!aligned16(q) || ld_q % 16 != 0)
+    return fail(B200MOE_ERR_UNSUPPORTED, "b200moe_gate_up: output rows must be 16-byte aligned%s");
+  if (M == 0) return B200MOE_OK;
+  if (x && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
+            workspace_bytes < dense_quant_bytes(M, H)))
+    return fail(B200MOE_ERR_WORKSPACE, "b200moe_gate_up: workspace too small or not 256-byte aligned%s");
+  st = dense_quantise(in, M, H, static_cast<uint8_t*>(workspace), stream);
+  if (st) return st;
+  DenseParams p{};
+  p.q = q;
+  p.ld_q = ld_q;
+  p.s = s;
+  p.ld_s = ld_s;
+  return run_dense("b200moe_gate_up", DENSE_SILU, in, M, 2 * I, H, w13, ld_w, w13_scale, p, err_word, stream);
+}
+
+size_t b200moe_mlp_workspace_size(int64_t M, int64_t H, int64_t I) {
+  return M > 0 && H > 0 && I > 0 ? dense_quant_bytes(M, H) + dense_quant_bytes(M, I) : 0;
+}
+
+int b200moe_mlp(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs, int64_t M,
+                int64_t H, int64_t I, const uint8_t* w13, const float* w13_scale, const uint8_t* w2,
+                const float* w2_scale, const void* residual, int64_t ld_res, void* out, int64_t ld_out,
+                void* workspace, size_t workspace_bytes, int32_t* err_word, void* stream) {
+  DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
+  if (I <= 0 || I > (1 << 20)) return fail(B200MOE_ERR_INVALID_ARG, "b200moe_mlp: bad argument%s");
+  int st = check_dense("b200moe_mlp", in, M, 2 * I, H, w13, H, w13_scale, err_word);
+  if (st) return st;
+  if (I % 128 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "b200moe_mlp: I must be a multiple of 128%s");
+  if (!w2 || !w2_scale) return fail(B200MOE_ERR_INVALID_ARG, "b200moe_mlp: bad argument%s");
+  if (!aligned16(w2)) return fail(B200MOE_ERR_UNSUPPORTED, "b200moe_mlp: weight rows must be 16-byte aligned%s");
+  DenseParams p{};
+  st = check_dense_out("b200moe_mlp", M, H, residual, ld_res, out, ld_out, 0, p);
+  if (st) return st;
+  if (M == 0) return B200MOE_OK;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
+      workspace_bytes < b200moe_mlp_workspace_size(M, H, I))
+    return fail(B200MOE_ERR_WORKSPACE, "b200moe_mlp: workspace too small or not 256-byte aligned%s");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  st = dense_quantise(in, M, H, ws, stream);
+  if (st) return st;
+  uint8_t* iq = ws + dense_quant_bytes(M, H);
+  float* is = reinterpret_cast<float*>(iq + round_up(M * I, 256));
+  DenseParams g{};
+  g.q = iq;
+  g.ld_q = I;
+  g.s = is;
+  g.ld_s = I / 128;
+  st = run_dense("b200moe_mlp", DENSE_SILU, in, M, 2 * I, H, w13, H, w13_scale, g, err_word, stream);
+  if (st) return st;
+  const DenseInput mid{nullptr, iq, is, I, I / 128};
+  return run_dense("b200moe_mlp", DENSE_OUT, mid, M, H, I, w2, I, w2_scale, p, err_word, stream);
 }
 
 int b200moe_read_error(int32_t* err_word, int32_t* value, int clear, void* stream) {

@@ -36,7 +36,8 @@ cudaError_t launch_quant_1x128(const QuantArgs& a, cudaStream_t stream) {
 // ---------------------------------------------------------------------------
 // 128 x 128 block quantisation of weights (per_block_quant_fp8,
 // phase5_orchestrator.py:35-41). One CTA of 256 threads per block; thread t
-// owns row t/2, columns (t%2)*64 .. +64.
+// owns row t/2, columns (t%2)*64 .. +64. The last block of a weight whose rows
+// are no multiple of 128 covers the rows that exist.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) quant_block128_kernel(const __nv_bfloat16* __restrict__ w, int64_t N,
                                                              int64_t K, uint8_t* __restrict__ q,
@@ -46,10 +47,11 @@ __global__ void __launch_bounds__(256) quant_block128_kernel(const __nv_bfloat16
   const int64_t e = blockIdx.z;
   const int r = threadIdx.x >> 1, half = threadIdx.x & 1;
   const int64_t off = (e * N + (int64_t)nb * 128 + r) * K + (int64_t)kb * 128 + half * 64;
+  const bool exists = (int64_t)nb * 128 + r < N;
   float v[64];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(w + off) + i);
+    const uint4 raw = exists ? __ldg(reinterpret_cast<const uint4*>(w + off) + i) : make_uint4(0, 0, 0, 0);
     const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -79,15 +81,15 @@ __global__ void __launch_bounds__(256) quant_block128_kernel(const __nv_bfloat16
       for (int t = 0; t < 4; ++t) b |= (uint32_t)quant_e4m3(v[i * 16 + k * 4 + t], scale) << (8 * t);
       word[k] = b;
     }
-    *reinterpret_cast<uint4*>(q + off + i * 16) = make_uint4(word[0], word[1], word[2], word[3]);
+    if (exists) *reinterpret_cast<uint4*>(q + off + i * 16) = make_uint4(word[0], word[1], word[2], word[3]);
   }
-  if (threadIdx.x == 0) s[(e * (N / 128) + nb) * (K / 128) + kb] = scale;
+  if (threadIdx.x == 0) s[(e * ((N + 127) / 128) + nb) * (K / 128) + kb] = scale;
 }
 
 cudaError_t launch_quant_block128(const void* w, int64_t E, int64_t N, int64_t K, uint8_t* q, float* s,
                                   cudaStream_t stream) {
   if (E <= 0) return cudaSuccess;
-  dim3 grid((unsigned)(K / 128), (unsigned)(N / 128), (unsigned)E);
+  dim3 grid((unsigned)(K / 128), (unsigned)((N + 127) / 128), (unsigned)E);
   quant_block128_kernel<<<grid, 256, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(w), N, K, q, s);
   return cudaGetLastError();
 }

@@ -60,7 +60,11 @@ class _Workspaces:
         self._lock = threading.Lock()
 
     def get(self, device: torch.device, nbytes: int) -> torch.Tensor:
-        key = (device.index, _stream(device))
+        return self.get_for(device, _stream(device), nbytes)
+
+    def get_for(self, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+        """The buffer of (device, stream), `stream` being the device's current one."""
+        key = (device.index, stream)
         with self._lock:
             buf = self._bufs.get(key)
             if buf is None or buf.numel() < nbytes:
@@ -157,16 +161,21 @@ def per_token_group_quant_fp8(x: torch.Tensor, group_size: int = 128):
 
 
 def per_block_quant_fp8(w: torch.Tensor, bn: int = 128, bk: int = 128):
-    """(E, N, K) bf16 -> (q e4m3 (E, N, K), s f32 (E, N/128, K/128))."""
+    """(E, N, K) bf16 -> (q e4m3 (E, N, K), s f32 (E, ceil(N/128), K/128)); a 2-D
+    (N, K) weight -> 2-D q and s. The last block of an N that is no multiple of
+    128 covers the rows that exist."""
     if bn != 128 or bk != 128:
         raise NotImplementedError("only 128x128 blocks are supported")
     dev = _require_cuda(w)
     if w.dtype != torch.bfloat16:
         raise NotImplementedError("per_block_quant_fp8 takes bf16 input")
+    if w.dim() == 2:
+        q, s = per_block_quant_fp8(w.unsqueeze(0), bn, bk)
+        return q[0], s[0]
     w = w.contiguous()
     E, N, K = w.shape
     q = torch.empty(E, N, K, dtype=FP8, device=dev)
-    s = torch.empty(E, N // 128, K // 128, dtype=torch.float32, device=dev)
+    s = torch.empty(E, (N + 127) // 128, K // 128, dtype=torch.float32, device=dev)
     _lib.check(_lib.lib().b200moe_quant_block128(_ptr(w), E, N, K, _ptr(q), _ptr(s), _stream(dev)),
                "per_block_quant_fp8")
     return q, s
