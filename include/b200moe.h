@@ -98,6 +98,24 @@ B200MOE_API int b200moe_router_topk(const void* logits, int logits_bf16, int64_t
                                     int scoring, const float* correction_bias, int renormalize, float scaling,
                                     float* topk_weights, int32_t* topk_ids, void* stream);
 
+/* Group-limited routing: the experts form num_groups equal runs of consecutive
+ * ids, and only those of the topk_groups best groups can be selected. With
+ * c = sigmoid + correction_bias (scoring 1 and a bias) a group's score is the
+ * sum of its two largest c, otherwise its largest logit; then the top-k c
+ * (logits) inside the selected groups, equal values broken by the lower index
+ * for groups and experts alike. Weights as above. The selection is the one
+ * that exact arithmetic on the given values makes. NaN logits count as -inf
+ * (score 0; without a bias selected last, in id order); a +inf logit of a
+ * softmax shares the whole weight with its equals; when renormalize is set and
+ * the selected scores sum to 0, the weights are 0. num_experts % num_groups
+ * == 0, topk <= topk_groups * num_experts / num_groups, at most 32 groups. The
+ * reference runs one group (measure_xcd_imbalance.py:50-55); more are what
+ * other checkpoints of this layer's geometries route with. */
+B200MOE_API int b200moe_router_topk_grouped(const void* logits, int logits_bf16, int64_t M, int num_experts,
+                                            int num_groups, int topk_groups, int topk, int scoring,
+                                            const float* correction_bias, int renormalize, float scaling,
+                                            float* topk_weights, int32_t* topk_ids, void* stream);
+
 /* ------------------------------------------------------------------------
  * Activation quantisation: per_token_group_quant_fp8(x, 128).
  * Replaces sglang's per_token_group_quant_fp8 called at
@@ -184,6 +202,19 @@ B200MOE_API int b200moe_layer_logits(const void* hidden, int64_t M, int64_t H, i
                                      const float* w2_scale, const int32_t* expert_map, int num_local_experts,
                                      float* topk_weights, int32_t* topk_ids, void* out, void* workspace,
                                      size_t workspace_bytes, void* stream);
+
+/* b200moe_layer_logits with the router of b200moe_router_topk_grouped, equal to
+ * it followed by b200moe_layer bit for bit. Launches as b200moe_layer_logits,
+ * except that the one-launch layer has the router in front as a launch of its
+ * own. */
+B200MOE_API int b200moe_layer_logits_grouped(const void* hidden, int64_t M, int64_t H, int64_t I, int num_experts,
+                                             int topk, const void* router_logits, int logits_bf16, int num_groups,
+                                             int topk_groups, int scoring, const float* correction_bias,
+                                             int renormalize, float scaling, const uint8_t* w13,
+                                             const float* w13_scale, const uint8_t* w2, const float* w2_scale,
+                                             const int32_t* expert_map, int num_local_experts, float* topk_weights,
+                                             int32_t* topk_ids, void* out, void* workspace, size_t workspace_bytes,
+                                             void* stream);
 
 /* Same layer with pre-quantised activations: hidden_q (M, H) fp8 e4m3 and
  * hidden_scale (M, H/128) f32 from a 1x128 per-token-group quantisation. This
@@ -405,6 +436,18 @@ B200MOE_API int b200moe_route_logits(const void* logits, int logits_bf16, int64_
                                      int32_t* num_rows, int32_t* slot_pos, int32_t* chunk_ready,
                                      int32_t* route_scratch, int64_t route_scratch_ints, int32_t* err_word,
                                      void* stream);
+
+/* b200moe_route_logits with the router of b200moe_router_topk_grouped. */
+B200MOE_API int b200moe_route_logits_grouped(const void* logits, int logits_bf16, int64_t M, int num_experts,
+                                             int num_groups, int topk_groups, int topk, int scoring,
+                                             const float* correction_bias, int renormalize, float scaling,
+                                             float* topk_weights, int32_t* topk_ids, const int32_t* expert_map,
+                                             int num_local_experts, int tile_tokens, int32_t* sorted_ids,
+                                             int64_t rows_capacity, int32_t* chunk_expert, int32_t* chunk_row0,
+                                             int32_t* chunk_rows, int64_t chunks_capacity, int32_t* n_chunks,
+                                             int32_t* num_rows, int32_t* slot_pos, int32_t* chunk_ready,
+                                             int32_t* route_scratch, int64_t route_scratch_ints, int32_t* err_word,
+                                             void* stream);
 
 /* Quantise hidden rows into the sorted layout: for every flat slot f with
  * p = slot_pos[f] >= 0 (from b200moe_route), row p of a_q (ld = H) holds

@@ -38,6 +38,7 @@ SIGNATURES = {
     "b200moe_align_capacity_blocks": (_L, [_L, _I, _I]),
     "b200moe_align": (_I, [_P, _L, _I, _I, _I, _P, _I, _P, _L, _P, _L, _P, _P, _P]),
     "b200moe_router_topk": (_I, [_P, _I, _L, _I, _I, _I, _P, _I, ctypes.c_float, _P, _P, _P]),
+    "b200moe_router_topk_grouped": (_I, [_P, _I, _L, _I, _I, _I, _I, _I, _P, _I, ctypes.c_float, _P, _P, _P]),
     "b200moe_quant_1x128": (_I, [_P, _L, _L, _L, _P, _L, _P, _L, _L, _P]),
     "b200moe_quant_block128": (_I, [_P, _L, _L, _L, _P, _P, _P]),
     "b200moe_layer_workspace_size": (_S, [_L, _L, _L, _I, _I, _I]),
@@ -46,6 +47,8 @@ SIGNATURES = {
     "b200moe_layer": (_I, [_P, _L, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _S, _P]),
     "b200moe_layer_logits": (_I, [_P, _L, _L, _L, _I, _I, _P, _I, _I, _P, _I, ctypes.c_float, _P, _P, _P, _P, _P, _I,
                                   _P, _P, _P, _P, _S, _P]),
+    "b200moe_layer_logits_grouped": (_I, [_P, _L, _L, _L, _I, _I, _P, _I, _I, _I, _I, _P, _I, ctypes.c_float, _P, _P,
+                                          _P, _P, _P, _I, _P, _P, _P, _P, _S, _P]),
     "b200moe_layer_quantized": (_I, [_P, _P, _L, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _S, _P]),
     "b200moe_ep_row_bytes": (_L, [_L, _I]),
     "b200moe_ep_dispatch": (_I, [_P, _P, _P, _P, _L, _L, _I, _I, _I, _I, _P, _I, _I, _L, _P, _P, _P, _P, _P, _P]),
@@ -74,6 +77,8 @@ SIGNATURES = {
     "b200moe_route_logits_scratch_ints": (_L, [_L, _I]),
     "b200moe_route_logits": (_I, [_P, _I, _L, _I, _I, _I, _P, _I, ctypes.c_float, _P, _P, _P, _I, _I, _P, _L, _P, _P,
                                   _P, _L, _P, _P, _P, _P, _P, _L, _P, _P]),
+    "b200moe_route_logits_grouped": (_I, [_P, _I, _L, _I, _I, _I, _I, _I, _P, _I, ctypes.c_float, _P, _P, _P, _I, _I,
+                                          _P, _L, _P, _P, _P, _L, _P, _P, _P, _P, _P, _L, _P, _P]),
     "b200moe_gather_quant": (_I, [_P, _L, _L, _I, _P, _L, _P, _P, _L, _P]),
     "b200moe_gather_rows": (_I, [_P, _P, _L, _L, _L, _L, _I, _P, _L, _P, _P, _L, _P]),
     "b200moe_gemm1_silu": (_I, [_P, _P, _L, _L, _P, _P, _I, _L, _L, _P, _P, _P, _P, _L, _I, _P, _P, _P, _I, _P]),

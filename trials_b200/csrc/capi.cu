@@ -283,6 +283,20 @@ int check_router(const char* name, const void* logits, int64_t M, int num_expert
   return B200MOE_OK;
 }
 
+// The same plus the groups of group-limited routing.
+int check_router_grouped(const char* name, const void* logits, int64_t M, int num_experts, int num_groups,
+                         int topk_groups, int topk, int scoring, const float* correction_bias,
+                         const float* topk_weights, const int32_t* topk_ids) {
+  const int st = check_router(name, logits, M, num_experts, topk, scoring, correction_bias, topk_weights, topk_ids);
+  if (st) return st;
+  if (num_groups <= 0 || num_experts % num_groups != 0 || topk_groups <= 0 || topk_groups > num_groups ||
+      topk > topk_groups * (num_experts / num_groups))
+    return fail(B200MOE_ERR_INVALID_ARG, "%s: groups must split the experts evenly and the selected ones hold top-k",
+                name);
+  if (num_groups > kRouterMaxGroups) return fail(B200MOE_ERR_UNSUPPORTED, "%s: at most 32 groups", name);
+  return B200MOE_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -555,6 +569,24 @@ int b200moe_route_logits(const void* logits, int logits_bf16, int64_t M, int num
   if (st) return st;
   const RouterArgs r{logits, logits_bf16 ? 1 : 0, num_experts, topk, scoring, renormalize ? 1 : 0,
                      correction_bias, scaling, topk_weights, topk_ids};
+  return route_impl(topk_ids, M, topk, num_experts, expert_map, num_local_experts, tile_tokens, sorted_ids,
+                    rows_capacity, chunk_expert, chunk_row0, chunk_rows, chunks_capacity, n_chunks, num_rows,
+                    slot_pos, chunk_ready, route_scratch, route_scratch_ints, err_word, stream, &r, nullptr);
+}
+
+int b200moe_route_logits_grouped(const void* logits, int logits_bf16, int64_t M, int num_experts, int num_groups,
+                                 int topk_groups, int topk, int scoring, const float* correction_bias,
+                                 int renormalize, float scaling, float* topk_weights, int32_t* topk_ids,
+                                 const int32_t* expert_map, int num_local_experts, int tile_tokens,
+                                 int32_t* sorted_ids, int64_t rows_capacity, int32_t* chunk_expert,
+                                 int32_t* chunk_row0, int32_t* chunk_rows, int64_t chunks_capacity, int32_t* n_chunks,
+                                 int32_t* num_rows, int32_t* slot_pos, int32_t* chunk_ready, int32_t* route_scratch,
+                                 int64_t route_scratch_ints, int32_t* err_word, void* stream) {
+  int st = check_router_grouped("b200moe_route_logits_grouped", logits, M, num_experts, num_groups, topk_groups, topk,
+                                scoring, correction_bias, topk_weights, topk_ids);
+  if (st) return st;
+  const RouterArgs r{logits,  logits_bf16 ? 1 : 0, num_experts, topk, scoring, renormalize ? 1 : 0, correction_bias,
+                     scaling, topk_weights,        topk_ids,    num_groups, topk_groups};
   return route_impl(topk_ids, M, topk, num_experts, expert_map, num_local_experts, tile_tokens, sorted_ids,
                     rows_capacity, chunk_expert, chunk_row0, chunk_rows, chunks_capacity, n_chunks, num_rows,
                     slot_pos, chunk_ready, route_scratch, route_scratch_ints, err_word, stream, &r, nullptr);
@@ -1040,9 +1072,17 @@ int layer_core(const char* name, const LayerInput& in, int64_t M, int64_t H, int
   // workspace header (zeroed with the error word; every call leaves it zero).
   // Mixed work lists (decode batches with heavy experts): counts[2] = heavy
   // chunks, counts[3] = first heavy row.
-  if (whole_layer_for(M, M * topk, pl.tile_tokens, pl.heavy_rows, peer_out != nullptr))
+  if (whole_layer_for(M, M * topk, pl.tile_tokens, pl.heavy_rows, peer_out != nullptr)) {
+    // The group-limited router is not part of the one-launch layer: it runs as
+    // a launch of its own in front of it.
+    if (router && router->groups > 0) {
+      st = cuda_status(launch_router_topk(*router, M, (cudaStream_t)stream), name);
+      if (st) return st;
+      router = nullptr;
+    }
     return whole_layer(name, in, M, H, I, num_experts, topk, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids,
                        expert_map, E, out, pl, wl, err, router, stream);
+  }
   MixedLists mx{};
   if (pl.heavy_rows) {
     mx = MixedLists{pl.heavy_rows, reinterpret_cast<int32_t*>(wl + pl.off_ce2),
@@ -1121,6 +1161,24 @@ int b200moe_layer_logits(const void* hidden, int64_t M, int64_t H, int64_t I, in
                      correction_bias, scaling, topk_weights, topk_ids};
   LayerInput in{hidden, nullptr, 0, nullptr, 0};
   return layer_core("b200moe_layer_logits", in, M, H, I, num_experts, topk, w13, w13_scale, w2, w2_scale,
+                    topk_weights, topk_ids, expert_map, num_local_experts, out, workspace, workspace_bytes, 0, stream,
+                    nullptr, nullptr, -1, &r);
+}
+
+int b200moe_layer_logits_grouped(const void* hidden, int64_t M, int64_t H, int64_t I, int num_experts, int topk,
+                                 const void* router_logits, int logits_bf16, int num_groups, int topk_groups,
+                                 int scoring, const float* correction_bias, int renormalize, float scaling,
+                                 const uint8_t* w13, const float* w13_scale, const uint8_t* w2, const float* w2_scale,
+                                 const int32_t* expert_map, int num_local_experts, float* topk_weights,
+                                 int32_t* topk_ids, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!hidden && M > 0) return fail(B200MOE_ERR_INVALID_ARG, "b200moe_layer_logits_grouped: null hidden%s");
+  int st = check_router_grouped("b200moe_layer_logits_grouped", router_logits, M, num_experts, num_groups, topk_groups,
+                                topk, scoring, correction_bias, topk_weights, topk_ids);
+  if (st) return st;
+  const RouterArgs r{router_logits, logits_bf16 ? 1 : 0, num_experts, topk, scoring, renormalize ? 1 : 0,
+                     correction_bias, scaling, topk_weights, topk_ids, num_groups, topk_groups};
+  LayerInput in{hidden, nullptr, 0, nullptr, 0};
+  return layer_core("b200moe_layer_logits_grouped", in, M, H, I, num_experts, topk, w13, w13_scale, w2, w2_scale,
                     topk_weights, topk_ids, expert_map, num_local_experts, out, workspace, workspace_bytes, 0, stream,
                     nullptr, nullptr, -1, &r);
 }
@@ -1376,9 +1434,20 @@ int b200moe_router_topk(const void* logits, int logits_bf16, int64_t M, int num_
   int st = check_router("b200moe_router_topk", logits, M, num_experts, topk, scoring, correction_bias, topk_weights,
                         topk_ids);
   if (st) return st;
-  return cuda_status(launch_router_topk(logits, logits_bf16, M, num_experts, topk, scoring, correction_bias,
-                                        renormalize, scaling, topk_weights, topk_ids, (cudaStream_t)stream),
-                     "router_topk");
+  const RouterArgs r{logits, logits_bf16 ? 1 : 0, num_experts, topk, scoring, renormalize ? 1 : 0,
+                     correction_bias, scaling, topk_weights, topk_ids};
+  return cuda_status(launch_router_topk(r, M, (cudaStream_t)stream), "router_topk");
+}
+
+int b200moe_router_topk_grouped(const void* logits, int logits_bf16, int64_t M, int num_experts, int num_groups,
+                                int topk_groups, int topk, int scoring, const float* correction_bias, int renormalize,
+                                float scaling, float* topk_weights, int32_t* topk_ids, void* stream) {
+  int st = check_router_grouped("b200moe_router_topk_grouped", logits, M, num_experts, num_groups, topk_groups, topk,
+                                scoring, correction_bias, topk_weights, topk_ids);
+  if (st) return st;
+  const RouterArgs r{logits,  logits_bf16 ? 1 : 0, num_experts, topk, scoring, renormalize ? 1 : 0, correction_bias,
+                     scaling, topk_weights,        topk_ids,    num_groups, topk_groups};
+  return cuda_status(launch_router_topk(r, M, (cudaStream_t)stream), "router_topk_grouped");
 }
 
 }  // extern "C"

@@ -214,9 +214,7 @@ cudaError_t launch_ep_combine_peer(const uint8_t* own, int64_t area_off, const i
                                    int G, int64_t rows_per_rank, int32_t epoch, void* out, int32_t* err,
                                    uint64_t limit_ns, cudaStream_t stream);
 
-cudaError_t launch_router_topk(const void* logits, int bf16, int64_t M, int E, int topk, int scoring,
-                               const float* bias, int renormalize, float scaling, float* out_w, int32_t* out_ids,
-                               cudaStream_t stream);
+cudaError_t launch_router_topk(const RouterArgs& r, int64_t M, cudaStream_t stream);
 
 cudaError_t launch_wait_timeout_selftest(int32_t* err, uint64_t timeout_ns, cudaStream_t stream);
 

@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) align_kernel(const AlignArgs
 // every id as align_kernel does, reading the ids the other CTAs stored
 // through L2. Few tokens per CTA (one up to 128 tokens) spread the router's
 // per-token work over many SMs.
-template <int PER>
+template <int PER, bool GROUPED>
 __global__ void __launch_bounds__(kRouteThreads, 1) router_align_kernel(const AlignArgs a, const RouterArgs r,
                                                                        int64_t M, int tpc, int32_t* counter) {
   extern __shared__ int32_t sm[];
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) router_align_kernel(const Al
   if (warp < tpc && t < M) {
     int id;
     float w;
-    route_token_warp<PER>(r, t, lane, id, w);
+    route_token<PER, GROUPED>(r, t, lane, id, w);
   }
   __threadfence();
   __syncthreads();
@@ -147,7 +147,7 @@ __device__ __forceinline__ void cta_segment(const AlignArgs& a, int64_t& beg, in
 
 // ROUTER: the CTA first routes the tokens of its segment (a.seg_align = topk,
 // a.topk_ids = r.out_ids) and counts the ids it just stored.
-template <bool ROUTER, int PER>
+template <bool ROUTER, int PER, bool GROUPED>
 __global__ void __launch_bounds__(kRouteThreads, 1) route_count_kernel(const AlignArgs a, int32_t* scratch,
                                                                       const RouterArgs r) {
   extern __shared__ int32_t sm[];
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_count_kernel(const Ali
     for (int64_t t = beg / r.topk + (tid >> 5); t < end / r.topk; t += kRouteWarps) {
       int id;
       float w;
-      route_token_warp<PER>(r, t, lane, id, w);
+      route_token<PER, GROUPED>(r, t, lane, id, w);
     }
   }
   __syncthreads();
@@ -338,17 +338,17 @@ int64_t route_scratch_ints(int64_t n, int E) {
 
 namespace {
 
-template <bool ROUTER, int PER>
+template <bool ROUTER, int PER, bool GROUPED = false>
 cudaError_t launch_route_multi(const AlignArgs& a, const RouterArgs& r, int C, int32_t* scratch,
                                cudaStream_t stream) {
   const size_t smem1 = (size_t)kRouteWarps * a.E * sizeof(int32_t);
   const size_t smem2 = (size_t)(kRouteWarps * a.E + 5 * a.E + 2) * sizeof(int32_t);
-  cudaError_t err = cudaFuncSetAttribute(route_count_kernel<ROUTER, PER>,
+  cudaError_t err = cudaFuncSetAttribute(route_count_kernel<ROUTER, PER, GROUPED>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem1);
   if (err == cudaSuccess)
     err = cudaFuncSetAttribute(route_scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem2);
   if (err != cudaSuccess) return err;
-  route_count_kernel<ROUTER, PER><<<C, kRouteThreads, smem1, stream>>>(a, scratch, r);
+  route_count_kernel<ROUTER, PER, GROUPED><<<C, kRouteThreads, smem1, stream>>>(a, scratch, r);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   route_scatter_kernel<<<C, kRouteThreads, smem2, stream>>>(a, scratch);
@@ -366,28 +366,40 @@ cudaError_t launch_route(const AlignArgs& a, int32_t* scratch, int64_t scratch_i
 
 int64_t route_logits_scratch_ints(int64_t n, int E) { return kRouteLogitsCounterInts + route_scratch_ints(n, E); }
 
-cudaError_t launch_route_logits(const AlignArgs& a_in, const RouterArgs& r, int64_t M, int32_t* counter,
-                                int32_t* counts, cudaStream_t stream) {
+namespace {
+
+template <bool GROUPED>
+cudaError_t launch_route_logits_impl(const AlignArgs& a_in, const RouterArgs& r, int64_t M, int32_t* counter,
+                                     int32_t* counts, cudaStream_t stream) {
   AlignArgs a = a_in;
   a.topk_ids = r.out_ids;
   a.seg_align = r.topk;
   const int C = route_ctas(a.n);
   const int per = router_per_lane(r.E);
   if (C > 1 && a.heavy_rows == 0) {
-    if (per == 8) return launch_route_multi<true, 8>(a, r, C, counts, stream);
-    if (per == 16) return launch_route_multi<true, 16>(a, r, C, counts, stream);
-    return launch_route_multi<true, 32>(a, r, C, counts, stream);
+    if (per == 8) return launch_route_multi<true, 8, GROUPED>(a, r, C, counts, stream);
+    if (per == 16) return launch_route_multi<true, 16, GROUPED>(a, r, C, counts, stream);
+    return launch_route_multi<true, 32, GROUPED>(a, r, C, counts, stream);
   }
   const size_t smem = align_smem_bytes(a.E);
   // tokens per CTA: one up to 128 tokens, then as many as keep 128 CTAs (at most 32)
   int tpc = M <= 128 ? 1 : (int)((M + 127) / 128);
   if (tpc > kRouteWarps) tpc = kRouteWarps;
   const int64_t ctas = M > 0 ? (M + tpc - 1) / tpc : 1;
-  auto kernel = per == 8 ? router_align_kernel<8> : (per == 16 ? router_align_kernel<16> : router_align_kernel<32>);
+  auto kernel = per == 8 ? router_align_kernel<8, GROUPED>
+                         : (per == 16 ? router_align_kernel<16, GROUPED> : router_align_kernel<32, GROUPED>);
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (err != cudaSuccess) return err;
   kernel<<<(unsigned)ctas, kRouteThreads, smem, stream>>>(a, r, M, tpc, counter);
   return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_route_logits(const AlignArgs& a, const RouterArgs& r, int64_t M, int32_t* counter, int32_t* counts,
+                                cudaStream_t stream) {
+  return r.groups > 0 ? launch_route_logits_impl<true>(a, r, M, counter, counts, stream)
+                      : launch_route_logits_impl<false>(a, r, M, counter, counts, stream);
 }
 
 }  // namespace b200moe

@@ -1,6 +1,6 @@
 // Router: scores -> top-k expert ids and weights, one warp per token (the
-// arithmetic is route_token_warp in router.cuh, shared with routing's first
-// launch when routing starts from logits).
+// arithmetic is route_token_warp / route_token_grouped in router.cuh, shared
+// with routing's first launch when routing starts from logits).
 #include "common.cuh"
 #include "launch.h"
 #include "router.cuh"
@@ -11,35 +11,37 @@ namespace {
 
 constexpr int kRouterWarps = 4;
 
-template <int PER>
+template <int PER, bool GROUPED>
 __global__ void __launch_bounds__(kRouterWarps * 32) router_topk_kernel(const RouterArgs r, int64_t M) {
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * kRouterWarps + (threadIdx.x >> 5);
   if (t >= M) return;
   int id;
   float w;
-  route_token_warp<PER>(r, t, lane, id, w);
+  route_token<PER, GROUPED>(r, t, lane, id, w);
+}
+
+template <bool GROUPED>
+cudaError_t launch_router_per(const RouterArgs& r, int64_t M, cudaStream_t stream) {
+  const unsigned blocks = (unsigned)((M + kRouterWarps - 1) / kRouterWarps);
+  switch (router_per_lane(r.E)) {
+    case 8:
+      router_topk_kernel<8, GROUPED><<<blocks, kRouterWarps * 32, 0, stream>>>(r, M);
+      break;
+    case 16:
+      router_topk_kernel<16, GROUPED><<<blocks, kRouterWarps * 32, 0, stream>>>(r, M);
+      break;
+    default:
+      router_topk_kernel<32, GROUPED><<<blocks, kRouterWarps * 32, 0, stream>>>(r, M);
+  }
+  return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_router_topk(const void* logits, int bf16, int64_t M, int E, int topk, int scoring,
-                               const float* bias, int renormalize, float scaling, float* out_w, int32_t* out_ids,
-                               cudaStream_t stream) {
+cudaError_t launch_router_topk(const RouterArgs& r, int64_t M, cudaStream_t stream) {
   if (M <= 0) return cudaSuccess;
-  const unsigned blocks = (unsigned)((M + kRouterWarps - 1) / kRouterWarps);
-  const RouterArgs r{logits, bf16, E, topk, scoring, renormalize, bias, scaling, out_w, out_ids};
-  switch (router_per_lane(E)) {
-    case 8:
-      router_topk_kernel<8><<<blocks, kRouterWarps * 32, 0, stream>>>(r, M);
-      break;
-    case 16:
-      router_topk_kernel<16><<<blocks, kRouterWarps * 32, 0, stream>>>(r, M);
-      break;
-    default:
-      router_topk_kernel<32><<<blocks, kRouterWarps * 32, 0, stream>>>(r, M);
-  }
-  return cudaGetLastError();
+  return r.groups > 0 ? launch_router_per<true>(r, M, stream) : launch_router_per<false>(r, M, stream);
 }
 
 }  // namespace b200moe

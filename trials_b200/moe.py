@@ -120,12 +120,23 @@ def moe_align_block_size(topk_ids: torch.Tensor, block_size: int, num_experts: i
     return sorted_ids, expert_ids, ntp
 
 
+def _check_groups(num_expert_group: Optional[int], topk_group: Optional[int]) -> bool:
+    if (num_expert_group is None) != (topk_group is None):
+        raise ValueError("num_expert_group and topk_group go together")
+    return num_expert_group is not None
+
+
 def select_experts(router_logits: torch.Tensor, top_k: int, scoring_func: str = "softmax",
                    correction_bias: Optional[torch.Tensor] = None, renormalize: bool = True,
-                   routed_scaling_factor: float = 1.0):
+                   routed_scaling_factor: float = 1.0, num_expert_group: Optional[int] = None,
+                   topk_group: Optional[int] = None):
     """Router: (M, E) f32/bf16 logits -> (topk_weights (M, k) f32, topk_ids (M, k) int32).
     softmax: top-k softmax probabilities; sigmoid: top-k of sigmoid + correction_bias
-    with the unbiased sigmoid as weights (GLM's routing). See b200moe_router_topk."""
+    with the unbiased sigmoid as weights (GLM's routing). See b200moe_router_topk.
+    num_expert_group, topk_group: group-limited routing, only the experts of the
+    topk_group best of num_expert_group equal groups can be selected (a group's
+    score is its largest value, with correction_bias the sum of its two largest).
+    See b200moe_router_topk_grouped."""
     dev = _require_cuda(router_logits)
     if router_logits.dtype not in (torch.float32, torch.bfloat16):
         raise NotImplementedError("router logits must be float32 or bfloat16")
@@ -137,6 +148,12 @@ def select_experts(router_logits: torch.Tensor, top_k: int, scoring_func: str = 
     w = torch.empty(M, top_k, dtype=torch.float32, device=dev)
     ids = torch.empty(M, top_k, dtype=torch.int32, device=dev)
     bias = None if correction_bias is None else correction_bias.to(device=dev, dtype=torch.float32).contiguous()
+    if _check_groups(num_expert_group, topk_group):
+        _lib.check(_lib.lib().b200moe_router_topk_grouped(
+            _ptr(logits), int(logits.dtype == torch.bfloat16), M, E, num_expert_group, topk_group, top_k, scoring,
+            _ptr(bias), int(renormalize), float(routed_scaling_factor), _ptr(w), _ptr(ids), _stream(dev)),
+            "select_experts")
+        return w, ids
     _lib.check(_lib.lib().b200moe_router_topk(_ptr(logits), int(logits.dtype == torch.bfloat16), M, E, top_k,
                                               scoring, _ptr(bias), int(renormalize), float(routed_scaling_factor),
                                               _ptr(w), _ptr(ids), _stream(dev)), "select_experts")
@@ -337,14 +354,18 @@ def moe_layer_from_logits(hidden_states: torch.Tensor, router_logits: torch.Tens
                           w13_scale: torch.Tensor, w2_fp8: torch.Tensor, w2_scale: torch.Tensor, top_k: int,
                           scoring_func: str = "sigmoid", correction_bias: Optional[torch.Tensor] = None,
                           renormalize: bool = True, routed_scaling_factor: float = 1.0,
-                          expert_map: Optional[torch.Tensor] = None):
+                          expert_map: Optional[torch.Tensor] = None, num_expert_group: Optional[int] = None,
+                          topk_group: Optional[int] = None, shared_expert: Optional[tuple] = None):
     """Router + layer: select_experts(router_logits, ...) followed by
     moe_decode_megakernel_full, with the router inside routing's first launch
     (b200moe_layer_logits). Returns (out (M, H) bf16, topk_weights (M, k) f32,
     topk_ids (M, k) int32), bit-identical to the two calls. expert_map
     (num_experts,) maps a global id to a local weight index or -1 (the weights
-    then hold only the mapped experts)."""
+    then hold only the mapped experts). num_expert_group, topk_group: as in
+    select_experts. shared_expert: (w13, w13_scale, w2, w2_scale) of a dense
+    expert that every token passes through; dense.fp8_mlp adds it to out."""
     dev = _require_cuda(hidden_states, router_logits, w13_fp8, w2_fp8)
+    grouped = _check_groups(num_expert_group, topk_group)
     if hidden_states.dtype != torch.bfloat16:
         raise NotImplementedError("moe_layer_from_logits takes bf16 hidden_states")
     if router_logits.dtype not in (torch.float32, torch.bfloat16):
@@ -369,12 +390,20 @@ def moe_layer_from_logits(hidden_states: torch.Tensor, router_logits: torch.Tens
     w13_scale, w2_scale = w13_scale.contiguous(), w2_scale.contiguous()  # held through the call
     L = _lib.lib()
     ws = _workspaces.get(dev, L.b200moe_layer_workspace_size(M, H, I, E_router, E_w, top_k))
-    _lib.check(L.b200moe_layer_logits(_ptr(hidden), M, H, I, E_router, top_k, _ptr(logits),
-                                      int(logits.dtype == torch.bfloat16), scoring, _ptr(bias), int(renormalize),
-                                      float(routed_scaling_factor), _ptr(w13_fp8), _ptr(w13_scale),
-                                      _ptr(w2_fp8), _ptr(w2_scale), _ptr(expert_map), E_w, _ptr(tw),
-                                      _ptr(ids), _ptr(out), _ptr(ws), ws.numel(), _stream(dev)),
-               "b200moe_layer_logits")
+    args = (_ptr(bias), int(renormalize), float(routed_scaling_factor), _ptr(w13_fp8), _ptr(w13_scale), _ptr(w2_fp8),
+            _ptr(w2_scale), _ptr(expert_map), E_w, _ptr(tw), _ptr(ids), _ptr(out), _ptr(ws), ws.numel(), _stream(dev))
+    if grouped:
+        _lib.check(L.b200moe_layer_logits_grouped(_ptr(hidden), M, H, I, E_router, top_k, _ptr(logits),
+                                                  int(logits.dtype == torch.bfloat16), num_expert_group, topk_group,
+                                                  scoring, *args), "b200moe_layer_logits_grouped")
+    else:
+        _lib.check(L.b200moe_layer_logits(_ptr(hidden), M, H, I, E_router, top_k, _ptr(logits),
+                                          int(logits.dtype == torch.bfloat16), scoring, *args),
+                   "b200moe_layer_logits")
+    if shared_expert is not None:
+        from .dense import fp8_mlp
+
+        fp8_mlp(hidden, *shared_expert, residual=out, out=out)
     return out, tw, ids
 
 

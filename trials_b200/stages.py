@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .moe import FP8, _ptr, _require_cuda, _stream
+from .moe import FP8, _check_groups, _ptr, _require_cuda, _stream
 
 
 @dataclass
@@ -83,9 +83,11 @@ def route(topk_ids: torch.Tensor, num_experts: int, tile_tokens: int, expert_map
 def route_logits(logits: torch.Tensor, top_k: int, tile_tokens: int, scoring_func: str = "sigmoid",
                  correction_bias: Optional[torch.Tensor] = None, renormalize: bool = True,
                  routed_scaling_factor: float = 1.0, expert_map: Optional[torch.Tensor] = None,
-                 num_local_experts: Optional[int] = None, err: Optional[torch.Tensor] = None):
-    """Router + routing (b200moe_route_logits) -> (Routing, topk_weights (M, k)
-    f32, topk_ids (M, k) int32), equal to select_experts followed by route()."""
+                 num_local_experts: Optional[int] = None, err: Optional[torch.Tensor] = None,
+                 num_expert_group: Optional[int] = None, topk_group: Optional[int] = None):
+    """Router + routing (b200moe_route_logits, with groups
+    b200moe_route_logits_grouped) -> (Routing, topk_weights (M, k) f32, topk_ids
+    (M, k) int32), equal to select_experts followed by route()."""
     dev = _require_cuda(logits)
     logits = logits.contiguous()
     M, E_router = logits.shape
@@ -106,12 +108,15 @@ def route_logits(logits: torch.Tensor, top_k: int, tile_tokens: int, scoring_fun
     scratch = torch.zeros(ns, dtype=torch.int32, device=dev)
     bias = None if correction_bias is None else correction_bias.to(device=dev, dtype=torch.float32).contiguous()
     scoring = {"softmax": 0, "sigmoid": 1}[scoring_func]
-    _lib.check(L.b200moe_route_logits(_ptr(logits), int(logits.dtype == torch.bfloat16), M, E_router, top_k, scoring,
-                                      _ptr(bias), int(renormalize), float(routed_scaling_factor), _ptr(tw), _ptr(ids),
-                                      _ptr(expert_map), E, tile_tokens, _ptr(r.sorted_ids), rows_cap,
-                                      _ptr(r.chunk_expert), _ptr(r.chunk_row0), _ptr(r.chunk_rows), chunks_cap,
-                                      _ptr(r.n_chunks), _ptr(r.num_rows), _ptr(r.slot_pos), _ptr(r.chunk_ready),
-                                      _ptr(scratch), ns, _ptr(r.err), _stream(dev)), "route_logits")
+    head = (_ptr(logits), int(logits.dtype == torch.bfloat16), M, E_router)
+    tail = (top_k, scoring, _ptr(bias), int(renormalize), float(routed_scaling_factor), _ptr(tw), _ptr(ids),
+            _ptr(expert_map), E, tile_tokens, _ptr(r.sorted_ids), rows_cap, _ptr(r.chunk_expert), _ptr(r.chunk_row0),
+            _ptr(r.chunk_rows), chunks_cap, _ptr(r.n_chunks), _ptr(r.num_rows), _ptr(r.slot_pos), _ptr(r.chunk_ready),
+            _ptr(scratch), ns, _ptr(r.err), _stream(dev))
+    if _check_groups(num_expert_group, topk_group):
+        _lib.check(L.b200moe_route_logits_grouped(*head, num_expert_group, topk_group, *tail), "route_logits")
+    else:
+        _lib.check(L.b200moe_route_logits(*head, *tail), "route_logits")
     return r, tw, ids
 
 
@@ -306,7 +311,7 @@ class LayerPipeline:
                  split: bool = False, one_launch: Optional[bool] = None, router: Optional[dict] = None,
                  whole: Optional[bool] = None):
         """router: {"scoring_func", "correction_bias", "renormalize",
-        "routed_scaling_factor"} to run the layer from router logits
+        "routed_scaling_factor", "num_expert_group", "topk_group"} to run the layer from router logits
         (run_from_logits: the router inside routing's first launch).
         whole: None = the whole-layer launch where b200moe_layer uses it,
         False = separate launches."""
@@ -368,6 +373,9 @@ class LayerPipeline:
             self.router = (({"softmax": 0, "sigmoid": 1}[r.get("scoring_func", "sigmoid")]),
                            None if bias is None else bias.to(device=device, dtype=torch.float32).contiguous(),
                            int(r.get("renormalize", True)), float(r.get("routed_scaling_factor", 1.0)))
+            self.groups = (r.get("num_expert_group"), r.get("topk_group"))
+            if not _check_groups(*self.groups):
+                self.groups = ()
             self.topk_weights = torch.zeros(M, topk, dtype=torch.float32, device=device)
             self.topk_ids = torch.zeros(M, topk, dtype=torch.int32, device=device)
             self.lscratch_ints = L.b200moe_route_logits_scratch_ints(numel, self.E)
@@ -394,22 +402,22 @@ class LayerPipeline:
         scoring, bias, renorm, scale = self.router
         cnt = _ptr(self.counts)
         rec(0)
+        head = (_ptr(logits), int(logits.dtype == torch.bfloat16))
+        rest = (scoring, _ptr(bias), renorm, scale)
         if self.whole:
-            _lib.check(L.b200moe_layer_logits(_ptr(hidden), self.M, self.H, self.I, self.num_experts, self.topk,
-                                              _ptr(logits), int(logits.dtype == torch.bfloat16), scoring, _ptr(bias),
-                                              renorm, scale, _ptr(w13), _ptr(w13_scale), _ptr(w2), _ptr(w2_scale),
-                                              _ptr(self.expert_map), self.E, _ptr(self.topk_weights),
-                                              _ptr(self.topk_ids), _ptr(self.out), _ptr(self.ws), self.ws.numel(),
-                                              st), "layer_logits")
+            fn = L.b200moe_layer_logits_grouped if self.groups else L.b200moe_layer_logits
+            _lib.check(fn(_ptr(hidden), self.M, self.H, self.I, self.num_experts, self.topk, *head, *self.groups, *rest,
+                          _ptr(w13), _ptr(w13_scale), _ptr(w2), _ptr(w2_scale), _ptr(self.expert_map), self.E,
+                          _ptr(self.topk_weights), _ptr(self.topk_ids), _ptr(self.out), _ptr(self.ws),
+                          self.ws.numel(), st), "layer_logits")
             rec(1)
             return self.out
-        _lib.check(L.b200moe_route_logits(_ptr(logits), int(logits.dtype == torch.bfloat16), self.M, self.num_experts,
-                                          self.topk, scoring, _ptr(bias), renorm, scale, _ptr(self.topk_weights),
-                                          _ptr(self.topk_ids), _ptr(self.expert_map), self.E, self.tile,
-                                          _ptr(self.sorted_ids), self.rows_cap, _ptr(self.ce), _ptr(self.cr0),
-                                          _ptr(self.crows), self.chunks_cap, cnt, cnt + 4, _ptr(self.slot_pos),
-                                          _ptr(self.ready), _ptr(self.lscratch), self.lscratch_ints, _ptr(self.err),
-                                          st), "route_logits")
+        fn = L.b200moe_route_logits_grouped if self.groups else L.b200moe_route_logits
+        _lib.check(fn(*head, self.M, self.num_experts, *self.groups, self.topk, *rest, _ptr(self.topk_weights),
+                      _ptr(self.topk_ids), _ptr(self.expert_map), self.E, self.tile, _ptr(self.sorted_ids),
+                      self.rows_cap, _ptr(self.ce), _ptr(self.cr0), _ptr(self.crows), self.chunks_cap, cnt, cnt + 4,
+                      _ptr(self.slot_pos), _ptr(self.ready), _ptr(self.lscratch), self.lscratch_ints,
+                      _ptr(self.err), st), "route_logits")
         rec(1)
         return self._after_route(hidden, self.topk_weights, w13, w13_scale, w2, w2_scale, rec, grid_ctas)
 
