@@ -8,7 +8,9 @@
 // MMA per K step. An epilogue thread owns one token and 128 weight rows of one
 // scale block, so its factor is one scalar per K block; gate/up pairs
 // (interleaved rows 2j, 2j+1) meet in one thread.
-// Warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2..9 epilogue.
+// Warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 4..11 epilogue (two
+// warpgroups, which take over the first one's registers: 168 a thread at launch
+// spilled the accumulators' neighbours).
 // Rows past M and weight rows past N are zero-filled by TMA and not stored.
 #pragma once
 
@@ -25,61 +27,82 @@ struct DenseTokCfg {
   static constexpr int TN = 256;
   static constexpr int EW = 8;     // epilogue warps: 4 lane quarters x 2 column halves
   static constexpr int COLS = 128; // columns per epilogue thread
-  static constexpr int THREADS = 64 + 32 * EW;
+  static constexpr int THREADS = 128 + 32 * EW;
+  // 384 threads x 168 registers at launch = 128 x (40 + 232 + 232).
+  static constexpr int REGS_LOAD = 40, REGS_EPI = 232;
   static constexpr int X_BYTES = TM * 128;
   static constexpr int W_BYTES = TN * 128;
   static constexpr int TILE_BYTES = X_BYTES + W_BYTES;
   static constexpr int NBUF = 2;
   static constexpr int TMEM_COLS = 512;
   static constexpr int NSTAGE = 4;
-  static constexpr int RED = 2 * 2 * TM * 4;  // amax exchange, double-buffered by unit parity
-  static constexpr int SMEM_BYTES = 1024 + NSTAGE * TILE_BYTES + RED + 256;
+  // DENSE_SILU: amax exchange, double-buffered by unit parity. DENSE_OUT: 32
+  // rows x 32 columns of fp32 per epilogue warp on their way out.
+  static constexpr int RED = 2 * 2 * TM * 4;
+  static constexpr int STAGING = EW * 32 * 128;
+  static constexpr int SMEM_BYTES = 1024 + NSTAGE * TILE_BYTES + (STAGING > RED ? STAGING : RED) + 256;
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
 
-// 128 consecutive columns n0.. of one output row; cols = how many exist.
-__device__ __forceinline__ void dense_store_row(const DenseParams& p, int64_t m, int n0, int cols,
-                                                const float (&acc)[128]) {
-  const __nv_bfloat16* res =
-      p.residual ? static_cast<const __nv_bfloat16*>(p.residual) + m * p.ld_res + n0 : nullptr;
-  if (p.vec) {  // cols is a multiple of 8
+// Stores 32 rows (m0.., one per lane) x 128 columns (n0..) of fp32 results. They
+// pass through st (4 KB of this warp, rows of 32 columns, 16-byte pieces
+// swizzled by row), so that a store instruction covers whole 64-byte (bf16) or
+// 128-byte (f32) runs of 4 rows, or 32 consecutive columns of one row where
+// rows are not aligned.
+__device__ __forceinline__ void dense_store_tile(const DenseParams& p, int m0, int n0, const float (&acc)[128],
+                                                 uint8_t* st, int lane) {
+  const int rows = p.M - m0 < 32 ? p.M - m0 : 32;
 #pragma unroll
-    for (int j = 0; j < 128; j += 8) {
-      if (j >= cols) break;
-      float v[8];
+  for (int cb = 0; cb < 4; ++cb) {
+    const int n1 = n0 + cb * 32;
+    if (n1 < p.N) {  // warp-uniform
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = acc[j + i];
-      if (res) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(res + j);
-        const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
+      for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<float4*>(st + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+            make_float4(acc[cb * 32 + 4 * c], acc[cb * 32 + 4 * c + 1], acc[cb * 32 + 4 * c + 2],
+                        acc[cb * 32 + 4 * c + 3]);
+      __syncwarp();
+      if (p.vec) {  // N is a multiple of 8: a piece of 4 columns exists or does not
+        const int c = lane & 7, n = n1 + 4 * c;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = __bfloat1622float2(h2[i]);
-          v[2 * i] += f.x;
-          v[2 * i + 1] += f.y;
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + (lane >> 3);
+          if (r < rows && n < p.N) {
+            float4 v = *reinterpret_cast<const float4*>(st + r * 128 + ((c ^ (r & 7)) << 4));
+            const int64_t m = m0 + r;
+            if (p.residual) {
+              const uint2 raw = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.residual) +
+                                                                m * p.ld_res + n);
+              const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
+              const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+              v.x += lo.x;
+              v.y += lo.y;
+              v.z += hi.x;
+              v.w += hi.y;
+            }
+            if (p.out_f32) {
+              *reinterpret_cast<float4*>(static_cast<float*>(p.out) + m * p.ld_out + n) = v;
+            } else {
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+              uint2 pk;
+              pk.x = *reinterpret_cast<const uint32_t*>(&lo);
+              pk.y = *reinterpret_cast<const uint32_t*>(&hi);
+              *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + m * p.ld_out + n) = pk;
+            }
+          }
+        }
+      } else if (n1 + lane < p.N) {
+        for (int r = 0; r < rows; ++r) {
+          float v = *reinterpret_cast<const float*>(st + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+          const int64_t m = m0 + r;
+          const int n = n1 + lane;
+          if (p.residual) v += __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[m * p.ld_res + n]);
+          if (p.out_f32) static_cast<float*>(p.out)[m * p.ld_out + n] = v;
+          else static_cast<__nv_bfloat16*>(p.out)[m * p.ld_out + n] = __float2bfloat16_rn(v);
         }
       }
-      if (p.out_f32) {
-        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + m * p.ld_out + n0 + j);
-        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        __nv_bfloat162 o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + m * p.ld_out + n0 + j) =
-            *reinterpret_cast<const uint4*>(o);
-      }
+      __syncwarp();
     }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 128; ++j) {
-    if (j >= cols) break;
-    float v = acc[j];
-    if (res) v += __bfloat162float(res[j]);
-    if (p.out_f32) static_cast<float*>(p.out)[m * p.ld_out + n0 + j] = v;
-    else static_cast<__nv_bfloat16*>(p.out)[m * p.ld_out + n0 + j] = __float2bfloat16_rn(v);
   }
 }
 
@@ -91,8 +114,8 @@ __global__ void __launch_bounds__(DenseTokCfg::THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* tiles = smem;
-  float* red = reinterpret_cast<float*>(tiles + C::NSTAGE * C::TILE_BYTES);
-  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(red) + C::RED);
+  uint8_t* scratch = tiles + C::NSTAGE * C::TILE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(scratch + (EPI == DENSE_SILU ? C::RED : C::STAGING));
   uint64_t* empty = full + C::NSTAGE;
   uint64_t* tfull = empty + C::NSTAGE;
   uint64_t* tempty = tfull + C::NBUF;
@@ -131,87 +154,91 @@ __global__ void __launch_bounds__(DenseTokCfg::THREADS, 1)
   griddep_wait();  // the kernel ahead of it wrote x (programmatic launch)
   griddep_launch_dependents();
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      long issued = 0;
-      bool ok = true;
-      for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
-        int mt, nt;
-        unit_coords(u, n_mt, n_nt, group, mt, nt);
-        for (int kb = 0; kb < NKB; ++kb) {
-          if (*abort_flag || !mbar_wait_bounded(&empty[stage], phase ^ 1, p.timeout_ns)) {
-            ok = false;
-            break;
-          }
-          uint8_t* tile = tiles + stage * C::TILE_BYTES;
-          mbar_arrive_expect_tx(&full[stage], C::TILE_BYTES);
-          tma_load_2d(tile, &tm_x, &full[stage], kb * 128, mt * C::TM);
-          tma_load_2d(tile + C::X_BYTES, &tm_w, &full[stage], kb * 128, nt * C::TN);
-          ++issued;
-          if (++stage == C::NSTAGE) {
-            stage = 0;
-            phase ^= 1;
+  if (warp < 4) {
+    regs_dec<C::REGS_LOAD>();
+    if (warp == 0) {
+      // ------------------------------------------------------------ producer
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        long issued = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
+          int mt, nt;
+          unit_coords(u, n_mt, n_nt, group, mt, nt);
+          for (int kb = 0; kb < NKB; ++kb) {
+            if (*abort_flag || !mbar_wait_bounded(&empty[stage], phase ^ 1, p.timeout_ns)) {
+              ok = false;
+              break;
+            }
+            uint8_t* tile = tiles + stage * C::TILE_BYTES;
+            mbar_arrive_expect_tx(&full[stage], C::TILE_BYTES);
+            tma_load_2d(tile, &tm_x, &full[stage], kb * 128, mt * C::TM);
+            tma_load_2d(tile + C::X_BYTES, &tm_w, &full[stage], kb * 128, nt * C::TN);
+            ++issued;
+            if (++stage == C::NSTAGE) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
         }
+        if (!ok) {
+          atomicOr(p.err, ERR_DEV_TIMEOUT);
+          *abort_flag = 1;
+          const long first = issued > C::NSTAGE ? issued - C::NSTAGE : 0;
+          for (long g = first; g < issued; ++g)
+            mbar_wait_bounded(&full[g % C::NSTAGE], (uint32_t)((g / C::NSTAGE) & 1), p.timeout_ns);
+        }
       }
-      if (!ok) {
-        atomicOr(p.err, ERR_DEV_TIMEOUT);
-        *abort_flag = 1;
-        const long first = issued > C::NSTAGE ? issued - C::NSTAGE : 0;
-        for (long g = first; g < issued; ++g)
-          mbar_wait_bounded(&full[g % C::NSTAGE], (uint32_t)((g / C::NSTAGE) & 1), p.timeout_ns);
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      const uint32_t idesc = idesc_e4m3_f32(C::TM, C::TN);
-      int stage = 0, buf = 0, last_buf = 0;
-      uint32_t phase = 0, bphase = 0, last_bphase = 0;
-      bool ok = true, any = false;
-      for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
-        for (int kb = 0; kb < NKB; ++kb) {
-          if (*abort_flag || !mbar_wait_bounded(&tempty[buf], bphase ^ 1, p.timeout_ns) ||
-              !mbar_wait_bounded(&full[stage], phase, p.timeout_ns)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t x_addr = smem_u32(tiles + stage * C::TILE_BYTES);
-          const uint32_t w_addr = x_addr + C::X_BYTES;
-          const uint32_t d = tmem_base + (uint32_t)(buf * C::TN);
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer
+      if (lane == 0) {
+        const uint32_t idesc = idesc_e4m3_f32(C::TM, C::TN);
+        int stage = 0, buf = 0, last_buf = 0;
+        uint32_t phase = 0, bphase = 0, last_bphase = 0;
+        bool ok = true, any = false;
+        for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
+          for (int kb = 0; kb < NKB; ++kb) {
+            if (*abort_flag || !mbar_wait_bounded(&tempty[buf], bphase ^ 1, p.timeout_ns) ||
+                !mbar_wait_bounded(&full[stage], phase, p.timeout_ns)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t x_addr = smem_u32(tiles + stage * C::TILE_BYTES);
+            const uint32_t w_addr = x_addr + C::X_BYTES;
+            const uint32_t d = tmem_base + (uint32_t)(buf * C::TN);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma_f8(d, sdesc_kmajor_sw128(x_addr + ks * 32), sdesc_kmajor_sw128(w_addr + ks * 32), idesc,
-                    ks > 0 ? 1u : 0u);
-          umma_commit(&empty[stage]);
-          umma_commit(&tfull[buf]);
-          any = true;
-          last_buf = buf;
-          last_bphase = bphase;
-          if (++stage == C::NSTAGE) {
-            stage = 0;
-            phase ^= 1;
-          }
-          if (++buf == C::NBUF) {
-            buf = 0;
-            bphase ^= 1;
+            for (int ks = 0; ks < 4; ++ks)
+              umma_f8(d, sdesc_kmajor_sw128(x_addr + ks * 32), sdesc_kmajor_sw128(w_addr + ks * 32), idesc,
+                      ks > 0 ? 1u : 0u);
+            umma_commit(&empty[stage]);
+            umma_commit(&tfull[buf]);
+            any = true;
+            last_buf = buf;
+            last_bphase = bphase;
+            if (++stage == C::NSTAGE) {
+              stage = 0;
+              phase ^= 1;
+            }
+            if (++buf == C::NBUF) {
+              buf = 0;
+              bphase ^= 1;
+            }
           }
         }
+        if (!ok) {
+          atomicOr(p.err, ERR_DEV_TIMEOUT);
+          *abort_flag = 1;
+        }
+        // The tensor core must be done with TMEM before it is released.
+        if (any) mbar_wait_bounded(&tfull[last_buf], last_bphase, p.timeout_ns);
       }
-      if (!ok) {
-        atomicOr(p.err, ERR_DEV_TIMEOUT);
-        *abort_flag = 1;
-      }
-      // The tensor core must be done with TMEM before it is released.
-      if (any) mbar_wait_bounded(&tfull[last_buf], last_bphase, p.timeout_ns);
     }
   } else {
+    regs_inc<C::REGS_EPI>();
     // ------------------------------------------------------------ epilogue
-    const int ew = warp - 2;
+    const int ew = warp - 4;
     const int q = warp & 3;       // TMEM lane quarter
     const int h = ew >> 2;        // column half = one weight scale block
     const int r = q * 32 + lane;  // token of the tile
@@ -284,7 +311,7 @@ __global__ void __launch_bounds__(DenseTokCfg::THREADS, 1)
           acc[i] = silu_f32(acc[2 * i]) * acc[2 * i + 1];
           mx = fmaxf(mx, fabsf(acc[i]));
         }
-        float* rb = red + parity * 2 * C::TM;
+        float* rb = reinterpret_cast<float*>(scratch) + parity * 2 * C::TM;
         rb[h * C::TM + r] = mx;
         // One barrier per unit: the exchange buffer alternates, and a warp
         // reaches the write two units on only after every warp has passed the
@@ -308,7 +335,7 @@ __global__ void __launch_bounds__(DenseTokCfg::THREADS, 1)
           if (h == 0) p.s[m * p.ld_s + nt] = scale;
         }
       } else {
-        if (ok && m < p.M && n0 < p.N) dense_store_row(p, m, n0, p.N - n0, acc);
+        if (ok && live) dense_store_tile(p, mt * C::TM + q * 32, n0, acc, scratch + ew * 4096, lane);
       }
     }
   }

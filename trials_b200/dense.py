@@ -20,7 +20,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .moe import FP8, _ptr, _require_cuda, _workspaces
+from .moe import FP8, _ptr, _require_cuda, _stream, _workspaces
 
 
 def _on_device(dev: torch.device):
@@ -100,7 +100,7 @@ def _call_state(dev: torch.device, nbytes: int):
     """(stream, error word pointer, workspace) of one call. The workspace is
     this call's own, from torch's allocator on the current stream; the error
     word is the cached one of (device, stream) (moe.layer_error_word)."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
+    stream = _stream(dev)
     err = _workspaces.get_for(dev, stream, 256).data_ptr()
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     return stream, err, ws

@@ -34,7 +34,10 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of the device's current stream (the raw form of
+    torch.cuda.current_stream(device).cuda_stream, 0.1 us instead of 2.2)."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def _require_cuda(*tensors: torch.Tensor) -> torch.device:
