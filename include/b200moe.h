@@ -570,8 +570,8 @@ B200MOE_API int b200moe_combine_reduce(const void* out_pair, const int32_t* slot
  *               * sum_{k in block kb} x_q[m, k] * w[n, k]  (+ residual[m, n])
  * in fp32, rounded once to bf16 (out_f32 = 0) or stored as f32 (1).
  * Activations: either x (M, K) bf16, quantised first as b200moe_quant_1x128
- * does (into the workspace, b200moe_linear_workspace_size() bytes, 256-byte
- * aligned), or x_q (M, K) fp8 with x_scale (M, K/128); pass NULL for the other.
+ * does, or x_q (M, K) fp8 with x_scale (M, K/128); pass NULL for the other.
+ * workspace: b200moe_linear_workspace_size() bytes (may be 0), 256-byte aligned.
  * ld_x / ld_xs are row strides in elements of x or x_q / x_scale (ld_xs is not
  * read with bf16 rows). w (N, K) fp8 with row stride ld_w bytes; w_scale
  * (ceil(N/128), K/128) contiguous. residual (M, N) bf16 or NULL; it may be out
@@ -591,7 +591,8 @@ B200MOE_API int b200moe_combine_reduce(const void* out_pair, const int32_t* slot
  * A pipeline wait that gives up sets B200MOE_DEVERR_TIMEOUT in err_word
  * (required) and leaves the outputs undefined.
  * ---------------------------------------------------------------------- */
-B200MOE_API size_t b200moe_linear_workspace_size(int64_t M, int64_t K);
+/* x_bf16: the rows come in bf16; gate_up: for b200moe_gate_up, with N = 2I and K = H. */
+B200MOE_API size_t b200moe_linear_workspace_size(int64_t M, int64_t N, int64_t K, int x_bf16, int gate_up);
 B200MOE_API int b200moe_linear(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs,
                                int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ld_w, const float* w_scale,
                                const void* residual, int64_t ld_res, void* out, int64_t ld_out, int out_f32,
@@ -600,7 +601,7 @@ B200MOE_API int b200moe_gate_up(const void* x, const uint8_t* x_q, const float* 
                                 int64_t M, int64_t H, int64_t I, const uint8_t* w13, int64_t ld_w,
                                 const float* w13_scale, uint8_t* q, int64_t ld_q, float* s, int64_t ld_s,
                                 void* workspace, size_t workspace_bytes, int32_t* err_word, void* stream);
-B200MOE_API size_t b200moe_mlp_workspace_size(int64_t M, int64_t H, int64_t I);
+B200MOE_API size_t b200moe_mlp_workspace_size(int64_t M, int64_t H, int64_t I, int x_bf16);
 B200MOE_API int b200moe_mlp(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs,
                             int64_t M, int64_t H, int64_t I, const uint8_t* w13, const float* w13_scale,
                             const uint8_t* w2, const float* w2_scale, const void* residual, int64_t ld_res, void* out,

@@ -31,7 +31,7 @@ def test_linear_unsupported_layouts(kw):
     assert linear(**kw) == _lib.ERR_UNSUPPORTED
 
 
-@pytest.mark.parametrize("kw", [dict(work=None), dict(nwork=100), dict(work=P + 16)])
+@pytest.mark.parametrize("kw", [dict(M=3000, work=None), dict(M=3000, nwork=100), dict(M=3000, work=P + 16)])
 def test_linear_workspace(kw):
     assert linear(**kw) == _lib.ERR_WORKSPACE
 
@@ -43,7 +43,8 @@ def test_empty_batches_launch_nothing():
                              None) == _lib.OK
     assert L.b200moe_mlp(None, None, None, 0, 0, 0, 256, 128, P, P, P, P, None, 0, None, 0, None, 0, P,
                          None) == _lib.OK
-    assert L.b200moe_linear_workspace_size(0, 256) == 0 and L.b200moe_mlp_workspace_size(0, 256, 128) == 0
+    assert L.b200moe_linear_workspace_size(0, 256, 256, 1, 0) == 0
+    assert L.b200moe_mlp_workspace_size(0, 256, 128, 1) == 0
 
 
 def test_gate_up_and_mlp_host_checks():
@@ -67,13 +68,17 @@ def test_gate_up_and_mlp_host_checks():
     assert mlp(w2=None) == _lib.ERR_INVALID_ARG
     assert mlp(w2=P + 8) == _lib.ERR_UNSUPPORTED
     assert mlp(res=P) == _lib.ERR_INVALID_ARG  # residual without a stride
-    assert mlp(nwork=L.b200moe_mlp_workspace_size(4, 256, 128) - 1) == _lib.ERR_WORKSPACE
+    assert mlp(nwork=L.b200moe_mlp_workspace_size(4, 256, 128, 1) - 1) == _lib.ERR_WORKSPACE
 
 
 def test_workspace_sizes_cover_codes_and_scales():
     L = _lib.lib()
-    assert L.b200moe_linear_workspace_size(3, 384) >= 3 * 384 + 3 * 3 * 4
-    assert L.b200moe_mlp_workspace_size(3, 384, 128) >= 3 * 384 + 3 * 3 * 4 + 3 * 128 + 3 * 4
+    # many bf16 rows are quantised into the workspace
+    assert L.b200moe_linear_workspace_size(3000, 384, 384, 1, 0) >= 3000 * 384 + 3000 * 3 * 4
+    assert L.b200moe_mlp_workspace_size(3, 384, 128, 0) >= 3 * 128 + 3 * 4
+    assert L.b200moe_mlp_workspace_size(3000, 384, 128, 1) >= 3000 * (384 + 3 * 4) + 3000 * (128 + 4)
+    for bad in ((-1, 1, 128), (1, 0, 128), (1, 1, 100)):
+        assert L.b200moe_linear_workspace_size(*bad, 1, 0) == 0
 
 
 def test_python_ops_refuse_cpu_tensors():
@@ -116,7 +121,8 @@ def test_python_weight_and_output_checks():
         with pytest.raises(NotImplementedError):
             dense._weight(*bad, 256, "weight")
     out = torch.zeros(3, 5, dtype=torch.bfloat16)
-    assert dense._output(out, out, 3, 5, torch.bfloat16, out.device) == (out, out)
+    got = dense._output(out, out, 3, 5, torch.bfloat16, out.device)
+    assert got[0] is out and got[1:] == (5, 5)
     for o, r in ((out[:2], None), (out.float(), None), (None, out[:, :4])):
         with pytest.raises(ValueError):
             dense._output(o, r, 3, 5, torch.bfloat16, out.device)

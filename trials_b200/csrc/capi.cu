@@ -1487,9 +1487,8 @@ size_t dense_quant_bytes(int64_t M, int64_t K) {
   return (size_t)round_up(M * K, 256) + (size_t)round_up(M * (K / 128) * 4, 256);
 }
 
-// bf16 rows -> fp8 rows in ws (dense_quant_bytes); fp8 rows stay as they are.
+// bf16 rows -> fp8 rows in ws (dense_quant_bytes).
 int dense_quantise(DenseInput& in, int64_t M, int64_t K, uint8_t* ws, void* stream) {
-  if (!in.x) return B200MOE_OK;
   uint8_t* q = ws;
   float* s = reinterpret_cast<float*>(ws + round_up(M * K, 256));
   const int st = b200moe_quant_1x128(in.x, M, K, in.ld_x, q, K, s, K / 128, 1, stream);
@@ -1498,24 +1497,49 @@ int dense_quantise(DenseInput& in, int64_t M, int64_t K, uint8_t* ws, void* stre
   return B200MOE_OK;
 }
 
-// One product of quantised rows; the output fields of p are set by the caller.
-int run_dense(const char* name, int epi, const DenseInput& in, int64_t M, int64_t N, int64_t K, const uint8_t* w,
-              int64_t ld_w, const float* w_scale, DenseParams p, int32_t* err_word, void* stream) {
-  const DensePlan pl = dense_plan(epi, M, N, K);
+// Workspace of one product: bf16 rows that the kernel does not quantise itself.
+size_t dense_bytes(const DensePlan& pl, int64_t M, int64_t K, bool x_bf16) {
+  return x_bf16 && !pl.quantise_x ? dense_quant_bytes(M, K) : 0;
+}
+
+int check_dense_work(const char* name, const void* workspace, size_t have, size_t need) {
+  if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 || have < need))
+    return fail(B200MOE_ERR_WORKSPACE, "%s: workspace too small or not 256-byte aligned", name);
+  return B200MOE_OK;
+}
+
+// One product; the output fields of p are set by the caller. quant: room for the
+// quantised rows (dense_bytes). chained: the launch ahead of it in the stream is
+// one of this call's own and does not write w.
+int run_dense(const char* name, int epi, const DensePlan& pl, DenseInput in, int64_t M, int64_t N, int64_t K,
+              const uint8_t* w, int64_t ld_w, const float* w_scale, DenseParams p, bool chained, uint8_t* quant,
+              int32_t* err_word, void* stream) {
+  int st;
+  if (in.x && !pl.quantise_x) {
+    st = dense_quantise(in, M, K, quant, stream);
+    if (st) return st;
+    chained = true;
+  }
   CUtensorMap tm_x, tm_w;
-  int st = make_tmap_u8(&tm_x, in.q, M, K, pl.x_box_rows, in.ld_x);
-  if (st) return st;
   st = make_tmap_u8(&tm_w, w, N, K, pl.w_box_rows, ld_w);
   if (st) return st;
-  p.xs = in.s;
-  p.ld_xs = in.ld_s;
+  if (in.x) {
+    tm_x = tm_w;  // not read
+    p.xb = in.x;
+    p.ld_xb = in.ld_x;
+  } else {
+    st = make_tmap_u8(&tm_x, in.q, M, K, pl.x_box_rows, in.ld_x);
+    if (st) return st;
+    p.xs = in.s;
+    p.ld_xs = in.ld_s;
+  }
   p.ws = w_scale;
   p.M = (int)M;
   p.N = (int)N;
   p.K = (int)K;
   p.err = err_word;
   p.timeout_ns = kTimeoutNs;
-  return cuda_status(launch_dense(epi, pl, tm_x, tm_w, p, (cudaStream_t)stream), name);
+  return cuda_status(launch_dense(epi, pl, tm_x, tm_w, p, chained, (cudaStream_t)stream), name);
 }
 
 int check_dense_out(const char* name, int64_t M, int64_t N, const void* residual, int64_t ld_res, const void* out,
@@ -1539,90 +1563,116 @@ int check_dense_out(const char* name, int64_t M, int64_t N, const void* residual
 
 extern "C" {
 
-size_t b200moe_linear_workspace_size(int64_t M, int64_t K) { return M > 0 && K > 0 ? dense_quant_bytes(M, K) : 0; }
+size_t b200moe_linear_workspace_size(int64_t M, int64_t N, int64_t K, int x_bf16, int gate_up) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % 128 != 0 || M > (1 << 30) || N > (1 << 24) || K > (1 << 20)) return 0;
+  return dense_bytes(dense_plan(gate_up ? DENSE_SILU : DENSE_OUT, M, N, K, x_bf16 != 0), M, K, x_bf16 != 0);
+}
 
 int b200moe_linear(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs, int64_t M,
                    int64_t N, int64_t K, const uint8_t* w, int64_t ld_w, const float* w_scale, const void* residual,
                    int64_t ld_res, void* out, int64_t ld_out, int out_f32, void* workspace, size_t workspace_bytes,
                    int32_t* err_word, void* stream) {
-  DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
-  int st = check_dense("b200moe_linear", in, M, N, K, w, ld_w, w_scale, err_word);
+  const char* name = "b200moe_linear";
+  const DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
+  int st = check_dense(name, in, M, N, K, w, ld_w, w_scale, err_word);
   if (st) return st;
   DenseParams p{};
-  st = check_dense_out("b200moe_linear", M, N, residual, ld_res, out, ld_out, out_f32, p);
+  st = check_dense_out(name, M, N, residual, ld_res, out, ld_out, out_f32, p);
   if (st) return st;
   if (M == 0) return B200MOE_OK;
-  if (x && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
-            workspace_bytes < dense_quant_bytes(M, K)))
-    return fail(B200MOE_ERR_WORKSPACE, "b200moe_linear: workspace too small or not 256-byte aligned%s");
-  st = dense_quantise(in, M, K, static_cast<uint8_t*>(workspace), stream);
+  const DensePlan pl = dense_plan(DENSE_OUT, M, N, K, x != nullptr);
+  st = check_dense_work(name, workspace, workspace_bytes, dense_bytes(pl, M, K, x != nullptr));
   if (st) return st;
-  return run_dense("b200moe_linear", DENSE_OUT, in, M, N, K, w, ld_w, w_scale, p, err_word, stream);
+  return run_dense(name, DENSE_OUT, pl, in, M, N, K, w, ld_w, w_scale, p, false, static_cast<uint8_t*>(workspace),
+                   err_word, stream);
 }
 
 int b200moe_gate_up(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs, int64_t M,
                     int64_t H, int64_t I, const uint8_t* w13, int64_t ld_w, const float* w13_scale, uint8_t* q,
                     int64_t ld_q, float* s, int64_t ld_s, void* workspace, size_t workspace_bytes, int32_t* err_word,
                     void* stream) {
-  DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
-  if (I <= 0 || I > (1 << 23)) return fail(B200MOE_ERR_INVALID_ARG, "b200moe_gate_up: bad argument%s");
-  int st = check_dense("b200moe_gate_up", in, M, 2 * I, H, w13, ld_w, w13_scale, err_word);
+  const char* name = "b200moe_gate_up";
+  const DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
+  if (I <= 0 || I > (1 << 23)) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
+  int st = check_dense(name, in, M, 2 * I, H, w13, ld_w, w13_scale, err_word);
   if (st) return st;
   if (M > 0 && (!q || !s || ld_q < I || ld_s < I / 128))
-    return fail(B200MOE_ERR_INVALID_ARG, "b200moe_gate_up: bad output%s");
-  if (I % 128 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "b200moe_gate_up: I must be a multiple of 128%s");
+    return fail(B200MOE_ERR_INVALID_ARG, "%s: bad output", name);
+  if (I % 128 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "%s: I must be a multiple of 128", name);
   if (!aligned16(q) || ld_q % 16 != 0)
-    return fail(B200MOE_ERR_UNSUPPORTED, "b200moe_gate_up: output rows must be 16-byte aligned%s");
+    return fail(B200MOE_ERR_UNSUPPORTED, "%s: output rows must be 16-byte aligned", name);
   if (M == 0) return B200MOE_OK;
-  if (x && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
-            workspace_bytes < dense_quant_bytes(M, H)))
-    return fail(B200MOE_ERR_WORKSPACE, "b200moe_gate_up: workspace too small or not 256-byte aligned%s");
-  st = dense_quantise(in, M, H, static_cast<uint8_t*>(workspace), stream);
+  const DensePlan pl = dense_plan(DENSE_SILU, M, 2 * I, H, x != nullptr);
+  st = check_dense_work(name, workspace, workspace_bytes, dense_bytes(pl, M, H, x != nullptr));
   if (st) return st;
   DenseParams p{};
   p.q = q;
   p.ld_q = ld_q;
   p.s = s;
   p.ld_s = ld_s;
-  return run_dense("b200moe_gate_up", DENSE_SILU, in, M, 2 * I, H, w13, ld_w, w13_scale, p, err_word, stream);
+  return run_dense(name, DENSE_SILU, pl, in, M, 2 * I, H, w13, ld_w, w13_scale, p, false,
+                   static_cast<uint8_t*>(workspace), err_word, stream);
 }
 
-size_t b200moe_mlp_workspace_size(int64_t M, int64_t H, int64_t I) {
-  return M > 0 && H > 0 && I > 0 ? dense_quant_bytes(M, H) + dense_quant_bytes(M, I) : 0;
+}  // extern "C"
+
+namespace {
+
+// Workspace of b200moe_mlp: [quantised rows][inter codes and scales].
+struct MlpPlan {
+  DensePlan up, down;
+  size_t off_inter, total;
+};
+MlpPlan plan_mlp(int64_t M, int64_t H, int64_t I, bool x_bf16) {
+  MlpPlan m{};
+  m.up = dense_plan(DENSE_SILU, M, 2 * I, H, x_bf16);
+  m.down = dense_plan(DENSE_OUT, M, H, I, false);
+  m.off_inter = dense_bytes(m.up, M, H, x_bf16);
+  m.total = m.off_inter + dense_quant_bytes(M, I);
+  return m;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t b200moe_mlp_workspace_size(int64_t M, int64_t H, int64_t I, int x_bf16) {
+  if (M <= 0 || H <= 0 || I <= 0 || H % 128 != 0 || I % 128 != 0 || M > (1 << 30) || H > (1 << 20) || I > (1 << 20))
+    return 0;
+  return plan_mlp(M, H, I, x_bf16 != 0).total;
 }
 
 int b200moe_mlp(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs, int64_t M,
                 int64_t H, int64_t I, const uint8_t* w13, const float* w13_scale, const uint8_t* w2,
                 const float* w2_scale, const void* residual, int64_t ld_res, void* out, int64_t ld_out,
                 void* workspace, size_t workspace_bytes, int32_t* err_word, void* stream) {
-  DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
-  if (I <= 0 || I > (1 << 20)) return fail(B200MOE_ERR_INVALID_ARG, "b200moe_mlp: bad argument%s");
-  int st = check_dense("b200moe_mlp", in, M, 2 * I, H, w13, H, w13_scale, err_word);
+  const char* name = "b200moe_mlp";
+  const DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
+  if (I <= 0 || I > (1 << 20)) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
+  int st = check_dense(name, in, M, 2 * I, H, w13, H, w13_scale, err_word);
   if (st) return st;
-  if (I % 128 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "b200moe_mlp: I must be a multiple of 128%s");
-  if (!w2 || !w2_scale) return fail(B200MOE_ERR_INVALID_ARG, "b200moe_mlp: bad argument%s");
-  if (!aligned16(w2)) return fail(B200MOE_ERR_UNSUPPORTED, "b200moe_mlp: weight rows must be 16-byte aligned%s");
+  if (I % 128 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "%s: I must be a multiple of 128", name);
+  if (!w2 || !w2_scale) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
+  if (!aligned16(w2)) return fail(B200MOE_ERR_UNSUPPORTED, "%s: weight rows must be 16-byte aligned", name);
   DenseParams p{};
-  st = check_dense_out("b200moe_mlp", M, H, residual, ld_res, out, ld_out, 0, p);
+  st = check_dense_out(name, M, H, residual, ld_res, out, ld_out, 0, p);
   if (st) return st;
   if (M == 0) return B200MOE_OK;
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
-      workspace_bytes < b200moe_mlp_workspace_size(M, H, I))
-    return fail(B200MOE_ERR_WORKSPACE, "b200moe_mlp: workspace too small or not 256-byte aligned%s");
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  st = dense_quantise(in, M, H, ws, stream);
+  const MlpPlan m = plan_mlp(M, H, I, x != nullptr);
+  st = check_dense_work(name, workspace, workspace_bytes, m.total);
   if (st) return st;
-  uint8_t* iq = ws + dense_quant_bytes(M, H);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  uint8_t* iq = ws + m.off_inter;
   float* is = reinterpret_cast<float*>(iq + round_up(M * I, 256));
   DenseParams g{};
   g.q = iq;
   g.ld_q = I;
   g.s = is;
   g.ld_s = I / 128;
-  st = run_dense("b200moe_mlp", DENSE_SILU, in, M, 2 * I, H, w13, H, w13_scale, g, err_word, stream);
+  st = run_dense(name, DENSE_SILU, m.up, in, M, 2 * I, H, w13, H, w13_scale, g, false, ws, err_word, stream);
   if (st) return st;
   const DenseInput mid{nullptr, iq, is, I, I / 128};
-  return run_dense("b200moe_mlp", DENSE_OUT, mid, M, H, I, w2, I, w2_scale, p, err_word, stream);
+  return run_dense(name, DENSE_OUT, m.down, mid, M, H, I, w2, I, w2_scale, p, true, nullptr, err_word, stream);
 }
 
 int b200moe_read_error(int32_t* err_word, int32_t* value, int clear, void* stream) {

@@ -1,6 +1,10 @@
-// Dense FP8 block-scaled products: launch of the token-major kernel.
+// Dense FP8 block-scaled products: choice and launch of the kernels.
 #include "dense.h"
 
+#include <atomic>
+
+#include "dense_pair.cuh"
+#include "dense_split.cuh"
 #include "dense_tok.cuh"
 #include "launch.h"
 
@@ -8,42 +12,261 @@ namespace b200moe {
 
 namespace {
 
-int sm_count_of_current() {
-  int dev = 0, n = 0;
+constexpr int kMaxDevices = 64;
+
+int current_device() {
+  int dev = 0;
   cudaGetDevice(&dev);
+  return dev;
+}
+
+int sm_count_of(int dev) {
+  static std::atomic<int> cache[kMaxDevices];
+  if (dev >= 0 && dev < kMaxDevices && cache[dev].load() > 0) return cache[dev].load();
+  int n = 0;
   cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 1;
+  if (n <= 0) n = 1;
+  if (dev >= 0 && dev < kMaxDevices) cache[dev].store(n);
+  return n;
+}
+
+// Raises the kernel's shared memory limit once per device.
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes, int dev, std::atomic<int> (&done)[kMaxDevices]) {
+  if (dev >= 0 && dev < kMaxDevices && done[dev].load() >= bytes) return cudaSuccess;
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess && dev >= 0 && dev < kMaxDevices) done[dev].store(bytes);
+  return err;
+}
+
+// Launch attributes of every kernel here: a cluster of R CTAs, programmatic
+// order behind the kernel ahead of it.
+void cluster_launch(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int R, dim3 grid, int threads, int smem,
+                    cudaStream_t stream) {
+  cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = R;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = B200MOE_PDL ? 2 : 1;
+}
+
+// Tiles are taken in groups of this many token tiles: CTAs that run at the same
+// time then share weight tiles and activations through L2.
+constexpr int kTileGroup = 8;
+
+template <int EPI>
+cudaError_t launch_tok_dense(const DensePlan& pl, const CUtensorMap& tm_x, const CUtensorMap& tm_w,
+                             const DenseParams& p, bool early_w, cudaStream_t stream) {
+  using C = DenseTokCfg;
+  static std::atomic<int> done[kMaxDevices];
+  auto kernel = dense_tok_kernel<EPI>;
+  const cudaError_t err = allow_smem(kernel, C::SMEM_BYTES, current_device(), done);
+  if (err != cudaSuccess) return err;
+  const int n_mt = (p.M + C::TM - 1) / C::TM, n_nt = (p.N + C::TN - 1) / C::TN;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  cluster_launch(cfg, attr, pl.splits, dim3((unsigned)n_mt * n_nt * pl.splits), C::THREADS, C::SMEM_BYTES, stream);
+  return cudaLaunchKernelEx(&cfg, kernel, tm_x, tm_w, p, pl.splits, n_mt, n_nt, kTileGroup,
+                            early_w && B200MOE_PDL ? 1 : 0);
+}
+
+// Shared memory of a CTA of the split kernel. A CTA that waits for TMEM holds its
+// place in its cluster, and two clusters that wait for each other's TMEM never
+// end: so the CTAs that fit on an SM together (of one launch or of several
+// streams) must also have TMEM enough. The sizes see to it: at most two CTAs of
+// this kernel, with half of the TMEM each (3 x 79 KB > 228 KB, 1 KB of each the
+// system's), and none beside a CTA that takes all of it, as the token-major, pair
+// and expert kernels do with 194 KB and more.
+constexpr int kSplitSmem = 113 * 1024, kSplitSmemMin = 78 * 1024;
+static_assert(DenseTokCfg::SMEM_BYTES + kSplitSmemMin + 2048 > 228 * 1024 &&
+                  DensePairCfg::SMEM_BYTES + kSplitSmemMin + 2048 > 228 * 1024,
+              "no split CTA beside one that takes all of the TMEM");
+
+// Stages that fit next to the scales (and quantised rows) of nkb K blocks, or 0.
+template <int T>
+int split_stages(int nkb, int tt, bool qx) {
+  using C = DenseSplitCfg<T>;
+  int n = nkb < C::MAX_STAGE ? nkb : C::MAX_STAGE;
+  while (n * C::tile_bytes(tt, qx) < tt * 512) ++n;  // the CTA's sums reuse the tiles
+  while (n > 1 && C::smem_bytes(n, nkb, tt, qx) > kSplitSmem) --n;
+  const bool fits = C::smem_bytes(n, nkb, tt, qx) <= kSplitSmem && n * C::tile_bytes(tt, qx) >= tt * 512 &&
+                    (n >= 2 || nkb == 1);
+  return fits ? n : 0;
+}
+
+template <int EPI, int T, bool QX>
+cudaError_t launch_split_dense(const DensePlan& pl, const CUtensorMap& tm_x, const CUtensorMap& tm_w,
+                               const DenseParams& p, bool early_w, cudaStream_t stream) {
+  using C = DenseSplitCfg<T>;
+  constexpr int HALVES = EPI == DENSE_SILU ? 2 : 1;
+  static std::atomic<int> done[kMaxDevices];
+  auto kernel = dense_split_kernel<EPI, T, QX>;
+  const int nkb = ((p.K >> 7) + pl.splits - 1) / pl.splits;
+  const int nstage = split_stages<T>(nkb, pl.tokens, QX);
+  if (nstage == 0) return cudaErrorInvalidValue;
+  int smem = C::smem_bytes(nstage, nkb, pl.tokens, QX);
+  if (smem < kSplitSmemMin) smem = kSplitSmemMin;
+  cudaError_t err = allow_smem(kernel, smem, current_device(), done);
+  if (err != cudaSuccess) return err;
+  const int R = HALVES * pl.splits;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  cluster_launch(cfg, attr, R,
+                 dim3((unsigned)((p.N + 128 * HALVES - 1) / (128 * HALVES) * R),
+                      (unsigned)((p.M + pl.tokens - 1) / pl.tokens), 1),
+                 C::THREADS, smem, stream);
+  return cudaLaunchKernelEx(&cfg, kernel, tm_x, tm_w, p, pl.splits, pl.tokens, nstage,
+                            early_w && B200MOE_PDL ? 1 : 0);
+}
+
+// Clusters of R CTAs of a kernel that are resident at once on the current device.
+template <typename K>
+int resident_clusters(K kernel, int R, int threads, int smem, std::atomic<int> (&cache)[kMaxDevices][9]) {
+  const int dev = current_device();
+  const bool known = dev >= 0 && dev < kMaxDevices;
+  if (known && cache[dev][R].load() > 0) return cache[dev][R].load();
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  cluster_launch(cfg, attr, R, dim3(R), threads, smem, nullptr);
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = sm_count_of(dev) / R > 0 ? sm_count_of(dev) / R : 1;  // no such device: any plan will do
+  }
+  if (known) cache[dev][R].store(n);
+  return n;
+}
+int resident_split(int R) {
+  static std::atomic<int> cache[kMaxDevices][9];
+  return resident_clusters(dense_split_kernel<DENSE_OUT, 64, false>, R, DenseSplitCfg<64>::THREADS, kSplitSmem, cache);
+}
+int resident_tok(int R) {
+  static std::atomic<int> cache[kMaxDevices][9];
+  return resident_clusters(dense_tok_kernel<DENSE_OUT>, R, DenseTokCfg::THREADS, DenseTokCfg::SMEM_BYTES, cache);
+}
+int resident_pairs() {
+  static std::atomic<int> cache[kMaxDevices][9];
+  return resident_clusters(dense_pair_kernel<DENSE_OUT>, 2, DensePairCfg::THREADS, DensePairCfg::SMEM_BYTES, cache);
 }
 
 template <int EPI>
-cudaError_t launch_tok_dense(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const DenseParams& p,
-                             cudaStream_t stream) {
-  using C = DenseTokCfg;
-  auto kernel = dense_tok_kernel<EPI>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+cudaError_t launch_pair_dense(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const DenseParams& p,
+                              cudaStream_t stream) {
+  using C = DensePairCfg;
+  static std::atomic<int> done[kMaxDevices];
+  auto kernel = dense_pair_kernel<EPI>;
+  cudaError_t err = allow_smem(kernel, C::SMEM_BYTES, current_device(), done);
   if (err != cudaSuccess) return err;
-  const int n_mt = (p.M + C::TM - 1) / C::TM, n_nt = (p.N + C::TN - 1) / C::TN;
+  const int n_mt = (p.M + 2 * C::TM - 1) / (2 * C::TM), n_nt = (p.N + C::TN - 1) / C::TN;
   const int64_t units = (int64_t)n_mt * n_nt;
-  const int sms = sm_count_of_current();
-  const int grid = units < sms ? (int)units : sms;
-  return launch_pdl(kernel, dim3(grid), dim3(C::THREADS), C::SMEM_BYTES, stream, tm_x, tm_w, p, n_mt, n_nt, 8);
+  const int pairs = units < resident_pairs() ? (int)units : resident_pairs();
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  cluster_launch(cfg, attr, 2, dim3(2 * pairs), C::THREADS, C::SMEM_BYTES, stream);
+  return cudaLaunchKernelEx(&cfg, kernel, tm_x, tm_w, p, n_mt, n_nt, kTileGroup);
+}
+
+template <int EPI>
+cudaError_t launch_epi_dense(const DensePlan& pl, const CUtensorMap& tm_x, const CUtensorMap& tm_w,
+                             const DenseParams& p, bool early_w, cudaStream_t stream) {
+  switch (pl.cfg) {
+    case 16:
+      if (pl.quantise_x) return launch_split_dense<EPI, 16, true>(pl, tm_x, tm_w, p, early_w, stream);
+      if constexpr (EPI == DENSE_OUT) return launch_split_dense<EPI, 16, false>(pl, tm_x, tm_w, p, early_w, stream);
+      return cudaErrorInvalidValue;
+    case 32:
+      if constexpr (EPI == DENSE_OUT) return launch_split_dense<EPI, 32, false>(pl, tm_x, tm_w, p, early_w, stream);
+      return cudaErrorInvalidValue;
+    case 64:
+      if constexpr (EPI == DENSE_OUT) return launch_split_dense<EPI, 64, false>(pl, tm_x, tm_w, p, early_w, stream);
+      return cudaErrorInvalidValue;
+    case kDensePair:
+      return launch_pair_dense<EPI>(tm_x, tm_w, p, stream);
+    default:
+      return launch_tok_dense<EPI>(pl, tm_x, tm_w, p, early_w, stream);
+  }
 }
 
 }  // namespace
 
-DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K) {
-  (void)epi;
-  (void)M;
-  (void)N;
-  (void)K;
-  return DensePlan{DenseTokCfg::TM, DenseTokCfg::TN};
+namespace {
+
+// The split kernel for these sizes, or cfg = kDenseTok when it does not suit.
+DensePlan split_plan(int epi, int64_t M, int64_t N, int nkb, bool x_bf16) {
+  DensePlan pl{};
+  pl.cfg = kDenseTok;
+  const int halves = epi == DENSE_SILU ? 2 : 1;
+  const int64_t n_tt = (M + 63) / 64;
+  const int tt = (int)((M + n_tt - 1) / n_tt + 15) / 16 * 16;
+  const int T = tt <= 16 ? 16 : (tt <= 32 ? 32 : 64);
+  const int64_t units = (N + 128 * halves - 1) / (128 * halves) * n_tt;
+  // More than 64 tokens read the weights more than once, which only pays when
+  // the tiles are too few to fill the device otherwise: 100 x 576 x 7168 takes
+  // 7.7 us this way and 11.0 token-major, 100 x 4096 x 6144 15.3 and 12.8.
+  if (M > 64 && units > resident_split(8)) return pl;
+  // The most CTAs along K that still run in one wave, with at least two K blocks
+  // each: 6144 x 2048 takes 6.2 us with 4, 6.8 with 2 and, two waves, 10.8 with 6.
+  int s = 8 / halves;
+  while (s > 1 && (s * 2 > nkb || units > resident_split(s * halves))) --s;
+  const int per = (nkb + s - 1) / s;
+  bool qx = x_bf16 && T == 16 && M * per <= kQuantGroups && split_stages<16>(per, tt, true) > 0;
+  // Gate/up with rows of 256 columns to a CTA (token-major) is as fast from the
+  // first token on (9.8 against 10.0 us at 1, 11.8 against 12.4 at 64), so here it
+  // is only for saving the quantising launch.
+  if (epi == DENSE_SILU && !qx) return pl;
+  const int stages = qx ? 1
+                        : (T == 16 ? split_stages<16>(per, tt, false)
+                                   : (T == 32 ? split_stages<32>(per, tt, false) : split_stages<64>(per, tt, false)));
+  if (stages == 0) return pl;
+  pl.cfg = T;
+  pl.tokens = tt;
+  pl.splits = s;
+  pl.quantise_x = qx;
+  pl.x_box_rows = tt;
+  pl.w_box_rows = 128;
+  return pl;
+}
+
+}  // namespace
+
+DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K, bool x_bf16) {
+  const int nkb = (int)(K / 128);
+  DensePlan pl = split_plan(epi, M, N, nkb, x_bf16);
+  if (pl.cfg != kDenseTok) return pl;
+  // Token-major tiles while a cluster of two or more CTAs can share each (512 x
+  // 4096 x 6144: 20.9 us against 30.7 with pairs), pairs from there on (1024: 31.5
+  // against 32.9; 2048: 59.5 against 64.3).
+  using T = DenseTokCfg;
+  const int64_t units = (M + T::TM - 1) / T::TM * ((N + T::TN - 1) / T::TN);
+  if (units > resident_tok(2)) {
+    pl.cfg = kDensePair;
+    pl.splits = 1;
+    pl.x_box_rows = DensePairCfg::TM;
+    pl.w_box_rows = DensePairCfg::WR;
+    return pl;
+  }
+  int s = 8;
+  while (s > 1 && (s * 2 > nkb || units > resident_tok(s))) --s;
+  pl.splits = s;
+  pl.x_box_rows = T::TM;
+  pl.w_box_rows = T::TN;
+  return pl;
 }
 
 cudaError_t launch_dense(int epi, const DensePlan& pl, const CUtensorMap& tm_x, const CUtensorMap& tm_w,
-                         const DenseParams& p, cudaStream_t stream) {
-  (void)pl;
-  return epi == DENSE_SILU ? launch_tok_dense<DENSE_SILU>(tm_x, tm_w, p, stream)
-                           : launch_tok_dense<DENSE_OUT>(tm_x, tm_w, p, stream);
+                         const DenseParams& p, bool early_w, cudaStream_t stream) {
+  return epi == DENSE_SILU ? launch_epi_dense<DENSE_SILU>(pl, tm_x, tm_w, p, early_w, stream)
+                           : launch_epi_dense<DENSE_OUT>(pl, tm_x, tm_w, p, early_w, stream);
 }
 
 }  // namespace b200moe

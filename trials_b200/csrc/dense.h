@@ -11,6 +11,8 @@ namespace b200moe {
 struct DenseParams {
   const float* xs;  // activation scales: row m, K block kb at xs[m * ld_xs + kb]
   int64_t ld_xs;
+  const void* xb;   // bf16 rows instead (plan.quantise_x): row m at xb + m * ld_xb
+  int64_t ld_xb;
   const float* ws;  // weight scales (ceil(N/128), K/128)
   int M, N, K;
   // DENSE_OUT: out[m * ld_out + n] = y (+ residual[m * ld_res + n])
@@ -31,13 +33,21 @@ struct DenseParams {
 
 enum { DENSE_OUT = 0, DENSE_SILU = 1 };
 
-// How a product is cut up (dense_plan), and the boxes its tensor maps need.
+// How a product is cut up, and the boxes its tensor maps need.
+constexpr int kDenseTok = 0, kDensePair = 1;
 struct DensePlan {
+  int cfg;     // kDenseTok, kDensePair, or the split kernel's T (dense_split.cuh)
+  int tokens;  // split kernel: tokens of a tile, a multiple of 16 up to T
+  int splits;  // split and token-major kernel: CTAs that share K
+  int quantise_x;  // bf16 rows are quantised inside the kernel
   int x_box_rows;
   int w_box_rows;
 };
-DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K);
+// x_bf16: the rows come in bf16 (quantise_x can only be set then).
+DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K, bool x_bf16);
+// early_w: the kernel ahead of this one in the stream belongs to the same call
+// and does not write w.
 cudaError_t launch_dense(int epi, const DensePlan& pl, const CUtensorMap& tm_x, const CUtensorMap& tm_w,
-                         const DenseParams& p, cudaStream_t stream);
+                         const DenseParams& p, bool early_w, cudaStream_t stream);
 
 }  // namespace b200moe

@@ -1,0 +1,224 @@
+// Parts shared by the dense FP8 block-scaled product kernels.
+#pragma once
+
+#include "common.cuh"
+#include "dense.h"
+#include "moe_gemm.cuh"
+#include "moe_gemm_tok.cuh"
+#include "ptx.cuh"
+
+namespace b200moe {
+
+// acc += sc * (this warp's 32 TMEM lanes x NC columns from taddr on), LB 16-column
+// loads to a wait. Loads in flight behind the fmas, and releasing the buffer
+// before the last fmas, measured 1-5% slower.
+template <int NC, int LB>
+__device__ __forceinline__ void promote(float (&acc)[NC], uint32_t taddr, float sc) {
+#pragma unroll
+  for (int c0 = 0; c0 < NC / 16; c0 += LB) {
+    uint32_t v[LB][16];
+#pragma unroll
+    for (int b = 0; b < LB; ++b) tmem_ld16(taddr + (c0 + b) * 16, v[b]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int b = 0; b < LB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) tmem_reg_fence(v[b][i]);
+#pragma unroll
+    for (int b = 0; b < LB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2)
+        ffma2(acc[(c0 + b) * 16 + i], acc[(c0 + b) * 16 + i + 1], __uint_as_float(v[b][i]),
+              __uint_as_float(v[b][i + 1]), sc);
+  }
+}
+
+// silu(gate) * up of a token's NC / 2 (gate, up) pairs into acc[0 .. NC/2 - 1];
+// returns their largest magnitude.
+template <int NC>
+__device__ __forceinline__ float silu_pairs(float (&acc)[NC]) {
+  float mx = 0.f;
+#pragma unroll
+  for (int i = 0; i < NC / 2; ++i) {
+    acc[i] = silu_f32(acc[2 * i]) * acc[2 * i + 1];
+    mx = fmaxf(mx, fabsf(acc[i]));
+  }
+  return mx;
+}
+
+// acc[0 .. NC/2 - 1] quantised with `scale` to consecutive codes (16-byte aligned).
+template <int NC>
+__device__ __forceinline__ void store_codes(const float (&acc)[NC], float scale, uint8_t* q) {
+#pragma unroll
+  for (int k = 0; k < NC / 32; ++k) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) w[i] |= (uint32_t)quant_e4m3(acc[k * 16 + i * 4 + t], scale) << (8 * t);
+    }
+    reinterpret_cast<uint4*>(q)[k] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// Stores 32 rows (m0.., one per lane) x NC columns (n0..) of fp32 results. They
+// pass through st (4 KB of this warp, rows of 32 columns, 16-byte pieces
+// swizzled by row), so that a store instruction covers whole 64-byte (bf16) or
+// 128-byte (f32) runs of 4 rows, or 32 consecutive columns of one row where
+// rows are not aligned.
+template <int NC>
+__device__ __forceinline__ void dense_store_tile(const DenseParams& p, int m0, int n0, const float (&acc)[NC],
+                                                 uint8_t* st, int lane) {
+  const int rows = p.M - m0 < 32 ? p.M - m0 : 32;
+#pragma unroll
+  for (int cb = 0; cb < NC / 32; ++cb) {
+    const int n1 = n0 + cb * 32;
+    if (n1 < p.N) {  // warp-uniform
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<float4*>(st + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+            make_float4(acc[cb * 32 + 4 * c], acc[cb * 32 + 4 * c + 1], acc[cb * 32 + 4 * c + 2],
+                        acc[cb * 32 + 4 * c + 3]);
+      __syncwarp();
+      if (p.vec) {  // N is a multiple of 8: a piece of 4 columns exists or does not
+        const int c = lane & 7, n = n1 + 4 * c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + (lane >> 3);
+          if (r < rows && n < p.N) {
+            float4 v = *reinterpret_cast<const float4*>(st + r * 128 + ((c ^ (r & 7)) << 4));
+            const int64_t m = m0 + r;
+            if (p.residual) {
+              const uint2 raw = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.residual) +
+                                                                m * p.ld_res + n);
+              const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
+              const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+              v.x += lo.x;
+              v.y += lo.y;
+              v.z += hi.x;
+              v.w += hi.y;
+            }
+            if (p.out_f32) {
+              *reinterpret_cast<float4*>(static_cast<float*>(p.out) + m * p.ld_out + n) = v;
+            } else {
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+              uint2 pk;
+              pk.x = *reinterpret_cast<const uint32_t*>(&lo);
+              pk.y = *reinterpret_cast<const uint32_t*>(&hi);
+              *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + m * p.ld_out + n) = pk;
+            }
+          }
+        }
+      } else if (n1 + lane < p.N) {
+        for (int r = 0; r < rows; ++r) {
+          float v = *reinterpret_cast<const float*>(st + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+          const int64_t m = m0 + r;
+          const int n = n1 + lane;
+          if (p.residual) v += __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[m * p.ld_res + n]);
+          if (p.out_f32) static_cast<float*>(p.out)[m * p.ld_out + n] = v;
+          else static_cast<__nv_bfloat16*>(p.out)[m * p.ld_out + n] = __float2bfloat16_rn(v);
+        }
+      }
+      __syncwarp();
+    }
+  }
+}
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// Four consecutive outputs n..n+3 of token m.
+__device__ __forceinline__ void dense_store4(const DenseParams& p, int64_t m, int n, float4 v) {
+  if (p.vec) {
+    if (n >= p.N) return;
+    if (p.residual) {
+      const uint2 raw =
+          *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.residual) + m * p.ld_res + n);
+      const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
+      const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+      v.x += lo.x;
+      v.y += lo.y;
+      v.z += hi.x;
+      v.w += hi.y;
+    }
+    if (p.out_f32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + m * p.ld_out + n) = v;
+    } else {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+      uint2 pk;
+      pk.x = *reinterpret_cast<const uint32_t*>(&lo);
+      pk.y = *reinterpret_cast<const uint32_t*>(&hi);
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + m * p.ld_out + n) = pk;
+    }
+    return;
+  }
+  const float a[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < p.N) {
+      float y = a[i];
+      if (p.residual) y += __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[m * p.ld_res + n + i]);
+      if (p.out_f32) static_cast<float*>(p.out)[m * p.ld_out + n + i] = y;
+      else static_cast<__nv_bfloat16*>(p.out)[m * p.ld_out + n + i] = __float2bfloat16_rn(y);
+    }
+}
+
+// One warp: row sums of a token over the S CTAs of a cluster that share K, and
+// their epilogue. at(s, h): cluster address of this lane's four columns
+// (4 * lane ..) of 128-column half h in CTA s's sums. Added in the order of s.
+// DENSE_SILU (HALVES = 2): the 256 columns are one 1x128 group of gate/up pairs,
+// output columns 128 * unit ..; DENSE_OUT: columns n0 + 128 * h + 4 * lane ..
+template <int EPI, int HALVES, typename F>
+__device__ __forceinline__ void finish_token(const DenseParams& p, int64_t m, int n0, int splits, int lane, F at) {
+  constexpr int MAXS = 8;
+  float4 sum[HALVES];
+#pragma unroll
+  for (int h = 0; h < HALVES; ++h) {
+    float4 v[MAXS];
+#pragma unroll
+    for (int s = 0; s < MAXS; ++s)
+      if (s < splits) v[s] = ld_cluster_f4(at(s, h));
+    sum[h] = v[0];
+#pragma unroll
+    for (int s = 1; s < MAXS; ++s)
+      if (s < splits) {
+        sum[h].x += v[s].x;
+        sum[h].y += v[s].y;
+        sum[h].z += v[s].z;
+        sum[h].w += v[s].w;
+      }
+  }
+  if constexpr (EPI == DENSE_SILU) {
+    static_assert(HALVES == 2, "a group of gate/up pairs is 256 columns");
+    // lane: inter columns 2 * lane, 2 * lane + 1 of each 64-column half
+    float y[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      y[2 * h] = silu_f32(sum[h].x) * sum[h].y;
+      y[2 * h + 1] = silu_f32(sum[h].z) * sum[h].w;
+    }
+    float mx = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float scale = group_scale(mx);
+    const int unit = n0 >> 8;
+    uint8_t* dst = p.q + m * p.ld_q + unit * 128 + lane * 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *reinterpret_cast<uint16_t*>(dst + h * 64) =
+          (uint16_t)(quant_e4m3(y[2 * h], scale) | (quant_e4m3(y[2 * h + 1], scale) << 8));
+    if (lane == 0) p.s[m * p.ld_s + unit] = scale;
+  } else {
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) dense_store4(p, m, n0 + 128 * h + lane * 4, sum[h]);
+  }
+}
+
+}  // namespace b200moe

@@ -14,96 +14,130 @@ the current torch stream of its tensors' device; there is no fallback path.
 """
 from __future__ import annotations
 
-import contextlib
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .moe import FP8, _ptr, _require_cuda, _stream, _workspaces
+from .moe import FP8, _require_cuda, _stream, _workspaces
+
+# These calls take a few microseconds on the GPU for a few tokens, so the checks
+# below read each attribute once and build no intermediate objects.
 
 
-def _on_device(dev: torch.device):
-    """Kernels launch on the current device: make it the tensors' device."""
-    if torch.cuda.current_device() == dev.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+def _device_of(x: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """Index of the one CUDA device all tensors are on."""
+    index = x.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            _require_cuda(x, *others)  # says what is wrong
+    if index < 0:
+        _require_cuda(x)
+    return index
+
+
+def _call(fn, where: str, index: int, args: tuple) -> None:
+    """Calls a C entry on the current stream of device `index` (kernels launch on
+    the current device); args end before the error word and the stream. The error
+    word is the cached one of (device, stream) (moe.layer_error_word)."""
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _call(fn, where, index, args)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    status = fn(*args, _workspaces.error_ptr(index, stream), stream)
+    if status:
+        _lib.check(status, where)
 
 
 def _rows(t: torch.Tensor, what: str) -> int:
     """Row stride in elements of a 2-D tensor whose rows are contiguous."""
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    s0, s1 = t.stride()
+    n, m = t.shape
+    if m > 1 and s1 != 1:
         raise ValueError(f"{what}: elements of a row must be contiguous")
-    if t.shape[0] <= 1:
-        return t.shape[1]  # the stride of a single row says nothing
-    if t.stride(0) < t.shape[1]:
+    if n <= 1:
+        return m  # the stride of a single row says nothing
+    if s0 < m:
         raise ValueError(f"{what}: rows must not overlap")
-    return t.stride(0)
-
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy whose rows are contiguous and start 16-byte aligned."""
-    size = t.element_size()
-    ok = (t.stride(1) == 1 and (t.shape[0] <= 1 or (t.stride(0) * size % 16 == 0 and t.stride(0) >= t.shape[1]))
-          and t.data_ptr() % 16 == 0)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    return s0
 
 
 def _input(x: torch.Tensor, x_scale: Optional[torch.Tensor]):
-    """Checked activation rows and scales, copied only where their layout asks for it."""
+    """Checked activation rows and scales and their row strides, copied only where
+    their layout asks for it: (x, x_scale, stride of x, stride of x_scale)."""
     if x.dim() != 2:
         raise ValueError("x must be (M, K)")
+    M, K = x.shape
+    ld_s = 0
     if x.dtype == FP8:
-        if x_scale is None or x_scale.dim() != 2 or tuple(x_scale.shape) != (x.shape[0], x.shape[1] // 128):
+        size = 1
+        if x_scale is None or x_scale.shape != (M, K // 128):
             raise ValueError("fp8 x needs x_scale of shape (M, K/128) (1x128 per-token-group scales)")
         if x_scale.dtype != torch.float32:
             raise NotImplementedError("x_scale must be float32")
-        if x_scale.stride(1) != 1 or (x_scale.shape[0] > 1 and x_scale.stride(0) < x_scale.shape[1]):
+        ld_s, s1 = x_scale.stride()
+        if s1 != 1 or (M > 1 and ld_s < K // 128):
             x_scale = x_scale.contiguous()
+            ld_s = K // 128
+        elif M <= 1:
+            ld_s = K // 128
     elif x.dtype == torch.bfloat16:
+        size = 2
         if x_scale is not None:
             raise ValueError("x_scale is only meaningful with fp8 x")
     else:
         raise NotImplementedError("x must be bf16, or fp8 e4m3 with (M, K/128) x_scale")
-    if x.shape[1] == 0 or x.shape[1] % 128:
+    if K == 0 or K % 128:
         raise NotImplementedError("K must be a multiple of 128")
-    return _aligned(x), x_scale
+    s0, s1 = x.stride()
+    if M <= 1:
+        s0 = K
+    if s1 != 1 or s0 < K or s0 * size % 16 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        s0 = K
+    return x, x_scale, s0, ld_s
 
 
 def _weight(w: torch.Tensor, scale: torch.Tensor, K: int, what: str):
+    """(row stride of the weight, contiguous scales), checked."""
     if w.dtype != FP8:
         raise NotImplementedError(f"{what} must be float8_e4m3fn with 128x128 block scales")
     if w.dim() != 2 or w.shape[1] != K or w.shape[0] == 0:
         raise ValueError(f"{what} must be (N, {K}), got {tuple(w.shape)}")
     if scale.dtype != torch.float32:
         raise NotImplementedError(f"{what}_scale must be float32")
-    if tuple(scale.shape) != ((w.shape[0] + 127) // 128, K // 128):
+    if scale.shape != ((w.shape[0] + 127) // 128, K // 128):
         raise ValueError(f"{what}_scale must be (ceil(N/128), K/128), got {tuple(scale.shape)}")
-    return _rows(w, what), scale.contiguous()
+    return _rows(w, what), scale if scale.is_contiguous() else scale.contiguous()
 
 
 def _output(out: Optional[torch.Tensor], residual: Optional[torch.Tensor], M: int, N: int, dtype: torch.dtype,
             dev: torch.device):
+    """(out, its row stride, the residual's row stride), checked."""
     if out is None:
         out = torch.empty(M, N, dtype=dtype, device=dev)
-    elif tuple(out.shape) != (M, N) or out.dtype != dtype:
-        raise ValueError(f"out must be ({M}, {N}) {dtype}")
-    if residual is not None:
-        if residual.dtype != torch.bfloat16:
-            raise NotImplementedError("residual must be bf16")
-        if tuple(residual.shape) != (M, N):
-            raise ValueError(f"residual must be ({M}, {N})")
-    return out, residual
+        ld = N
+    else:
+        if out.shape != (M, N) or out.dtype != dtype:
+            raise ValueError(f"out must be ({M}, {N}) {dtype}")
+        ld = _rows(out, "out")
+    if residual is None:
+        return out, ld, 0
+    if residual.dtype != torch.bfloat16:
+        raise NotImplementedError("residual must be bf16")
+    if residual.shape != (M, N):
+        raise ValueError(f"residual must be ({M}, {N})")
+    return out, ld, _rows(residual, "residual")
 
 
-def _call_state(dev: torch.device, nbytes: int):
-    """(stream, error word pointer, workspace) of one call. The workspace is
-    this call's own, from torch's allocator on the current stream; the error
-    word is the cached one of (device, stream) (moe.layer_error_word)."""
-    stream = _stream(dev)
-    err = _workspaces.get_for(dev, stream, 256).data_ptr()
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    return stream, err, ws
+def _workspace(nbytes: int, dev: torch.device):
+    """(tensor to hold until the call returns, pointer, size): this call's own, from
+    torch's allocator on the current stream, so calls on other streams and captured
+    graphs have theirs."""
+    if nbytes == 0:
+        return None, None, 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return ws, ws.data_ptr(), nbytes
 
 
 def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -114,26 +148,28 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     weight_scale (ceil(N/128), K/128) f32; residual (M, N) bf16, added in fp32.
     Accumulated in fp32 and rounded once to out_dtype (bf16 or f32). Any M and
     N; K % 128 == 0. out may be residual itself. See b200moe_linear."""
-    dev = _require_cuda(x, weight, weight_scale, x_scale, residual, out)
-    if out_dtype not in (torch.bfloat16, torch.float32):
+    index = _device_of(x, weight, weight_scale, x_scale, residual, out)
+    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
         raise NotImplementedError("out_dtype must be bf16 or float32")
-    x, x_scale = _input(x, x_scale)
+    x, x_scale, ld_x, ld_s = _input(x, x_scale)
     M, K = x.shape
     N = weight.shape[0]
+    dev = x.device
     ld_w, weight_scale = _weight(weight, weight_scale, K, "weight")
-    out, residual = _output(out, residual, M, N, out_dtype, dev)
+    out, ld_out, ld_res = _output(out, residual, M, N, out_dtype, dev)
     if M == 0:
         return out
     L = _lib.lib()
-    quantised = x_scale is not None
-    with _on_device(dev):
-        stream, err, ws = _call_state(dev, 0 if quantised else L.b200moe_linear_workspace_size(M, K))
-        _lib.check(L.b200moe_linear(
-            None if quantised else x.data_ptr(), x.data_ptr() if quantised else None, _ptr(x_scale), _rows(x, "x"),
-            _rows(x_scale, "x_scale") if quantised else 0, M, N, K, weight.data_ptr(), ld_w, weight_scale.data_ptr(),
-            _ptr(residual), 0 if residual is None else _rows(residual, "residual"), out.data_ptr(),
-            _rows(out, "out"), int(out_dtype == torch.float32), _ptr(ws), 0 if ws is None else ws.numel(), err,
-            stream), "fp8_block_linear")
+    if x_scale is None:
+        ws, ws_ptr, ws_bytes = _workspace(L.b200moe_linear_workspace_size(M, N, K, 1, 0), dev)
+        rows = (x.data_ptr(), None, None)
+    else:
+        ws_ptr, ws_bytes = None, 0
+        rows = (None, x.data_ptr(), x_scale.data_ptr())
+    _call(L.b200moe_linear, "fp8_block_linear", index,
+          (*rows, ld_x, ld_s, M, N, K, weight.data_ptr(), ld_w, weight_scale.data_ptr(),
+           None if residual is None else residual.data_ptr(), ld_res, out.data_ptr(), ld_out,
+           out_dtype is torch.float32, ws_ptr, ws_bytes))
     return out
 
 
@@ -142,9 +178,10 @@ def fp8_gate_up(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, x_s
     (gate, up) = x . w13^T with gate/up rows interleaved (row 2j = gate j, 2j+1 =
     up j). x as in fp8_block_linear; w13 (2I, H) fp8 e4m3, w13_scale (2I/128,
     H/128) f32; I % 128 == 0. See b200moe_gate_up."""
-    dev = _require_cuda(x, w13, w13_scale, x_scale)
-    x, x_scale = _input(x, x_scale)
+    index = _device_of(x, w13, w13_scale, x_scale)
+    x, x_scale, ld_x, ld_s = _input(x, x_scale)
     M, H = x.shape
+    dev = x.device
     ld_w, w13_scale = _weight(w13, w13_scale, H, "w13")
     if w13.shape[0] % 256:
         raise NotImplementedError("w13 must have 2I rows with I a multiple of 128")
@@ -154,14 +191,15 @@ def fp8_gate_up(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, x_s
     if M == 0:
         return q, s
     L = _lib.lib()
-    quantised = x_scale is not None
-    with _on_device(dev):
-        stream, err, ws = _call_state(dev, 0 if quantised else L.b200moe_linear_workspace_size(M, H))
-        _lib.check(L.b200moe_gate_up(
-            None if quantised else x.data_ptr(), x.data_ptr() if quantised else None, _ptr(x_scale), _rows(x, "x"),
-            _rows(x_scale, "x_scale") if quantised else 0, M, H, I, w13.data_ptr(), ld_w, w13_scale.data_ptr(),
-            q.data_ptr(), I, s.data_ptr(), I // 128, _ptr(ws), 0 if ws is None else ws.numel(), err, stream),
-            "fp8_gate_up")
+    if x_scale is None:
+        ws, ws_ptr, ws_bytes = _workspace(L.b200moe_linear_workspace_size(M, 2 * I, H, 1, 1), dev)
+        rows = (x.data_ptr(), None, None)
+    else:
+        ws_ptr, ws_bytes = None, 0
+        rows = (None, x.data_ptr(), x_scale.data_ptr())
+    _call(L.b200moe_gate_up, "fp8_gate_up", index,
+          (*rows, ld_x, ld_s, M, H, I, w13.data_ptr(), ld_w, w13_scale.data_ptr(), q.data_ptr(), I, s.data_ptr(),
+           I // 128, ws_ptr, ws_bytes))
     return q, s
 
 
@@ -171,9 +209,10 @@ def fp8_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
     """(M, H) bf16 = w2 . (silu(gate) * up) (+ residual): fp8_gate_up with w13
     (2I, H), then fp8_block_linear with w2 (H, I), in one call (same bits).
     out may be residual itself. See b200moe_mlp."""
-    dev = _require_cuda(x, w13, w13_scale, w2, w2_scale, x_scale, residual, out)
-    x, x_scale = _input(x, x_scale)
+    index = _device_of(x, w13, w13_scale, w2, w2_scale, x_scale, residual, out)
+    x, x_scale, ld_x, ld_s = _input(x, x_scale)
     M, H = x.shape
+    dev = x.device
     ld13, w13_scale = _weight(w13, w13_scale, H, "w13")
     if w13.shape[0] % 256:
         raise NotImplementedError("w13 must have 2I rows with I a multiple of 128")
@@ -183,17 +222,13 @@ def fp8_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
         raise ValueError(f"w2 must be ({H}, {I}), got {tuple(w2.shape)}")
     if ld13 != H or ld2 != I:
         raise ValueError("w13 and w2 must be contiguous")
-    out, residual = _output(out, residual, M, H, torch.bfloat16, dev)
+    out, ld_out, ld_res = _output(out, residual, M, H, torch.bfloat16, dev)
     if M == 0:
         return out
     L = _lib.lib()
-    quantised = x_scale is not None
-    with _on_device(dev):
-        stream, err, ws = _call_state(dev, L.b200moe_mlp_workspace_size(M, H, I))
-        _lib.check(L.b200moe_mlp(
-            None if quantised else x.data_ptr(), x.data_ptr() if quantised else None, _ptr(x_scale), _rows(x, "x"),
-            _rows(x_scale, "x_scale") if quantised else 0, M, H, I, w13.data_ptr(), w13_scale.data_ptr(),
-            w2.data_ptr(), w2_scale.data_ptr(), _ptr(residual),
-            0 if residual is None else _rows(residual, "residual"), out.data_ptr(), _rows(out, "out"), ws.data_ptr(),
-            ws.numel(), err, stream), "fp8_mlp")
+    ws, ws_ptr, ws_bytes = _workspace(L.b200moe_mlp_workspace_size(M, H, I, x_scale is None), dev)
+    rows = (x.data_ptr(), None, None) if x_scale is None else (None, x.data_ptr(), x_scale.data_ptr())
+    _call(L.b200moe_mlp, "fp8_mlp", index,
+          (*rows, ld_x, ld_s, M, H, I, w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(),
+           None if residual is None else residual.data_ptr(), ld_res, out.data_ptr(), ld_out, ws_ptr, ws_bytes))
     return out

@@ -76,8 +76,14 @@ class _Workspaces:
                 self._bufs[key] = buf
             return buf
 
+    def error_ptr(self, index: int, stream: int) -> int:
+        """Address of the error word of (device index, its current stream)."""
+        buf = self._bufs.get((index, stream))
+        return (self.get_for(torch.device("cuda", index), stream, 256) if buf is None else buf).data_ptr()
+
 
 _workspaces = _Workspaces()
+_SCORING = {"softmax": 0, "sigmoid": 1}
 
 
 def read_device_error(err_word: torch.Tensor, clear: bool = True) -> int:
@@ -141,9 +147,10 @@ def select_experts(router_logits: torch.Tensor, top_k: int, scoring_func: str = 
     score is its largest value, with correction_bias the sum of its two largest).
     See b200moe_router_topk_grouped."""
     dev = _require_cuda(router_logits)
-    if router_logits.dtype not in (torch.float32, torch.bfloat16):
+    bf16 = router_logits.dtype == torch.bfloat16
+    if not bf16 and router_logits.dtype != torch.float32:
         raise NotImplementedError("router logits must be float32 or bfloat16")
-    scoring = {"softmax": 0, "sigmoid": 1}.get(scoring_func)
+    scoring = _SCORING.get(scoring_func)
     if scoring is None:
         raise NotImplementedError(f"scoring_func {scoring_func!r}")
     logits = router_logits.contiguous()
@@ -153,9 +160,8 @@ def select_experts(router_logits: torch.Tensor, top_k: int, scoring_func: str = 
     bias = None if correction_bias is None else correction_bias.to(device=dev, dtype=torch.float32).contiguous()
     if _check_groups(num_expert_group, topk_group):
         _lib.check(_lib.lib().b200moe_router_topk_grouped(
-            _ptr(logits), int(logits.dtype == torch.bfloat16), M, E, num_expert_group, topk_group, top_k, scoring,
-            _ptr(bias), int(renormalize), float(routed_scaling_factor), _ptr(w), _ptr(ids), _stream(dev)),
-            "select_experts")
+            logits.data_ptr(), bf16, M, E, num_expert_group, topk_group, top_k, scoring, _ptr(bias),
+            bool(renormalize), routed_scaling_factor, w.data_ptr(), ids.data_ptr(), _stream(dev)), "select_experts")
         return w, ids
     _lib.check(_lib.lib().b200moe_router_topk(_ptr(logits), int(logits.dtype == torch.bfloat16), M, E, top_k,
                                               scoring, _ptr(bias), int(renormalize), float(routed_scaling_factor),
