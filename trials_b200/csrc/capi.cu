@@ -283,6 +283,23 @@ int check_router(const char* name, const void* logits, int64_t M, int num_expert
   return B200MOE_OK;
 }
 
+RouterArgs grouped_router(const void* logits, int logits_bf16, int num_experts, int num_groups, int topk_groups,
+                          int topk, int scoring, const float* correction_bias, int renormalize, float scaling,
+                          float* topk_weights, int32_t* topk_ids) {
+  RouterArgs r{logits, logits_bf16 ? 1 : 0, num_experts, topk, scoring, renormalize ? 1 : 0,
+               correction_bias, scaling, topk_weights, topk_ids};
+  r.groups = num_groups;
+  r.topk_groups = topk_groups;
+  r.vec = aligned16(logits) && num_experts * (logits_bf16 ? 2 : 4) % 16 == 0;
+  r.vec_bias = aligned16(correction_bias);
+  r.per = grouped_per_lane(num_experts, num_groups);
+  r.gs = num_experts / num_groups;
+  r.span_log2 = -1;
+  for (int j = 0; j < 6; ++j)
+    if (r.per << j == r.gs) r.span_log2 = j;
+  return r;
+}
+
 // The same plus the groups of group-limited routing.
 int check_router_grouped(const char* name, const void* logits, int64_t M, int num_experts, int num_groups,
                          int topk_groups, int topk, int scoring, const float* correction_bias,
@@ -585,8 +602,8 @@ int b200moe_route_logits_grouped(const void* logits, int logits_bf16, int64_t M,
   int st = check_router_grouped("b200moe_route_logits_grouped", logits, M, num_experts, num_groups, topk_groups, topk,
                                 scoring, correction_bias, topk_weights, topk_ids);
   if (st) return st;
-  const RouterArgs r{logits,  logits_bf16 ? 1 : 0, num_experts, topk, scoring, renormalize ? 1 : 0, correction_bias,
-                     scaling, topk_weights,        topk_ids,    num_groups, topk_groups};
+  const RouterArgs r = grouped_router(logits, logits_bf16, num_experts, num_groups, topk_groups, topk, scoring,
+                                      correction_bias, renormalize, scaling, topk_weights, topk_ids);
   return route_impl(topk_ids, M, topk, num_experts, expert_map, num_local_experts, tile_tokens, sorted_ids,
                     rows_capacity, chunk_expert, chunk_row0, chunk_rows, chunks_capacity, n_chunks, num_rows,
                     slot_pos, chunk_ready, route_scratch, route_scratch_ints, err_word, stream, &r, nullptr);
@@ -1175,8 +1192,8 @@ int b200moe_layer_logits_grouped(const void* hidden, int64_t M, int64_t H, int64
   int st = check_router_grouped("b200moe_layer_logits_grouped", router_logits, M, num_experts, num_groups, topk_groups,
                                 topk, scoring, correction_bias, topk_weights, topk_ids);
   if (st) return st;
-  const RouterArgs r{router_logits, logits_bf16 ? 1 : 0, num_experts, topk, scoring, renormalize ? 1 : 0,
-                     correction_bias, scaling, topk_weights, topk_ids, num_groups, topk_groups};
+  const RouterArgs r = grouped_router(router_logits, logits_bf16, num_experts, num_groups, topk_groups, topk, scoring,
+                                      correction_bias, renormalize, scaling, topk_weights, topk_ids);
   LayerInput in{hidden, nullptr, 0, nullptr, 0};
   return layer_core("b200moe_layer_logits_grouped", in, M, H, I, num_experts, topk, w13, w13_scale, w2, w2_scale,
                     topk_weights, topk_ids, expert_map, num_local_experts, out, workspace, workspace_bytes, 0, stream,
@@ -1445,8 +1462,8 @@ int b200moe_router_topk_grouped(const void* logits, int logits_bf16, int64_t M, 
   int st = check_router_grouped("b200moe_router_topk_grouped", logits, M, num_experts, num_groups, topk_groups, topk,
                                 scoring, correction_bias, topk_weights, topk_ids);
   if (st) return st;
-  const RouterArgs r{logits,  logits_bf16 ? 1 : 0, num_experts, topk, scoring, renormalize ? 1 : 0, correction_bias,
-                     scaling, topk_weights,        topk_ids,    num_groups, topk_groups};
+  const RouterArgs r = grouped_router(logits, logits_bf16, num_experts, num_groups, topk_groups, topk, scoring,
+                                      correction_bias, renormalize, scaling, topk_weights, topk_ids);
   return cuda_status(launch_router_topk(r, M, (cudaStream_t)stream), "router_topk_grouped");
 }
 

@@ -38,9 +38,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) router_align_kernel(const Al
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t t = (int64_t)blockIdx.x * tpc + warp;
   if (warp < tpc && t < M) {
-    int id;
-    float w;
-    route_token<PER, GROUPED>(r, t, lane, id, w);
+    route_token<PER, GROUPED>(r, t, lane);
   }
   __threadfence();
   __syncthreads();
@@ -164,9 +162,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_count_kernel(const Ali
   if (ROUTER) {
     const int lane = tid & 31;
     for (int64_t t = beg / r.topk + (tid >> 5); t < end / r.topk; t += kRouteWarps) {
-      int id;
-      float w;
-      route_token<PER, GROUPED>(r, t, lane, id, w);
+      route_token<PER, GROUPED>(r, t, lane);
     }
   }
   __syncthreads();

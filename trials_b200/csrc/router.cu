@@ -16,9 +16,7 @@ __global__ void __launch_bounds__(kRouterWarps * 32) router_topk_kernel(const Ro
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * kRouterWarps + (threadIdx.x >> 5);
   if (t >= M) return;
-  int id;
-  float w;
-  route_token<PER, GROUPED>(r, t, lane, id, w);
+  route_token<PER, GROUPED>(r, t, lane);
 }
 
 template <bool GROUPED>

@@ -32,6 +32,11 @@ struct RouterArgs {
   int32_t* out_ids;    // (M, topk)
   int groups;          // group-limited routing (route_token_grouped); 0 = ungrouped
   int topk_groups;     // groups whose experts may be selected
+  int vec;             // rows of logits start 16-byte aligned (E * element size too)
+  int vec_bias;        // bias 16-byte aligned
+  int per;             // with groups: consecutive experts a lane owns (grouped_per_lane)
+  int gs;              // experts of a group
+  int span_log2;       // log2 of the whole lanes a group fills, -1: groups do not fill lanes
 };
 
 __device__ __forceinline__ float router_logit(const RouterArgs& r, int64_t t, int e) {
@@ -144,26 +149,38 @@ __device__ __forceinline__ void route_token_warp(const RouterArgs& r, int64_t t,
 //   s = softmax(x) or sigmoid(x);  c = s + bias (sigmoid only) or s
 //   group score: without a bias the largest c, with one the sum of the two
 //   largest; best groups, then best experts, equal values lower index first.
-// The selection is the one exact arithmetic on the given f32 (bf16) values
-// makes. Without a bias s is monotone in x, so x itself is compared. With one,
-// c is computed in fp32 and is off by at most ~4e-7 + 6e-8 |c|; when two values
-// whose order matters are closer than kGroupedEps + kGroupedEpsRel * |c| (about
-// one token in a thousand) the token's selection is redone in fp64.
 // NaN logits count as -inf (score 0), NaN c as -inf; a row whose selected
 // scores sum to 0 has weights 0 when renormalised.
 //
-// One warp per token; lane l owns the experts [l * per, (l + 1) * per), so the
-// lowest lane holding a value also holds its lowest id and the warp's argmax is
-// one redux of order-preserving integer keys and one ballot.
+// The selection is the one exact arithmetic on the given f32 (bf16) values
+// makes. Without a bias s is monotone in x, so x itself is compared. With one, c
+// is computed in fp32 and is off by at most 4.5e-7 + 7e-8 |c|. Experts are
+// compared by integer keys in the order of the values whose low bits hold the
+// expert's place in its lane, so the value in a key is off by up to 32 units in
+// the last place (none for bf16 logits, whose low bits are zero). Where two
+// neighbours in the order are closer than the errors (one token in a few
+// hundred), every expert not clearly behind the last one taken joins the
+// candidates, which are put in order by their exact values in fp64; where groups
+// are that close, their scores are computed again in fp64.
+//
+// One warp per token; lane l owns the experts [l * per, (l + 1) * per) (per chosen
+// so that groups fill a power of two of whole lanes wherever it can be), so the
+// lowest lane holding a value also holds its lowest id. What bounds it is the
+// number of instructions a warp issues: a round of the selection is one redux
+// and one ballot on the lanes' best keys, the lists behind them sorted once.
+// 8,192 tokens of 256 experts in 8 groups: 10.9 us with a bias (25.7 with every
+// value compared in turn and each close token redone in fp64), 8.7 without.
 // ---------------------------------------------------------------------------
 constexpr int kRouterMaxGroups = 32;
-constexpr float kGroupedEps = 2e-6f;
-constexpr float kGroupedEpsRel = 5e-7f;
+// Bound of the error of two values c together: the sigmoid's (exp 6e-8 where its
+// slope lets it through, 1 + e 6e-8, the 2-ulp division 2.4e-7) and the addition's
+// half step, twice.
+constexpr float kValueEps = 9e-7f, kValueEpsRel = 1.5e-7f;
 
 // Integers in the order of the floats (-0 = +0); 0 is below every float.
 __device__ __forceinline__ uint32_t order_key(float f) {
   const uint32_t b = __float_as_uint(f + 0.0f);
-  return (b >> 31) ? ~b : (b | 0x80000000u);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float order_value(uint32_t k) {
   return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
@@ -178,24 +195,28 @@ __device__ __forceinline__ void merge_top2(T& a1, T& a2, T b1, T b2) {
 }
 
 // Scores of the groups, group g's in lane g (-inf in the lanes past the last),
-// from this lane's per values c.
+// from this lane's per values c. size: the magnitudes added in the score.
 template <typename T, int PER>
-__device__ __forceinline__ T group_scores(const T (&c)[PER], int E, int groups, int per, bool two, int lane) {
+__device__ __forceinline__ T group_scores(const RouterArgs& r, const T (&c)[PER], bool two, int lane, T& size) {
   const T ninf = -INFINITY;
-  const int gs = E / groups;
-  const int span = gs / per;  // lanes of a group, if its experts fill whole lanes
-  T score = ninf;
-  if (gs % per == 0 && (span & (span - 1)) == 0) {
-    T a1 = ninf, a2 = ninf;
+  const int groups = r.groups, gs = r.gs, per = r.per;
+  two = two && gs > 1;
+  T s1 = ninf, s2 = ninf;
+  if (r.span_log2 >= 0) {
+    const int span = 1 << r.span_log2;
+    T a1 = c[0], a2 = ninf;
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (i < per) merge_top2(a1, a2, c[i], ninf);
+    for (int i = 1; i < PER; ++i) {  // values past `per` are -inf
+      const T lo = a1 < c[i] ? a1 : c[i];
+      a1 = a1 < c[i] ? c[i] : a1;
+      a2 = a2 < lo ? lo : a2;
+    }
     for (int o = 1; o < span; o <<= 1) {
       const T b1 = __shfl_xor_sync(0xffffffffu, a1, o), b2 = __shfl_xor_sync(0xffffffffu, a2, o);
       merge_top2(a1, a2, b1, b2);
     }
-    const T v = two && gs > 1 ? a1 + a2 : a1;
-    score = __shfl_sync(0xffffffffu, v, (lane * span) & 31);
+    s1 = __shfl_sync(0xffffffffu, a1, (lane << r.span_log2) & 31);
+    s2 = __shfl_sync(0xffffffffu, a2, (lane << r.span_log2) & 31);
   } else {
     for (int g = 0; g < groups; ++g) {
       T a1 = ninf, a2 = ninf;
@@ -209,50 +230,63 @@ __device__ __forceinline__ T group_scores(const T (&c)[PER], int E, int groups, 
         const T b1 = __shfl_xor_sync(0xffffffffu, a1, o), b2 = __shfl_xor_sync(0xffffffffu, a2, o);
         merge_top2(a1, a2, b1, b2);
       }
-      const T v = two && gs > 1 ? a1 + a2 : a1;
-      if (lane == g) score = v;
+      if (lane == g) {
+        s1 = a1;
+        s2 = a2;
+      }
     }
   }
-  if (lane >= groups || score != score) score = ninf;
+  const T score = two ? s1 + s2 : s1;
+  if (lane >= groups || score != score) {
+    size = 0;
+    return ninf;
+  }
+  size = (s1 < 0 ? -s1 : s1) + (two ? (s2 < 0 ? -s2 : s2) : T(0));
   return score;
 }
 
-// Rank of lane g's group among the groups (lane < groups).
-template <typename T>
-__device__ __forceinline__ int group_rank(T score, int groups, int lane) {
-  int rank = 0;
-  for (int h = 0; h < groups; ++h) {
-    const T other = __shfl_sync(0xffffffffu, score, h);
-    rank += (other > score || (other == score && h < lane)) ? 1 : 0;
-  }
-  return rank;
+// Expert e's value c in fp64 (-inf for a NaN).
+__device__ __forceinline__ double grouped_value_f64(const RouterArgs& r, int64_t t, int e) {
+  const double x = router_logit(r, t, e);
+  double v = x;
+  if (r.bias) v = (x == x ? 1.0 / (1.0 + exp(-x)) : 0.0) + (double)__ldg(&r.bias[e]);
+  return v == v ? v : -INFINITY;
 }
 
-// The selection of one token with a bias in fp64; lane j < topk returns the
-// j-th id.
+// The groups that may be selected from (bit g), in fp64.
 template <int PER>
-__device__ __noinline__ int grouped_select_f64(const RouterArgs r, int64_t t, int lane) {
-  const int per = (r.E + 31) >> 5, gs = r.E / r.groups;
+__device__ __noinline__ uint32_t grouped_taken_f64(const RouterArgs r, int64_t t, int lane) {
+  double c[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane * r.per + i;
+    c[i] = i < r.per && e < r.E ? grouped_value_f64(r, t, e) : -INFINITY;
+  }
+  double size;
+  const double score = group_scores<double, PER>(r, c, r.bias != nullptr, lane, size);
+  int rank = 0;
+  for (int h = 0; h < r.groups; ++h) {
+    const double other = __shfl_sync(0xffffffffu, score, h);
+    rank += (other > score || (other == score && h < lane)) ? 1 : 0;
+  }
+  return __ballot_sync(0xffffffffu, lane < r.groups && rank < r.topk_groups);
+}
+
+// The selection from the groups `taken` in fp64, for a token with more experts
+// near its border than lanes; lane j < topk returns the j-th id.
+template <int PER>
+__device__ __noinline__ int grouped_select_f64(const RouterArgs r, int64_t t, uint32_t taken, int lane) {
   double c[PER];
   uint32_t open = 0;  // bit i: expert lane * per + i may still be selected
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int e = lane * per + i;
+    const int e = lane * r.per + i;
     c[i] = -INFINITY;
-    if (i < per && e < r.E) {
-      const double x = router_logit(r, t, e);
-      const double s = x == x ? 1.0 / (1.0 + exp(-x)) : 0.0;
-      const double v = s + (double)__ldg(&r.bias[e]);
-      if (v == v) c[i] = v;
+    if (i < r.per && e < r.E && ((taken >> (e / r.gs)) & 1u)) {
+      c[i] = grouped_value_f64(r, t, e);
       open |= 1u << i;
     }
   }
-  const double score = group_scores<double, PER>(c, r.E, r.groups, per, true, lane);
-  const int rank = group_rank(score, r.groups, lane);
-  const uint32_t taken = __ballot_sync(0xffffffffu, lane < r.groups && rank < r.topk_groups);
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if (((open >> i) & 1u) && !((taken >> ((lane * per + i) / gs)) & 1u)) open &= ~(1u << i);
   int id = 0;
   for (int k = 0; k < r.topk; ++k) {
     double bv = -INFINITY;
@@ -261,7 +295,7 @@ __device__ __noinline__ int grouped_select_f64(const RouterArgs r, int64_t t, in
     for (int i = 0; i < PER; ++i)
       if (((open >> i) & 1u) && (bi == 0x7fffffff || c[i] > bv)) {
         bv = c[i];
-        bi = lane * per + i;
+        bi = lane * r.per + i;
       }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
@@ -273,27 +307,107 @@ __device__ __noinline__ int grouped_select_f64(const RouterArgs r, int64_t t, in
         bi = oi;
       }
     }
-    if (bi / per == lane) open &= ~(1u << (bi - lane * per));
+    if (bi / r.per == lane) open &= ~(1u << (bi - lane * r.per));
     if (lane == k) id = bi;
   }
   return id;
 }
 
-// As route_token_warp, with groups.
-template <int PER>
-__device__ __forceinline__ void route_token_grouped(const RouterArgs& r, int64_t t, int lane, int& id_out,
-                                                    float& w_out) {
-  const int E = r.E, topk = r.topk, groups = r.groups;
-  const int per = (E + 31) >> 5, gs = E / groups;
-  const bool biased = r.bias != nullptr;
-  const int e0 = lane * per;
-  float x[PER];  // logits, then the values that are compared
+// n candidates in descending order of approximate values, lane j < n holding the
+// j-th one's id, among them every expert that can be one of the topk best: the
+// place of this lane's candidate among them in exact order (fp64; lower id first).
+static __device__ __noinline__ int grouped_order_f64(const RouterArgs r, int64_t t, int id, int n, int lane) {
+  const double c = lane < n ? grouped_value_f64(r, t, id) : -INFINITY;
+  int rank = 0;
+  for (int j = 0; j < n; ++j) {
+    const double other = __shfl_sync(0xffffffffu, c, j);
+    const int oid = __shfl_sync(0xffffffffu, id, j);
+    rank += (other > c || (other == c && oid < id)) ? 1 : 0;
+  }
+  return rank;
+}
+
+// Descending order of N keys (N = 8: a 19-exchange network; else halves, merged).
+__device__ __forceinline__ void key_exchange(uint32_t& a, uint32_t& b) {
+  const uint32_t hi = a > b ? a : b, lo = a > b ? b : a;
+  a = hi;
+  b = lo;
+}
+template <int N>
+__device__ __forceinline__ void merge_keys(uint32_t* k) {  // a bitonic sequence
+  if constexpr (N > 1) {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) x[i] = i < per && e0 + i < E ? router_logit(r, t, e0 + i) : -INFINITY;
-  float xmax = -INFINITY, denom = 0.f;
+    for (int i = 0; i < N / 2; ++i) key_exchange(k[i], k[i + N / 2]);
+    merge_keys<N / 2>(k);
+    merge_keys<N / 2>(k + N / 2);
+  }
+}
+template <int N>
+__device__ __forceinline__ void sort_keys(uint32_t* k) {
+  if constexpr (N == 8) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) key_exchange(k[i], k[i + 1]);
+    key_exchange(k[0], k[2]), key_exchange(k[1], k[3]), key_exchange(k[4], k[6]), key_exchange(k[5], k[7]);
+    key_exchange(k[1], k[2]), key_exchange(k[5], k[6]), key_exchange(k[0], k[4]), key_exchange(k[3], k[7]);
+    key_exchange(k[1], k[5]), key_exchange(k[2], k[6]);
+    key_exchange(k[1], k[4]), key_exchange(k[3], k[6]);
+    key_exchange(k[2], k[4]), key_exchange(k[3], k[5]);
+    key_exchange(k[3], k[4]);
+  } else {
+    sort_keys<N / 2>(k);
+    sort_keys<N / 2>(k + N / 2);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) key_exchange(k[i], k[N - 1 - i]);
+    merge_keys<N / 2>(k);
+    merge_keys<N / 2>(k + N / 2);
+  }
+}
+
+// Routes token t with groups (all 32 lanes call it): ids and weights go to
+// r.out_ids / r.out_w.
+template <int PER, bool BIASED>
+__device__ __forceinline__ void route_token_grouped(const RouterArgs& r, int64_t t, int lane) {
+  constexpr uint32_t kPlace = PER - 1;  // low bits of a key: kPlace - place in the lane
+  // How far apart two neighbours must be to be sure of their order: without a
+  // bias only equal values say nothing (dropping low bits keeps the order); with
+  // one, the errors of both, and the dropped bits.
+  constexpr float kEps = BIASED ? kValueEps : 0.f;
+  constexpr float kEpsRel = BIASED ? kValueEpsRel + PER * 1.2e-7f : 0.f;
+  const int E = r.E, topk = r.topk, groups = r.groups;
+  const int per = r.per, gs = r.gs;
+  const int e0 = lane * per;
+  const bool whole = per == PER && E == 32 * PER && r.vec;  // every lane full, rows aligned for vector loads
+  float x[PER];  // logits, then the values that are compared
+  if (whole && !r.bf16) {
+    const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(r.logits) + t * E + e0);
+#pragma unroll
+    for (int i = 0; i < PER / 4; ++i) {
+      const float4 v = __ldg(src + i);
+      x[4 * i] = v.x;
+      x[4 * i + 1] = v.y;
+      x[4 * i + 2] = v.z;
+      x[4 * i + 3] = v.w;
+    }
+  } else if (whole) {
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(r.logits) + t * E + e0);
+#pragma unroll
+    for (int i = 0; i < PER / 8; ++i) {
+      const uint4 v = __ldg(src + i);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+        x[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = i < per && e0 + i < E ? router_logit(r, t, e0 + i) : -INFINITY;
+  }
 #pragma unroll
   for (int i = 0; i < PER; ++i) x[i] = x[i] == x[i] ? x[i] : -INFINITY;
-  if (r.scoring == 0) {
+  float xmax = -INFINITY, denom = 0.f;
+  if (!BIASED && r.scoring == 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) xmax = fmaxf(xmax, x[i]);
     xmax = order_value(__reduce_max_sync(0xffffffffu, order_key(xmax)));
@@ -305,106 +419,159 @@ __device__ __forceinline__ void route_token_grouped(const RouterArgs& r, int64_t
       for (int o = 16; o >= 1; o >>= 1) denom += __shfl_xor_sync(0xffffffffu, denom, o);
     }
   }
-  if (biased) {
+  if (BIASED) {
+    float b[PER];
+    if (whole && r.vec_bias) {
+#pragma unroll
+      for (int i = 0; i < PER; i += 4) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(r.bias + e0 + i));
+        b[i] = v.x;
+        b[i + 1] = v.y;
+        b[i + 2] = v.z;
+        b[i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) b[i] = i < per && e0 + i < E ? __ldg(&r.bias[e0 + i]) : 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (i < per && e0 + i < E) {
+      if (whole || (i < per && e0 + i < E)) {
         const float d = 1.0f + __expf(-x[i]);
-        const float c = (d < 1e30f ? __fdividef(1.0f, d) : 0.0f) + __ldg(&r.bias[e0 + i]);
+        const float c = (d < 1e30f ? __fdividef(1.0f, d) : 0.0f) + b[i];
         x[i] = c == c ? c : -INFINITY;
       }
   }
-  // The groups whose experts may be selected, and whether fp32 could tell.
-  const float score = group_scores<float, PER>(x, E, groups, per, biased, lane);
-  const int rank = group_rank(score, groups, lane);
-  const uint32_t taken = __ballot_sync(0xffffffffu, lane < groups && rank < r.topk_groups);
-  bool close = false;
-  if (biased && r.topk_groups < groups) {
-    // A score is the sum of two values of any size: its error goes by the largest.
-    float big = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) big = fabsf(x[i]) < INFINITY ? fmaxf(big, fabsf(x[i])) : big;
-    big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
-    const int in = __ffs(__ballot_sync(0xffffffffu, lane < groups && rank == r.topk_groups - 1)) - 1;
-    const int out = __ffs(__ballot_sync(0xffffffffu, lane < groups && rank == r.topk_groups)) - 1;
-    const float a = __shfl_sync(0xffffffffu, score, in), b = __shfl_sync(0xffffffffu, score, out);
-    close = !(a - b > 2.0f * (kGroupedEps + kGroupedEpsRel * big));
+  // The groups whose experts may be selected: best ones first; again in fp64 if
+  // the last of them is not clearly ahead of the first that is left out.
+  uint32_t taken = 0xffffffffu;
+  if (r.topk_groups < groups) {
+    taken = 0;
+    float size;
+    const float score = group_scores<float, PER>(r, x, BIASED, lane, size);
+    uint32_t sk = lane < groups ? order_key(score) : 0u;
+    uint32_t m = 0;
+    for (int k = 0; k < r.topk_groups; ++k) {
+      m = __reduce_max_sync(0xffffffffu, sk);
+      const uint32_t who = __ballot_sync(0xffffffffu, sk == m);
+      const uint32_t first = who & (0u - who);
+      taken |= first;
+      if ((first >> lane) & 1u) sk = 0;
+    }
+    if (BIASED) {
+      const float a = order_value(m), b = order_value(__reduce_max_sync(0xffffffffu, sk));
+      // a sum of two values of any size: its error goes by the largest
+      const float big = __uint_as_float(__reduce_max_sync(0xffffffffu, size < INFINITY ? __float_as_uint(size) : 0u));
+      if (!(a - b > 2.0f * (kValueEps + kValueEpsRel * big))) taken = grouped_taken_f64<PER>(r, t, lane);
+    }
   }
   // Keys of this lane's experts; 0 = cannot be selected (any more).
   uint32_t key[PER];
-  uint32_t best = 0;
-  int at = 0;
-  {
+  if (r.span_log2 >= 0) {
+    const bool in = (taken >> (lane >> r.span_log2)) & 1u;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      key[i] = in && (whole || (i < per && e0 + i < E)) ? ((order_key(x[i]) & ~kPlace) | (kPlace - i)) : 0u;
+  } else {
     int g = e0 / gs, left = (g + 1) * gs - e0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      key[i] = i < per && e0 + i < E && ((taken >> (g & 31)) & 1u) ? order_key(x[i]) : 0u;
-      if (key[i] > best) {
-        best = key[i];
-        at = i;
-      }
+      key[i] = i < per && e0 + i < E && ((taken >> (g & 31)) & 1u) ? ((order_key(x[i]) & ~kPlace) | (kPlace - i)) : 0u;
       if (--left == 0) {
         ++g;
         left = gs;
       }
     }
   }
-  int my_id = 0;
-  // With a bias one round more: is the last one taken clearly ahead of the next?
-  const int rounds = biased && topk < r.topk_groups * gs ? topk + 1 : topk;
-  float prev = 0.f;
-  for (int k = 0; k < rounds; ++k) {
-    const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-    const int src = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
-    const int id = __shfl_sync(0xffffffffu, e0 + at, src);
-    if (lane == k) my_id = id;
-    if (biased) {
-      const float v = order_value(m);
-      if (k > 0 && !(prev - v > kGroupedEps + kGroupedEpsRel * fabsf(prev))) close = true;
-      prev = v;
+  sort_keys<PER>(key);
+  // Rounds: lane n keeps the n-th best key (there are topk experts at least), and
+  // the lane it came from.
+  const uint32_t cut = ~kPlace;
+  uint32_t my_key = 0;
+  int my_src = 0, n = 0;
+  auto take = [&](uint32_t m) {
+    // the lowest lane with the largest value; its place is its key's own
+    const int src = __ffs(__ballot_sync(0xffffffffu, (key[0] & cut) == m)) - 1;
+    const uint32_t won = __shfl_sync(0xffffffffu, key[0], src);
+    if (lane == n) {
+      my_key = won;
+      my_src = src;
     }
-    if (lane == src) {
-      best = 0;
-      int next = 0;
+    ++n;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (i == at) key[i] = 0;
-        if (key[i] > best) {
-          best = key[i];
-          next = i;
-        }
+    for (int i = 0; i < PER; ++i) key[i] = lane == src ? (i + 1 < PER ? key[i + 1] : 0u) : key[i];
+  };
+  while (n < topk) take(__reduce_max_sync(0xffffffffu, key[0] & cut));
+  // Where values can be off, the ones not clearly behind the last of them join.
+  bool order = false;  // two candidates too close to tell which comes first
+  bool many = false;   // more of them than lanes
+  if (BIASED || !r.bf16) {
+    const float last = order_value(__shfl_sync(0xffffffffu, my_key, topk - 1) & cut);
+    while (true) {
+      const uint32_t m = __reduce_max_sync(0xffffffffu, key[0] & cut);
+      if (m == 0 || last - order_value(m) > kEps + kEpsRel * fabsf(last)) break;
+      if (n == 32) {
+        many = true;
+        break;
       }
-      at = next;
+      take(m);
     }
+    const float v = order_value(my_key & cut);
+    const float next = __shfl_down_sync(0xffffffffu, v, 1);
+    order = __any_sync(0xffffffffu, lane + 1 < n && !(v - next > kEps + kEpsRel * fabsf(v)));
   }
-  if (biased && close) my_id = grouped_select_f64<PER>(r, t, lane);  // warp-uniform
+  int my_id = my_src * per + (int)(kPlace - (my_key & kPlace));
+  int place = lane;  // of this lane's expert in the output (topk and more: none)
+  if (many) my_id = grouped_select_f64<PER>(r, t, taken, lane);  // warp-uniform
+  else if (order) place = grouped_order_f64(r, t, my_id, n, lane);
+  const bool mine = place < topk && (many || lane < n);
   float w = 0.f;
-  if (lane < topk) {
+  if (mine) {
     const float v = router_logit(r, t, my_id);
     if (r.scoring == 1) w = v == v ? 1.0f / (1.0f + expf(-v)) : 0.f;
     else if (v == v && v != -INFINITY) w = v == xmax ? 1.0f : expf(v - xmax);
   }
-  float sum = w;
+  if (r.renormalize) {
+    float sum = w;
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (r.renormalize) w = sum > 0.f ? w / sum : 0.f;
-  else if (r.scoring == 0) w = denom > 0.f ? w / denom : 0.f;
-  id_out = my_id;
-  w_out = 0.f;
-  if (lane < topk) {
-    w_out = w * r.scaling;
-    r.out_w[t * topk + lane] = w_out;
-    r.out_ids[t * topk + lane] = my_id;
+    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    w = sum > 0.f ? w / sum : 0.f;
+  } else if (r.scoring == 0) {
+    w = denom > 0.f ? w / denom : 0.f;
+  }
+  if (mine) {
+    r.out_w[t * topk + place] = w * r.scaling;
+    r.out_ids[t * topk + place] = my_id;
   }
 }
 
 template <int PER, bool GROUPED>
-__device__ __forceinline__ void route_token(const RouterArgs& r, int64_t t, int lane, int& id, float& w) {
-  if constexpr (GROUPED) route_token_grouped<PER>(r, t, lane, id, w);
-  else route_token_warp<PER>(r, t, lane, id, w);
+__device__ __forceinline__ void route_token(const RouterArgs& r, int64_t t, int lane) {
+  if constexpr (GROUPED) {
+    if (r.bias) route_token_grouped<PER, true>(r, t, lane);
+    else route_token_grouped<PER, false>(r, t, lane);
+  } else {
+    int id;
+    float w;
+    route_token_warp<PER>(r, t, lane, id, w);
+  }
 }
 
 // Values per lane for E experts (see route_token_warp).
 __host__ __device__ __forceinline__ int router_per_lane(int E) { return E <= 256 ? 8 : (E <= 512 ? 16 : 32); }
+
+// Consecutive experts a lane owns in group-limited routing: at least ceil(E / 32)
+// and at most router_per_lane(E), a group's size divided by a power of two if one
+// fits.
+inline int grouped_per_lane(int E, int groups) {
+  const int least = (E + 31) / 32;
+  int fit = 0;
+  for (int per = E / groups;; per /= 2) {
+    if (per < least) break;
+    if (per <= router_per_lane(E)) fit = per;
+    if (per % 2) break;
+  }
+  return fit ? fit : least;
+}
 
 }  // namespace b200moe
