@@ -48,7 +48,7 @@ def check(out, y, bound):
     assert (off <= bound).all(), float((off / bound).max())
 
 
-SHAPES = [(1, 128, 128), (1, 4096, 1024), (2, 1, 128), (7, 300, 256), (16, 256, 6144), (17, 129, 384), (33, 576, 896),
+SHAPES = [(1, 128, 128), (1, 4096, 1024), (2, 6144, 2048), (3, 256, 6144), (11, 4096, 512), (2, 1, 128), (7, 300, 256), (16, 256, 6144), (17, 129, 384), (33, 576, 896),
           (64, 2048, 2048), (65, 257, 512), (100, 8, 1152), (127, 1000, 256), (128, 512, 640), (129, 383, 2048),
           (255, 64, 128), (300, 1280, 768), (512, 640, 1024), (1000, 384, 512), (2100, 520, 384), (5000, 130, 256)]
 
@@ -72,7 +72,7 @@ def test_linear(cuda_device, M, N, K):
     assert read_device_error(layer_error_word(cuda_device)) == 0
 
 
-@pytest.mark.parametrize("M,H,I", [(1, 256, 128), (3, 640, 256), (16, 1024, 384), (63, 256, 1280), (64, 2048, 256),
+@pytest.mark.parametrize("M,H,I", [(1, 256, 128), (1, 6144, 512), (2, 6144, 2048), (5, 4096, 512), (3, 640, 256), (16, 1024, 384), (63, 256, 1280), (64, 2048, 256),
                                    (65, 384, 128), (128, 512, 512), (200, 1152, 640), (513, 256, 384),
                                    (1500, 384, 256)])
 def test_gate_up(cuda_device, M, H, I):

@@ -181,9 +181,8 @@ cudaError_t launch_epi_dense(const DensePlan& pl, const CUtensorMap& tm_x, const
                              const DenseParams& p, bool early_w, cudaStream_t stream) {
   switch (pl.cfg) {
     case 16:
-      if (pl.quantise_x) return launch_split_dense<EPI, 16, true>(pl, tm_x, tm_w, p, early_w, stream);
-      if constexpr (EPI == DENSE_OUT) return launch_split_dense<EPI, 16, false>(pl, tm_x, tm_w, p, early_w, stream);
-      return cudaErrorInvalidValue;
+      return pl.quantise_x ? launch_split_dense<EPI, 16, true>(pl, tm_x, tm_w, p, early_w, stream)
+                           : launch_split_dense<EPI, 16, false>(pl, tm_x, tm_w, p, early_w, stream);
     case 32:
       if constexpr (EPI == DENSE_OUT) return launch_split_dense<EPI, 32, false>(pl, tm_x, tm_w, p, early_w, stream);
       return cudaErrorInvalidValue;
@@ -219,11 +218,14 @@ DensePlan split_plan(int epi, int64_t M, int64_t N, int nkb, bool x_bf16) {
   int s = 8 / halves;
   while (s > 1 && (s * 2 > nkb || units > resident_split(s * halves))) --s;
   const int per = (nkb + s - 1) / s;
-  bool qx = x_bf16 && T == 16 && M * per <= kQuantGroups && split_stages<16>(per, tt, true) > 0;
+  // A token or two: a CTA can quantise its own K blocks of bf16 rows.
+  const bool few = T == 16 && M * per <= kQuantGroups && split_stages<16>(per, tt, true) > 0;
+  const bool qx = few && x_bf16;
   // Gate/up with rows of 256 columns to a CTA (token-major) is as fast from the
-  // first token on (9.8 against 10.0 us at 1, 11.8 against 12.4 at 64), so here it
-  // is only for saving the quantising launch.
-  if (epi == DENSE_SILU && !qx) return pl;
+  // first token on (9.8 against 10.0 us at 1, 11.8 against 12.4 at 64), so this
+  // kernel only serves it where it saves the quantising launch; fp8 rows go the
+  // same way, so that they give the same bits.
+  if (epi == DENSE_SILU && !few) return pl;
   const int stages = qx ? 1
                         : (T == 16 ? split_stages<16>(per, tt, false)
                                    : (T == 32 ? split_stages<32>(per, tt, false) : split_stages<64>(per, tt, false)));
