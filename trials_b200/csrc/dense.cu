@@ -146,10 +146,6 @@ int resident_clusters(K kernel, int R, int threads, int smem, std::atomic<int> (
   if (known) cache[dev][R].store(n);
   return n;
 }
-int resident_split(int R) {
-  static std::atomic<int> cache[kMaxDevices][9];
-  return resident_clusters(dense_split_kernel<DENSE_OUT, 64, false>, R, DenseSplitCfg<64>::THREADS, kSplitSmem, cache);
-}
 int resident_tok(int R) {
   static std::atomic<int> cache[kMaxDevices][9];
   return resident_clusters(dense_tok_kernel<DENSE_OUT>, R, DenseTokCfg::THREADS, DenseTokCfg::SMEM_BYTES, cache);
@@ -209,14 +205,19 @@ DensePlan split_plan(int epi, int64_t M, int64_t N, int nkb, bool x_bf16) {
   const int tt = (int)((M + n_tt - 1) / n_tt + 15) / 16 * 16;
   const int T = tt <= 16 ? 16 : (tt <= 32 ? 32 : 64);
   const int64_t units = (N + 128 * halves - 1) / (128 * halves) * n_tt;
+  const int sms = sm_count_of(current_device());
   // More than 64 tokens read the weights more than once, which only pays when
-  // the tiles are too few to fill the device otherwise: 100 x 576 x 7168 takes
-  // 7.7 us this way and 11.0 token-major, 100 x 4096 x 6144 15.3 and 12.8.
-  if (M > 64 && units > resident_split(8)) return pl;
-  // The most CTAs along K that still run in one wave, with at least two K blocks
-  // each: 6144 x 2048 takes 6.2 us with 4, 6.8 with 2 and, two waves, 10.8 with 6.
+  // the tiles are so few that 8 CTAs each still run in one wave (two CTAs an SM
+  // less what clusters of 8 cannot use): 100 x 576 x 7168 takes 7.7 us this way
+  // and 11.0 token-major, 100 x 4096 x 6144 15.3 and 12.8.
+  if (M > 64 && units * halves * 8 > (int64_t)sms * 7 / 4) return pl;
+  // CTAs along K, at least two K blocks each. Up to 4/3 of the SMs measured best:
+  // one token of 6144 x 2048 (48 tiles) takes 6.2 us with 4, 6.8 with 2 and, in
+  // two waves, 10.8 with 6; 4096 x 6144 (32 tiles) 8.9 with 4 and 9.0 with 8, 64
+  // tokens of it 11.4 and 11.9.
   int s = 8 / halves;
-  while (s > 1 && (s * 2 > nkb || units > resident_split(s * halves))) --s;
+  const int64_t most = M > 64 ? (int64_t)sms * 7 / 4 : (int64_t)sms * 4 / 3;
+  while (s > 1 && (s * 2 > nkb || units * halves * s > most)) s /= 2;
   const int per = (nkb + s - 1) / s;
   // A token or two: a CTA can quantise its own K blocks of bf16 rows.
   const bool few = T == 16 && M * per <= kQuantGroups && split_stages<16>(per, tt, true) > 0;
