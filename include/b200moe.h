@@ -588,24 +588,73 @@ B200MOE_API int b200moe_combine_reduce(const void* out_pair, const int32_t* slot
  * to add to. Weights contiguous; workspace b200moe_mlp_workspace_size() bytes,
  * 256-byte aligned.
  *
- * A pipeline wait that gives up sets B200MOE_DEVERR_TIMEOUT in err_word
- * (required) and leaves the outputs undefined.
+ * The calls take their twenty arguments in a struct whose members are all 8 bytes
+ * wide (set every one; a foreign-function interface fills it in one step). A
+ * pipeline wait that gives up sets B200MOE_DEVERR_TIMEOUT in err_word (required)
+ * and leaves the outputs undefined.
  * ---------------------------------------------------------------------- */
 /* x_bf16: the rows come in bf16; gate_up: for b200moe_gate_up, with N = 2I and K = H. */
 B200MOE_API size_t b200moe_linear_workspace_size(int64_t M, int64_t N, int64_t K, int x_bf16, int gate_up);
-B200MOE_API int b200moe_linear(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs,
-                               int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ld_w, const float* w_scale,
-                               const void* residual, int64_t ld_res, void* out, int64_t ld_out, int out_f32,
-                               void* workspace, size_t workspace_bytes, int32_t* err_word, void* stream);
-B200MOE_API int b200moe_gate_up(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs,
-                                int64_t M, int64_t H, int64_t I, const uint8_t* w13, int64_t ld_w,
-                                const float* w13_scale, uint8_t* q, int64_t ld_q, float* s, int64_t ld_s,
-                                void* workspace, size_t workspace_bytes, int32_t* err_word, void* stream);
+typedef struct b200moe_linear_args {
+  const void* x;
+  const uint8_t* x_q;
+  const float* x_scale;
+  int64_t ld_x, ld_xs;
+  int64_t M, N, K;
+  const uint8_t* w;
+  int64_t ld_w;
+  const float* w_scale;
+  const void* residual;
+  int64_t ld_res;
+  void* out;
+  int64_t ld_out;
+  int64_t out_f32;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int32_t* err_word;
+  void* stream;
+} b200moe_linear_args;
+B200MOE_API int b200moe_linear(const b200moe_linear_args* args);
+typedef struct b200moe_gate_up_args {
+  const void* x;
+  const uint8_t* x_q;
+  const float* x_scale;
+  int64_t ld_x, ld_xs;
+  int64_t M, H, I;
+  const uint8_t* w13;
+  int64_t ld_w;
+  const float* w13_scale;
+  uint8_t* q;
+  int64_t ld_q;
+  float* s;
+  int64_t ld_s;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int32_t* err_word;
+  void* stream;
+} b200moe_gate_up_args;
+B200MOE_API int b200moe_gate_up(const b200moe_gate_up_args* args);
 B200MOE_API size_t b200moe_mlp_workspace_size(int64_t M, int64_t H, int64_t I, int x_bf16);
-B200MOE_API int b200moe_mlp(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs,
-                            int64_t M, int64_t H, int64_t I, const uint8_t* w13, const float* w13_scale,
-                            const uint8_t* w2, const float* w2_scale, const void* residual, int64_t ld_res, void* out,
-                            int64_t ld_out, void* workspace, size_t workspace_bytes, int32_t* err_word, void* stream);
+typedef struct b200moe_mlp_args {
+  const void* x;
+  const uint8_t* x_q;
+  const float* x_scale;
+  int64_t ld_x, ld_xs;
+  int64_t M, H, I;
+  const uint8_t* w13;
+  const float* w13_scale;
+  const uint8_t* w2;
+  const float* w2_scale;
+  const void* residual;
+  int64_t ld_res;
+  void* out;
+  int64_t ld_out;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int32_t* err_word;
+  void* stream;
+} b200moe_mlp_args;
+B200MOE_API int b200moe_mlp(const b200moe_mlp_args* args);
 
 /* ------------------------------------------------------------------------
  * Diagnostics.

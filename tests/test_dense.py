@@ -1,5 +1,7 @@
 """Refusals of the dense FP8 products (fp8_block_linear, fp8_gate_up, fp8_mlp):
 checked on the host before anything is launched, so no GPU is needed."""
+import struct
+
 import pytest
 import torch
 
@@ -9,10 +11,15 @@ P = 256  # a non-null, aligned address that no refused call touches
 FP8 = torch.float8_e4m3fn
 
 
+def call(name, *args):
+    """A C entry whose arguments come packed (None = NULL)."""
+    return getattr(_lib.lib(), name)(struct.pack(f"{len(args)}q", *(0 if a is None else a for a in args)))
+
+
 def linear(x=P, xq=None, xs=None, ld_x=256, ld_xs=2, M=4, N=100, K=256, w=P, ld_w=256, ws=P, res=None, ld_res=0,
            out=P, ld_out=100, f32=0, work=P, nwork=1 << 20, err=P):
-    return _lib.lib().b200moe_linear(x, xq, xs, ld_x, ld_xs, M, N, K, w, ld_w, ws, res, ld_res, out, ld_out, f32, work,
-                                     nwork, err, None)
+    return call("b200moe_linear", x, xq, xs, ld_x, ld_xs, M, N, K, w, ld_w, ws, res, ld_res, out, ld_out, f32, work,
+                nwork, err, None)
 
 
 @pytest.mark.parametrize("kw", [
@@ -39,10 +46,12 @@ def test_linear_workspace(kw):
 def test_empty_batches_launch_nothing():
     L = _lib.lib()
     assert linear(M=0, x=None, out=None, work=None, nwork=0) == _lib.OK
-    assert L.b200moe_gate_up(None, None, None, 0, 0, 0, 256, 128, P, 256, P, None, 0, None, 0, None, 0, P,
-                             None) == _lib.OK
-    assert L.b200moe_mlp(None, None, None, 0, 0, 0, 256, 128, P, P, P, P, None, 0, None, 0, None, 0, P,
-                         None) == _lib.OK
+    assert call("b200moe_gate_up", None, None, None, 0, 0, 0, 256, 128, P, 256, P, None, 0, None, 0, None, 0, P,
+                None) == _lib.OK
+    assert call("b200moe_mlp", None, None, None, 0, 0, 0, 256, 128, P, P, P, P, None, 0, None, 0, None, 0, P,
+                None) == _lib.OK
+    for name in ("b200moe_linear", "b200moe_gate_up", "b200moe_mlp"):
+        assert getattr(L, name)(None) == _lib.ERR_INVALID_ARG
     assert L.b200moe_linear_workspace_size(0, 256, 256, 1, 0) == 0
     assert L.b200moe_mlp_workspace_size(0, 256, 128, 1) == 0
 
@@ -51,7 +60,8 @@ def test_gate_up_and_mlp_host_checks():
     L = _lib.lib()
 
     def gate_up(I=128, q=P, ld_q=128, s=P, ld_s=1, H=256):
-        return L.b200moe_gate_up(P, None, None, 256, 0, 4, H, I, P, 256, P, q, ld_q, s, ld_s, P, 1 << 20, P, None)
+        return call("b200moe_gate_up", P, None, None, 256, 0, 4, H, I, P, 256, P, q, ld_q, s, ld_s, P, 1 << 20, P,
+                    None)
 
     assert gate_up(I=0) == _lib.ERR_INVALID_ARG
     assert gate_up(q=None) == _lib.ERR_INVALID_ARG
@@ -61,7 +71,7 @@ def test_gate_up_and_mlp_host_checks():
     assert gate_up(H=384) == _lib.ERR_INVALID_ARG  # row stride 256 is shorter than a row
 
     def mlp(I=128, w2=P, out=P, nwork=1 << 20, res=None):
-        return L.b200moe_mlp(P, None, None, 256, 0, 4, 256, I, P, P, w2, P, res, 0, out, 256, P, nwork, P, None)
+        return call("b200moe_mlp", P, None, None, 256, 0, 4, 256, I, P, P, w2, P, res, 0, out, 256, P, nwork, P, None)
 
     assert mlp(I=0) == _lib.ERR_INVALID_ARG
     assert mlp(I=192) == _lib.ERR_UNSUPPORTED

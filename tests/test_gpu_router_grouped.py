@@ -119,6 +119,29 @@ def test_bad_biases(cuda_device):
     check(x, 8, 3, 6, "sigmoid", b.to(cuda_device))
 
 
+def test_refusals_on_device(cuda_device):
+    x = torch.randn(4, 64, device=cuda_device)
+    for kw in (dict(num_expert_group=8), dict(num_expert_group=7, topk_group=2), dict(num_expert_group=8, topk_group=9)):
+        with pytest.raises(ValueError):
+            moe.select_experts(x, 4, "sigmoid", **kw)
+    with pytest.raises(ValueError):  # a bias that does not cover the experts
+        moe.select_experts(x, 4, "sigmoid", torch.zeros(32, device=cuda_device), num_expert_group=8, topk_group=2)
+    with pytest.raises(NotImplementedError):
+        moe.select_experts(x.half(), 4, "sigmoid", num_expert_group=8, topk_group=2)
+
+
+def test_bias_of_another_type_or_layout(cuda_device):
+    x = torch.randn(50, 64, generator=torch.Generator().manual_seed(8)).to(cuda_device)
+    b = torch.randn(128, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16)[::2]
+    check(x, 8, 3, 6, "sigmoid", b)  # bf16, strided, on the host
+    buf = torch.zeros(65, device=cuda_device)
+    buf[1:] = b.to(cuda_device)
+    check(x, 8, 3, 6, "sigmoid", buf[1:])  # 4-byte aligned
+    wide = torch.zeros(50 * 64 + 1, device=cuda_device)[1:].view(50, 64)
+    wide.copy_(x)
+    check(wide, 8, 3, 6, "sigmoid", buf[1:])
+
+
 def test_one_group_is_ungrouped_routing(cuda_device):
     x = torch.randn(500, 256, generator=torch.Generator().manual_seed(2)).to(cuda_device)
     w, ids = moe.select_experts(x, 8, "softmax")

@@ -92,10 +92,10 @@ SIGNATURES = {
                                    _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P]),
     "b200moe_combine_reduce": (_I, [_P, _P, _I, _L, _I, _L, _P, _P]),
     "b200moe_linear_workspace_size": (_S, [_L, _L, _L, _I, _I]),
-    "b200moe_linear": (_I, [_P, _P, _P, _L, _L, _L, _L, _L, _P, _L, _P, _P, _L, _P, _L, _I, _P, _S, _P, _P]),
-    "b200moe_gate_up": (_I, [_P, _P, _P, _L, _L, _L, _L, _L, _P, _L, _P, _P, _L, _P, _L, _P, _S, _P, _P]),
+    "b200moe_linear": (_I, [ctypes.c_char_p]),  # a packed argument struct, as the next ones
+    "b200moe_gate_up": (_I, [ctypes.c_char_p]),
     "b200moe_mlp_workspace_size": (_S, [_L, _L, _L, _I]),
-    "b200moe_mlp": (_I, [_P, _P, _P, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _L, _P, _L, _P, _S, _P, _P]),
+    "b200moe_mlp": (_I, [ctypes.c_char_p]),
     "b200moe_read_error": (_I, [_P, _P, _I, _P]),
     "b200moe_selftest_wait_timeout": (_I, [_P, _I, _P]),
 }

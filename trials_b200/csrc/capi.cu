@@ -1585,50 +1585,48 @@ size_t b200moe_linear_workspace_size(int64_t M, int64_t N, int64_t K, int x_bf16
   return dense_bytes(dense_plan(gate_up ? DENSE_SILU : DENSE_OUT, M, N, K, x_bf16 != 0), M, K, x_bf16 != 0);
 }
 
-int b200moe_linear(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs, int64_t M,
-                   int64_t N, int64_t K, const uint8_t* w, int64_t ld_w, const float* w_scale, const void* residual,
-                   int64_t ld_res, void* out, int64_t ld_out, int out_f32, void* workspace, size_t workspace_bytes,
-                   int32_t* err_word, void* stream) {
+int b200moe_linear(const b200moe_linear_args* a) {
   const char* name = "b200moe_linear";
-  const DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
-  int st = check_dense(name, in, M, N, K, w, ld_w, w_scale, err_word);
+  if (!a) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
+  const DenseInput in{a->x, a->x_q, a->x_scale, a->ld_x, a->ld_xs};
+  const int64_t M = a->M, N = a->N, K = a->K;
+  int st = check_dense(name, in, M, N, K, a->w, a->ld_w, a->w_scale, a->err_word);
   if (st) return st;
   DenseParams p{};
-  st = check_dense_out(name, M, N, residual, ld_res, out, ld_out, out_f32, p);
+  st = check_dense_out(name, M, N, a->residual, a->ld_res, a->out, a->ld_out, a->out_f32 != 0, p);
   if (st) return st;
   if (M == 0) return B200MOE_OK;
-  const DensePlan pl = dense_plan(DENSE_OUT, M, N, K, x != nullptr);
-  st = check_dense_work(name, workspace, workspace_bytes, dense_bytes(pl, M, K, x != nullptr));
+  const DensePlan pl = dense_plan(DENSE_OUT, M, N, K, in.x != nullptr);
+  st = check_dense_work(name, a->workspace, a->workspace_bytes, dense_bytes(pl, M, K, in.x != nullptr));
   if (st) return st;
-  return run_dense(name, DENSE_OUT, pl, in, M, N, K, w, ld_w, w_scale, p, false, static_cast<uint8_t*>(workspace),
-                   err_word, stream);
+  return run_dense(name, DENSE_OUT, pl, in, M, N, K, a->w, a->ld_w, a->w_scale, p, false,
+                   static_cast<uint8_t*>(a->workspace), a->err_word, a->stream);
 }
 
-int b200moe_gate_up(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs, int64_t M,
-                    int64_t H, int64_t I, const uint8_t* w13, int64_t ld_w, const float* w13_scale, uint8_t* q,
-                    int64_t ld_q, float* s, int64_t ld_s, void* workspace, size_t workspace_bytes, int32_t* err_word,
-                    void* stream) {
+int b200moe_gate_up(const b200moe_gate_up_args* a) {
   const char* name = "b200moe_gate_up";
-  const DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
+  if (!a) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
+  const DenseInput in{a->x, a->x_q, a->x_scale, a->ld_x, a->ld_xs};
+  const int64_t M = a->M, H = a->H, I = a->I;
   if (I <= 0 || I > (1 << 23)) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
-  int st = check_dense(name, in, M, 2 * I, H, w13, ld_w, w13_scale, err_word);
+  int st = check_dense(name, in, M, 2 * I, H, a->w13, a->ld_w, a->w13_scale, a->err_word);
   if (st) return st;
-  if (M > 0 && (!q || !s || ld_q < I || ld_s < I / 128))
+  if (M > 0 && (!a->q || !a->s || a->ld_q < I || a->ld_s < I / 128))
     return fail(B200MOE_ERR_INVALID_ARG, "%s: bad output", name);
   if (I % 128 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "%s: I must be a multiple of 128", name);
-  if (!aligned16(q) || ld_q % 16 != 0)
+  if (!aligned16(a->q) || a->ld_q % 16 != 0)
     return fail(B200MOE_ERR_UNSUPPORTED, "%s: output rows must be 16-byte aligned", name);
   if (M == 0) return B200MOE_OK;
-  const DensePlan pl = dense_plan(DENSE_SILU, M, 2 * I, H, x != nullptr);
-  st = check_dense_work(name, workspace, workspace_bytes, dense_bytes(pl, M, H, x != nullptr));
+  const DensePlan pl = dense_plan(DENSE_SILU, M, 2 * I, H, in.x != nullptr);
+  st = check_dense_work(name, a->workspace, a->workspace_bytes, dense_bytes(pl, M, H, in.x != nullptr));
   if (st) return st;
   DenseParams p{};
-  p.q = q;
-  p.ld_q = ld_q;
-  p.s = s;
-  p.ld_s = ld_s;
-  return run_dense(name, DENSE_SILU, pl, in, M, 2 * I, H, w13, ld_w, w13_scale, p, false,
-                   static_cast<uint8_t*>(workspace), err_word, stream);
+  p.q = a->q;
+  p.ld_q = a->ld_q;
+  p.s = a->s;
+  p.ld_s = a->ld_s;
+  return run_dense(name, DENSE_SILU, pl, in, M, 2 * I, H, a->w13, a->ld_w, a->w13_scale, p, false,
+                   static_cast<uint8_t*>(a->workspace), a->err_word, a->stream);
 }
 
 }  // extern "C"
@@ -1659,26 +1657,25 @@ size_t b200moe_mlp_workspace_size(int64_t M, int64_t H, int64_t I, int x_bf16) {
   return plan_mlp(M, H, I, x_bf16 != 0).total;
 }
 
-int b200moe_mlp(const void* x, const uint8_t* x_q, const float* x_scale, int64_t ld_x, int64_t ld_xs, int64_t M,
-                int64_t H, int64_t I, const uint8_t* w13, const float* w13_scale, const uint8_t* w2,
-                const float* w2_scale, const void* residual, int64_t ld_res, void* out, int64_t ld_out,
-                void* workspace, size_t workspace_bytes, int32_t* err_word, void* stream) {
+int b200moe_mlp(const b200moe_mlp_args* a) {
   const char* name = "b200moe_mlp";
-  const DenseInput in{x, x_q, x_scale, ld_x, ld_xs};
+  if (!a) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
+  const DenseInput in{a->x, a->x_q, a->x_scale, a->ld_x, a->ld_xs};
+  const int64_t M = a->M, H = a->H, I = a->I;
   if (I <= 0 || I > (1 << 20)) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
-  int st = check_dense(name, in, M, 2 * I, H, w13, H, w13_scale, err_word);
+  int st = check_dense(name, in, M, 2 * I, H, a->w13, H, a->w13_scale, a->err_word);
   if (st) return st;
   if (I % 128 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "%s: I must be a multiple of 128", name);
-  if (!w2 || !w2_scale) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
-  if (!aligned16(w2)) return fail(B200MOE_ERR_UNSUPPORTED, "%s: weight rows must be 16-byte aligned", name);
+  if (!a->w2 || !a->w2_scale) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
+  if (!aligned16(a->w2)) return fail(B200MOE_ERR_UNSUPPORTED, "%s: weight rows must be 16-byte aligned", name);
   DenseParams p{};
-  st = check_dense_out(name, M, H, residual, ld_res, out, ld_out, 0, p);
+  st = check_dense_out(name, M, H, a->residual, a->ld_res, a->out, a->ld_out, 0, p);
   if (st) return st;
   if (M == 0) return B200MOE_OK;
-  const MlpPlan m = plan_mlp(M, H, I, x != nullptr);
-  st = check_dense_work(name, workspace, workspace_bytes, m.total);
+  const MlpPlan m = plan_mlp(M, H, I, in.x != nullptr);
+  st = check_dense_work(name, a->workspace, a->workspace_bytes, m.total);
   if (st) return st;
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   uint8_t* iq = ws + m.off_inter;
   float* is = reinterpret_cast<float*>(iq + round_up(M * I, 256));
   DenseParams g{};
@@ -1686,10 +1683,12 @@ int b200moe_mlp(const void* x, const uint8_t* x_q, const float* x_scale, int64_t
   g.ld_q = I;
   g.s = is;
   g.ld_s = I / 128;
-  st = run_dense(name, DENSE_SILU, m.up, in, M, 2 * I, H, w13, H, w13_scale, g, false, ws, err_word, stream);
+  st = run_dense(name, DENSE_SILU, m.up, in, M, 2 * I, H, a->w13, H, a->w13_scale, g, false, ws, a->err_word,
+                 a->stream);
   if (st) return st;
   const DenseInput mid{nullptr, iq, is, I, I / 128};
-  return run_dense(name, DENSE_OUT, m.down, mid, M, H, I, w2, I, w2_scale, p, true, nullptr, err_word, stream);
+  return run_dense(name, DENSE_OUT, m.down, mid, M, H, I, a->w2, I, a->w2_scale, p, true, nullptr, a->err_word,
+                   a->stream);
 }
 
 int b200moe_read_error(int32_t* err_word, int32_t* value, int clear, void* stream) {

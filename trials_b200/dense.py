@@ -14,6 +14,7 @@ the current torch stream of its tensors' device; there is no fallback path.
 """
 from __future__ import annotations
 
+import struct
 from typing import Optional
 
 import torch
@@ -22,7 +23,9 @@ from . import _lib
 from .moe import FP8, _require_cuda, _stream, _workspaces
 
 # These calls take a few microseconds on the GPU for a few tokens, so the checks
-# below read each attribute once and build no intermediate objects.
+# below read each attribute once and build no intermediate objects, and the C
+# entries get their arguments packed as one struct of 8-byte members (0 = NULL).
+_PACK = {n: struct.Struct(f"{n}q").pack for n in (19, 20)}
 
 
 def _device_of(x: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
@@ -36,15 +39,16 @@ def _device_of(x: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
     return index
 
 
-def _call(fn, where: str, index: int, args: tuple) -> None:
+def _call(fn, where: str, index: int, *args: int) -> None:
     """Calls a C entry on the current stream of device `index` (kernels launch on
-    the current device); args end before the error word and the stream. The error
-    word is the cached one of (device, stream) (moe.layer_error_word)."""
+    the current device); args are its arguments up to the error word and the
+    stream. The error word is the cached one of (device, stream)
+    (moe.layer_error_word)."""
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
-            return _call(fn, where, index, args)
+            return _call(fn, where, index, *args)
     stream = torch._C._cuda_getCurrentRawStream(index)
-    status = fn(*args, _workspaces.error_ptr(index, stream), stream)
+    status = fn(_PACK[len(args) + 2](*args, _workspaces.error_ptr(index, stream), stream))
     if status:
         _lib.check(status, where)
 
@@ -135,7 +139,7 @@ def _workspace(nbytes: int, dev: torch.device):
     torch's allocator on the current stream, so calls on other streams and captured
     graphs have theirs."""
     if nbytes == 0:
-        return None, None, 0
+        return None, 0, 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     return ws, ws.data_ptr(), nbytes
 
@@ -162,14 +166,14 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     L = _lib.lib()
     if x_scale is None:
         ws, ws_ptr, ws_bytes = _workspace(L.b200moe_linear_workspace_size(M, N, K, 1, 0), dev)
-        rows = (x.data_ptr(), None, None)
+        rows = (x.data_ptr(), 0, 0)
     else:
-        ws_ptr, ws_bytes = None, 0
-        rows = (None, x.data_ptr(), x_scale.data_ptr())
+        ws_ptr, ws_bytes = 0, 0
+        rows = (0, x.data_ptr(), x_scale.data_ptr())
     _call(L.b200moe_linear, "fp8_block_linear", index,
-          (*rows, ld_x, ld_s, M, N, K, weight.data_ptr(), ld_w, weight_scale.data_ptr(),
-           None if residual is None else residual.data_ptr(), ld_res, out.data_ptr(), ld_out,
-           out_dtype is torch.float32, ws_ptr, ws_bytes))
+          *rows, ld_x, ld_s, M, N, K, weight.data_ptr(), ld_w, weight_scale.data_ptr(),
+          0 if residual is None else residual.data_ptr(), ld_res, out.data_ptr(), ld_out,
+          out_dtype is torch.float32, ws_ptr, ws_bytes)
     return out
 
 
@@ -193,13 +197,13 @@ def fp8_gate_up(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, x_s
     L = _lib.lib()
     if x_scale is None:
         ws, ws_ptr, ws_bytes = _workspace(L.b200moe_linear_workspace_size(M, 2 * I, H, 1, 1), dev)
-        rows = (x.data_ptr(), None, None)
+        rows = (x.data_ptr(), 0, 0)
     else:
-        ws_ptr, ws_bytes = None, 0
-        rows = (None, x.data_ptr(), x_scale.data_ptr())
+        ws_ptr, ws_bytes = 0, 0
+        rows = (0, x.data_ptr(), x_scale.data_ptr())
     _call(L.b200moe_gate_up, "fp8_gate_up", index,
-          (*rows, ld_x, ld_s, M, H, I, w13.data_ptr(), ld_w, w13_scale.data_ptr(), q.data_ptr(), I, s.data_ptr(),
-           I // 128, ws_ptr, ws_bytes))
+          *rows, ld_x, ld_s, M, H, I, w13.data_ptr(), ld_w, w13_scale.data_ptr(), q.data_ptr(), I, s.data_ptr(),
+          I // 128, ws_ptr, ws_bytes)
     return q, s
 
 
@@ -227,8 +231,8 @@ def fp8_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
         return out
     L = _lib.lib()
     ws, ws_ptr, ws_bytes = _workspace(L.b200moe_mlp_workspace_size(M, H, I, x_scale is None), dev)
-    rows = (x.data_ptr(), None, None) if x_scale is None else (None, x.data_ptr(), x_scale.data_ptr())
+    rows = (x.data_ptr(), 0, 0) if x_scale is None else (0, x.data_ptr(), x_scale.data_ptr())
     _call(L.b200moe_mlp, "fp8_mlp", index,
-          (*rows, ld_x, ld_s, M, H, I, w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(),
-           None if residual is None else residual.data_ptr(), ld_res, out.data_ptr(), ld_out, ws_ptr, ws_bytes))
+          *rows, ld_x, ld_s, M, H, I, w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(),
+          0 if residual is None else residual.data_ptr(), ld_res, out.data_ptr(), ld_out, ws_ptr, ws_bytes)
     return out

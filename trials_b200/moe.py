@@ -135,6 +135,17 @@ def _check_groups(num_expert_group: Optional[int], topk_group: Optional[int]) ->
     return num_expert_group is not None
 
 
+def _router_bias(bias: Optional[torch.Tensor], dev: torch.device, index: int, E: int) -> Optional[torch.Tensor]:
+    """The correction bias as the kernels read it: E contiguous f32 on the device."""
+    if bias is None:
+        return None
+    if bias.numel() != E:
+        raise ValueError(f"correction_bias must have {E} entries, got {tuple(bias.shape)}")
+    if bias.dtype is torch.float32 and bias.get_device() == index and bias.is_contiguous():
+        return bias
+    return bias.to(device=dev, dtype=torch.float32).contiguous()
+
+
 def select_experts(router_logits: torch.Tensor, top_k: int, scoring_func: str = "softmax",
                    correction_bias: Optional[torch.Tensor] = None, renormalize: bool = True,
                    routed_scaling_factor: float = 1.0, num_expert_group: Optional[int] = None,
@@ -146,22 +157,33 @@ def select_experts(router_logits: torch.Tensor, top_k: int, scoring_func: str = 
     topk_group best of num_expert_group equal groups can be selected (a group's
     score is its largest value, with correction_bias the sum of its two largest).
     See b200moe_router_topk_grouped."""
-    dev = _require_cuda(router_logits)
-    bf16 = router_logits.dtype == torch.bfloat16
-    if not bf16 and router_logits.dtype != torch.float32:
+    dev = router_logits.device
+    index = router_logits.get_device()
+    if index < 0:
+        _require_cuda(router_logits)
+    bf16 = router_logits.dtype is torch.bfloat16
+    if not bf16 and router_logits.dtype is not torch.float32:
         raise NotImplementedError("router logits must be float32 or bfloat16")
     scoring = _SCORING.get(scoring_func)
     if scoring is None:
         raise NotImplementedError(f"scoring_func {scoring_func!r}")
+    grouped = _check_groups(num_expert_group, topk_group)
     logits = router_logits.contiguous()
     M, E = logits.shape
+    bias = _router_bias(correction_bias, dev, index, E)
     w = torch.empty(M, top_k, dtype=torch.float32, device=dev)
     ids = torch.empty(M, top_k, dtype=torch.int32, device=dev)
-    bias = None if correction_bias is None else correction_bias.to(device=dev, dtype=torch.float32).contiguous()
-    if _check_groups(num_expert_group, topk_group):
-        _lib.check(_lib.lib().b200moe_router_topk_grouped(
+    if grouped:
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
+                return select_experts(logits, top_k, scoring_func, bias, renormalize, routed_scaling_factor,
+                                      num_expert_group, topk_group)
+        status = _lib.lib().b200moe_router_topk_grouped(
             logits.data_ptr(), bf16, M, E, num_expert_group, topk_group, top_k, scoring, _ptr(bias),
-            bool(renormalize), routed_scaling_factor, w.data_ptr(), ids.data_ptr(), _stream(dev)), "select_experts")
+            bool(renormalize), routed_scaling_factor, w.data_ptr(), ids.data_ptr(),
+            torch._C._cuda_getCurrentRawStream(index))
+        if status:
+            _lib.check(status, "select_experts")
         return w, ids
     _lib.check(_lib.lib().b200moe_router_topk(_ptr(logits), int(logits.dtype == torch.bfloat16), M, E, top_k,
                                               scoring, _ptr(bias), int(renormalize), float(routed_scaling_factor),
@@ -393,7 +415,7 @@ def moe_layer_from_logits(hidden_states: torch.Tensor, router_logits: torch.Tens
         expert_map = expert_map.to(device=dev, dtype=torch.int32).contiguous()
     elif E_w != E_router:
         raise ValueError("without expert_map the weights must hold every routed expert")
-    bias = None if correction_bias is None else correction_bias.to(device=dev, dtype=torch.float32).contiguous()
+    bias = _router_bias(correction_bias, dev, router_logits.get_device(), E_router)
     logits = router_logits.contiguous()
     hidden = hidden_states.contiguous()
     w13_scale, w2_scale = w13_scale.contiguous(), w2_scale.contiguous()  # held through the call
