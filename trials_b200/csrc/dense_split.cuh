@@ -319,11 +319,10 @@ __global__ void __launch_bounds__(DenseSplitCfg<T>::THREADS, 2)
   cluster_sync_all();
   if (warp >= 2) {
     const uint32_t part = smem_u32(tiles);
-    for (int t = rank + R * (warp - 2); t < live; t += R * C::EW) {
-      finish_token<EPI, HALVES>(p, t0 + t, unit * HALVES * 128, splits, lane, [&](int s, int h) {
-        return mapa_shared(part + (uint32_t)((t * 128 + lane * 4) * 4), s * HALVES + h);
-      });
-    }
+    finish_tokens<EPI, HALVES>(p, t0, unit * HALVES * 128, splits, lane, rank + R * (warp - 2), R * C::EW, live,
+                               [&](int t, int s, int h) {
+                                 return mapa_shared(part + (uint32_t)((t * 128 + lane * 4) * 4), s * HALVES + h);
+                               });
   }
   __syncwarp();
   tc_fence_before();

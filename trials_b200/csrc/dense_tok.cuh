@@ -227,10 +227,9 @@ __global__ void __launch_bounds__(DenseTokCfg::THREADS, 1)
     cluster_sync_all();
     const uint32_t sums = smem_u32(tiles);
     const int rows = p.M - m0 < C::TM ? p.M - m0 : C::TM;
-    for (int t = rank + splits * ew; t < rows; t += splits * C::EW)
-      finish_token<EPI, 2>(p, m0 + t, w0, splits, lane, [&](int s, int hh) {
-        return mapa_shared(sums + (uint32_t)(t * 1024 + (((hh * 32 + lane) ^ (t & 7)) << 4)), s);
-      });
+    finish_tokens<EPI, 2>(p, m0, w0, splits, lane, rank + splits * ew, splits * C::EW, rows, [&](int t, int s, int hh) {
+      return mapa_shared(sums + (uint32_t)(t * 1024 + (((hh * 32 + lane) ^ (t & 7)) << 4)), s);
+    });
   }
 
   __syncwarp();
