@@ -245,6 +245,32 @@ def test_ragged_weight_quantiser(cuda_device):
         assert torch.equal(q[e].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[e], s1)
 
 
+def test_row_quantiser_is_the_division(cuda_device):
+    """Codes of groups of every size, zeros of both signs, subnormals, infinities
+    and NaN: the bits of the IEEE quotient x / s, clamped and rounded."""
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    for k in range(6):
+        x = torch.randn(8192, 1024, generator=g, device=cuda_device)
+        if k > 0:  # spread inside a group, then groups from 2^-120 to 2^120
+            x *= torch.exp2(torch.rand(8192, 1024, generator=g, device=cuda_device) * -8 * k)
+            x *= torch.exp2(torch.randint(-120, 120, (8192, 1), generator=g, device=cuda_device).float())
+        x = x.to(torch.bfloat16)
+        x[0, ::3], x[1, ::2], x[2, :] = 0.0, -0.0, 0.0
+        x[3, 7], x[4, 9] = float("inf"), float("nan")
+        x[5] = torch.finfo(torch.bfloat16).max
+        x[6] = torch.tensor(2.0 ** -130)
+        x[7, ::2] = -x[7, ::2].abs() * 0.0
+        q, s = per_token_group_quant_fp8(x)
+        v = x.float().view(8192, 8, 128)
+        amax = torch.nan_to_num(v.abs(), nan=0.0, posinf=float("inf")).amax(2)
+        sw = (amax / torch.full_like(amax, 448.0)).clamp_min(1e-12)
+        assert torch.equal(s, sw)
+        quot = v / sw.unsqueeze(2)
+        clamped = torch.where(quot.isnan(), torch.full_like(quot, -448.0), quot.clamp(-448.0, 448.0))
+        want = clamped.to(FP8).view(8192, 1024)
+        assert torch.equal(q.view(torch.uint8), want.view(torch.uint8))
+
+
 def test_refusals_on_device(cuda_device):
     x, wq, ws = make(cuda_device, 4, 200, 256)
     with pytest.raises(ValueError):

@@ -107,11 +107,11 @@ __device__ __forceinline__ void quant_row_segment(const QuantArgs& a, int64_t ro
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     uint32_t lo = 0, hi = 0;
-    const float scale = group_scale(m);
+    const float scale = group_scale(m), rcp = __frcp_rn(scale);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) lo |= (uint32_t)quant_e4m3(v[i][j], scale) << (8 * j);
+    for (int j = 0; j < 2; ++j) lo |= quant_e4m3x2_by(v[i][2 * j], v[i][2 * j + 1], scale, rcp) << (16 * j);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) hi |= (uint32_t)quant_e4m3(v[i][4 + j], scale) << (8 * j);
+    for (int j = 0; j < 2; ++j) hi |= quant_e4m3x2_by(v[i][4 + 2 * j], v[i][5 + 2 * j], scale, rcp) << (16 * j);
     packed[i] = make_uint2(lo, hi);
     scl[i] = scale;
   }
