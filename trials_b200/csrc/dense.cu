@@ -180,11 +180,9 @@ cudaError_t launch_epi_dense(const DensePlan& pl, const CUtensorMap& tm_x, const
       return pl.quantise_x ? launch_split_dense<EPI, 16, true>(pl, tm_x, tm_w, p, early_w, stream)
                            : launch_split_dense<EPI, 16, false>(pl, tm_x, tm_w, p, early_w, stream);
     case 32:
-      if constexpr (EPI == DENSE_OUT) return launch_split_dense<EPI, 32, false>(pl, tm_x, tm_w, p, early_w, stream);
-      return cudaErrorInvalidValue;
+      return launch_split_dense<EPI, 32, false>(pl, tm_x, tm_w, p, early_w, stream);
     case 64:
-      if constexpr (EPI == DENSE_OUT) return launch_split_dense<EPI, 64, false>(pl, tm_x, tm_w, p, early_w, stream);
-      return cudaErrorInvalidValue;
+      return launch_split_dense<EPI, 64, false>(pl, tm_x, tm_w, p, early_w, stream);
     case kDensePair:
       return launch_pair_dense<EPI>(tm_x, tm_w, p, stream);
     default:
@@ -220,13 +218,7 @@ DensePlan split_plan(int epi, int64_t M, int64_t N, int nkb, bool x_bf16) {
   while (s > 1 && (s * 2 > nkb || units * halves * s > most)) s /= 2;
   const int per = (nkb + s - 1) / s;
   // A token or two: a CTA can quantise its own K blocks of bf16 rows.
-  const bool few = T == 16 && M * per <= kQuantGroups && split_stages<16>(per, tt, true) > 0;
-  const bool qx = few && x_bf16;
-  // Gate/up with rows of 256 columns to a CTA (token-major) is as fast from the
-  // first token on (9.8 against 10.0 us at 1, 11.8 against 12.4 at 64), so this
-  // kernel only serves it where it saves the quantising launch; fp8 rows go the
-  // same way, so that they give the same bits.
-  if (epi == DENSE_SILU && !few) return pl;
+  const bool qx = x_bf16 && T == 16 && M * per <= kQuantGroups && split_stages<16>(per, tt, true) > 0;
   const int stages = qx ? 1
                         : (T == 16 ? split_stages<16>(per, tt, false)
                                    : (T == 32 ? split_stages<32>(per, tt, false) : split_stages<64>(per, tt, false)));
@@ -247,19 +239,24 @@ DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K, bool x_bf16) {
   DensePlan pl = split_plan(epi, M, N, nkb, x_bf16);
   if (pl.cfg != kDenseTok) return pl;
   // Token-major tiles while a cluster of two or more CTAs can share each (512 x
-  // 4096 x 6144: 20.9 us against 30.7 with pairs), pairs from there on (1024: 31.5
-  // against 32.9; 2048: 59.5 against 64.3).
+  // 4096 x 6144: 20.9 us against 30.7 with pairs); then whichever takes fewer
+  // rounds, a K block of either costing about the same (89 tokens leave half of a
+  // pair's tile empty), and pairs if neither does (1024 x 4096 x 6144: 31.5 against
+  // 32.9; 2048: 59.5 against 64.3).
   using T = DenseTokCfg;
-  const int64_t units = (M + T::TM - 1) / T::TM * ((N + T::TN - 1) / T::TN);
-  if (units > resident_tok(2)) {
+  const int64_t n_nt = (N + T::TN - 1) / T::TN;
+  const int64_t units = (M + T::TM - 1) / T::TM * n_nt, pair_units = (M + 2 * T::TM - 1) / (2 * T::TM) * n_nt;
+  int s = 8;
+  while (s > 1 && (s * 2 > nkb || units > resident_tok(s))) --s;
+  const int64_t rounds = (units + resident_tok(1) - 1) / resident_tok(1);
+  const int64_t pair_rounds = (pair_units + resident_pairs() - 1) / resident_pairs();
+  if (units > resident_tok(2) && rounds >= pair_rounds) {
     pl.cfg = kDensePair;
     pl.splits = 1;
     pl.x_box_rows = DensePairCfg::TM;
     pl.w_box_rows = DensePairCfg::WR;
     return pl;
   }
-  int s = 8;
-  while (s > 1 && (s * 2 > nkb || units > resident_tok(s))) --s;
   pl.splits = s;
   pl.x_box_rows = T::TM;
   pl.w_box_rows = T::TN;

@@ -143,37 +143,52 @@ __device__ __forceinline__ uint2 dense_residual4(const DenseParams& p, int64_t m
   return *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.residual) + m * p.ld_res + n);
 }
 
-// Four consecutive outputs n..n+3 of token m; res: dense_residual4 of them.
+// Four consecutive outputs n..n+3 of token m (p.vec); res: dense_residual4 of them.
 __device__ __forceinline__ void dense_store4(const DenseParams& p, int64_t m, int n, float4 v, uint2 res) {
-  if (p.vec) {
-    if (n >= p.N) return;
-    if (p.residual) {
-      const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&res.x));
-      const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&res.y));
-      v.x += lo.x;
-      v.y += lo.y;
-      v.z += hi.x;
-      v.w += hi.y;
-    }
-    if (p.out_f32) {
-      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + m * p.ld_out + n) = v;
-    } else {
-      const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
-      uint2 pk;
-      pk.x = *reinterpret_cast<const uint32_t*>(&lo);
-      pk.y = *reinterpret_cast<const uint32_t*>(&hi);
-      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + m * p.ld_out + n) = pk;
-    }
-    return;
+  if (n >= p.N) return;
+  if (p.residual) {
+    const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&res.x));
+    const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&res.y));
+    v.x += lo.x;
+    v.y += lo.y;
+    v.z += hi.x;
+    v.w += hi.y;
   }
+  if (p.out_f32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + m * p.ld_out + n) = v;
+  } else {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+    uint2 pk;
+    pk.x = *reinterpret_cast<const uint32_t*>(&lo);
+    pk.y = *reinterpret_cast<const uint32_t*>(&hi);
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + m * p.ld_out + n) = pk;
+  }
+}
+
+// A lane's columns 4 * lane .. of 128 -> columns lane, lane + 32, lane + 64, lane + 96.
+__device__ __forceinline__ float4 spread_cols(float4 v, int lane) {
+  float o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int src = (lane >> 2) + 8 * i;
+    const float x = __shfl_sync(0xffffffffu, v.x, src), y = __shfl_sync(0xffffffffu, v.y, src);
+    const float z = __shfl_sync(0xffffffffu, v.z, src), w = __shfl_sync(0xffffffffu, v.w, src);
+    o[i] = (lane & 2) ? ((lane & 1) ? w : z) : ((lane & 1) ? y : x);
+  }
+  return make_float4(o[0], o[1], o[2], o[3]);
+}
+
+// Rows that are not vector aligned: outputs n, n + 32, n + 64, n + 96 of token m,
+// so that a store instruction of the warp covers 32 consecutive ones.
+__device__ __forceinline__ void dense_store_cols(const DenseParams& p, int64_t m, int n, float4 v) {
   const float a[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (n + i < p.N) {
+    if (n + 32 * i < p.N) {
       float y = a[i];
-      if (p.residual) y += __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[m * p.ld_res + n + i]);
-      if (p.out_f32) static_cast<float*>(p.out)[m * p.ld_out + n + i] = y;
-      else static_cast<__nv_bfloat16*>(p.out)[m * p.ld_out + n + i] = __float2bfloat16_rn(y);
+      if (p.residual) y += __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[m * p.ld_res + n + 32 * i]);
+      if (p.out_f32) static_cast<float*>(p.out)[m * p.ld_out + n + 32 * i] = y;
+      else static_cast<__nv_bfloat16*>(p.out)[m * p.ld_out + n + 32 * i] = __float2bfloat16_rn(y);
     }
 }
 
@@ -245,7 +260,10 @@ __device__ __forceinline__ void finish_tokens_of(const DenseParams& p, int64_t m
         if (lane == 0) p.s[m * p.ld_s + unit] = scale;
       } else {
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) dense_store4(p, m, n0 + 128 * h + lane * 4, sum[h], res[b][h]);
+        for (int h = 0; h < HALVES; ++h) {
+          if (p.vec) dense_store4(p, m, n0 + 128 * h + lane * 4, sum[h], res[b][h]);
+          else dense_store_cols(p, m, n0 + 128 * h + lane, spread_cols(sum[h], lane));
+        }
       }
     }
   }
