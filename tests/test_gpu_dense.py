@@ -50,7 +50,9 @@ def check(out, y, bound):
 
 SHAPES = [(1, 128, 128), (1, 4096, 1024), (2, 6144, 2048), (3, 256, 6144), (11, 4096, 512), (2, 1, 128), (7, 300, 256), (16, 256, 6144), (17, 129, 384), (33, 576, 896),
           (64, 2048, 2048), (65, 257, 512), (100, 8, 1152), (127, 1000, 256), (128, 512, 640), (129, 383, 2048),
-          (255, 64, 128), (300, 1280, 768), (512, 640, 1024), (1000, 384, 512), (2100, 520, 384), (5000, 130, 256)]
+          (255, 64, 128), (300, 1280, 768), (512, 640, 1024), (1000, 384, 512), (2100, 520, 384), (5000, 130, 256),
+          # 128-column tiles: split, one each over two rounds, and pairs past that
+          (300, 1000, 1152), (777, 77, 768), (20000, 24, 256), (40000, 128, 128)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)

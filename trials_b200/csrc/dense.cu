@@ -62,15 +62,15 @@ void cluster_launch(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int
 // time then share weight tiles and activations through L2.
 constexpr int kTileGroup = 8;
 
-template <int EPI>
+template <int EPI, int TN>
 cudaError_t launch_tok_dense(const DensePlan& pl, const CUtensorMap& tm_x, const CUtensorMap& tm_w,
                              const DenseParams& p, bool early_w, cudaStream_t stream) {
-  using C = DenseTokCfg;
+  using C = DenseTokCfg<TN>;
   static std::atomic<int> done[kMaxDevices];
-  auto kernel = dense_tok_kernel<EPI>;
+  auto kernel = dense_tok_kernel<EPI, TN>;
   const cudaError_t err = allow_smem(kernel, C::SMEM_BYTES, current_device(), done);
   if (err != cudaSuccess) return err;
-  const int n_mt = (p.M + C::TM - 1) / C::TM, n_nt = (p.N + C::TN - 1) / C::TN;
+  const int n_mt = (p.M + C::TM - 1) / C::TM, n_nt = (p.N + TN - 1) / TN;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
   cluster_launch(cfg, attr, pl.splits, dim3((unsigned)n_mt * n_nt * pl.splits), C::THREADS, C::SMEM_BYTES, stream);
@@ -86,7 +86,7 @@ cudaError_t launch_tok_dense(const DensePlan& pl, const CUtensorMap& tm_x, const
 // system's), and none beside a CTA that takes all of it, as the token-major, pair
 // and expert kernels do with 194 KB and more.
 constexpr int kSplitSmem = 113 * 1024, kSplitSmemMin = 78 * 1024;
-static_assert(DenseTokCfg::SMEM_BYTES + kSplitSmemMin + 2048 > 228 * 1024 &&
+static_assert(DenseTokCfg<256>::SMEM_BYTES + kSplitSmemMin + 2048 > 228 * 1024 &&
                   DensePairCfg::SMEM_BYTES + kSplitSmemMin + 2048 > 228 * 1024,
               "no split CTA beside one that takes all of the TMEM");
 
@@ -148,7 +148,9 @@ int resident_clusters(K kernel, int R, int threads, int smem, std::atomic<int> (
 }
 int resident_tok(int R) {
   static std::atomic<int> cache[kMaxDevices][9];
-  return resident_clusters(dense_tok_kernel<DENSE_OUT>, R, DenseTokCfg::THREADS, DenseTokCfg::SMEM_BYTES, cache);
+  using C = DenseTokCfg<256>;  // 128 columns take the same threads and shared memory
+  static_assert(C::THREADS == DenseTokCfg<128>::THREADS && C::SMEM_BYTES == DenseTokCfg<128>::SMEM_BYTES, "");
+  return resident_clusters(dense_tok_kernel<DENSE_OUT, 256>, R, C::THREADS, C::SMEM_BYTES, cache);
 }
 int resident_pairs() {
   static std::atomic<int> cache[kMaxDevices][9];
@@ -186,7 +188,10 @@ cudaError_t launch_epi_dense(const DensePlan& pl, const CUtensorMap& tm_x, const
     case kDensePair:
       return launch_pair_dense<EPI>(tm_x, tm_w, p, stream);
     default:
-      return launch_tok_dense<EPI>(pl, tm_x, tm_w, p, early_w, stream);
+      // (DENSE_SILU: a tile holds 128 gate and their 128 up rows.)
+      if constexpr (EPI == DENSE_OUT)
+        if (pl.w_box_rows == 128) return launch_tok_dense<EPI, 128>(pl, tm_x, tm_w, p, early_w, stream);
+      return launch_tok_dense<EPI, 256>(pl, tm_x, tm_w, p, early_w, stream);
   }
 }
 
@@ -238,16 +243,39 @@ DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K, bool x_bf16) {
   const int nkb = (int)(K / 128);
   DensePlan pl = split_plan(epi, M, N, nkb, x_bf16);
   if (pl.cfg != kDenseTok) return pl;
-  // Token-major tiles while a cluster of two or more CTAs can share each (512 x
-  // 4096 x 6144: 20.9 us against 30.7 with pairs); then whichever takes fewer
-  // rounds, a K block of either costing about the same (89 tokens leave half of a
-  // pair's tile empty), and pairs if neither does (1024 x 4096 x 6144: 31.5 against
+  // The largest cluster, one wave of them, that shares `tiles` output tiles' K blocks.
+  auto most_splits = [nkb](int64_t tiles) {
+    int s = 8;
+    while (s > 1 && (s * 2 > nkb || tiles > resident_tok(s))) --s;
+    return s;
+  };
+  const int64_t m_tiles = (M + 127) / 128;
+  // Tiles of 128 columns where they still leave three CTAs to each, since a CTA then
+  // has few K blocks and half the sums to exchange (300 x 1000 x 4096: 8.7 us against
+  // 11.3; 100 x 4096 x 6144: 11.1 against 13.1), or where 256 would be half empty and
+  // two rounds do (7796 x 11 x 3584: 14.4 against 21.5, 30000 x 128 x 4096: 39 against
+  // 44; in the six of 100000 x 100 x 2048 persistent pairs hide the start of each: 80
+  // against 90). With two CTAs each or one the longer tile's K block, 0.6 us against
+  // 2 x 0.44, decides (200 x 4096 x 6144: 15.0 against 15.6 with two, 200 x 6144 x
+  // 2048: 11.8 against 13.5 with one).
+  if (epi == DENSE_OUT) {
+    const int s = most_splits(m_tiles * ((N + 127) / 128));
+    if (s >= 3 || (N <= 128 && m_tiles <= 2 * resident_tok(1))) {
+      pl.splits = s;
+      pl.x_box_rows = 128;
+      pl.w_box_rows = 128;
+      return pl;
+    }
+  }
+  // Token-major tiles of 256 columns while a cluster of two or more CTAs can share
+  // each (512 x 4096 x 6144: 20.9 us against 30.7 with pairs); then whichever takes
+  // fewer rounds, a K block of either costing about the same (89 tokens leave half of
+  // a pair's tile empty), and pairs if neither does (1024 x 4096 x 6144: 31.5 against
   // 32.9; 2048: 59.5 against 64.3).
-  using T = DenseTokCfg;
+  using T = DenseTokCfg<256>;
   const int64_t n_nt = (N + T::TN - 1) / T::TN;
-  const int64_t units = (M + T::TM - 1) / T::TM * n_nt, pair_units = (M + 2 * T::TM - 1) / (2 * T::TM) * n_nt;
-  int s = 8;
-  while (s > 1 && (s * 2 > nkb || units > resident_tok(s))) --s;
+  const int64_t units = m_tiles * n_nt, pair_units = (M + 2 * T::TM - 1) / (2 * T::TM) * n_nt;
+  const int s = most_splits(units);
   const int64_t rounds = (units + resident_tok(1) - 1) / resident_tok(1);
   const int64_t pair_rounds = (pair_units + resident_pairs() - 1) / resident_pairs();
   if (units > resident_tok(2) && rounds >= pair_rounds) {

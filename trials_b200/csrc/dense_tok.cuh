@@ -5,14 +5,16 @@
 // from TMEM, multiplied by xs * ws and added to an fp32 accumulator in registers
 // ("promotion").
 //
-// Tile: MMA M = 128 tokens (x), MMA N = 256 weight rows (w), one 128x256x32 MMA
-// per K step. An epilogue thread owns one token and 128 weight rows of one scale
-// block, so its factor is one scalar per K block. A K block takes about 0.6 us
-// whatever its surroundings: the hand-off of a partial (commit, wake-up,
-// promotion, release) against two TMEM buffers bounds it, not the operands. So
-// where tiles are fewer than SMs, a cluster of S CTAs shares a tile's K blocks;
-// their fp32 sums meet in distributed shared memory, where CTA c finishes the
-// tokens c, c + S, .. (added in CTA order: the result does not depend on timing).
+// Tile: MMA M = 128 tokens (x), MMA N = TN = 256 or 128 weight rows (w), one MMA
+// per K step. An epilogue thread owns one token and TN / 2 weight rows of one
+// scale block, so its factor is one scalar per K block. A K block takes about 0.6
+// us with TN = 256 and 0.44 with 128 whatever its surroundings: the hand-off of a
+// partial (commit, wake-up, promotion, release) against the TMEM buffers bounds
+// it, not the operands. So where tiles are fewer than SMs, a cluster of S CTAs
+// shares a tile's K blocks; their fp32 sums meet in distributed shared memory,
+// where CTA c finishes the tokens c, c + S, .. (added in CTA order: the result
+// does not depend on timing). That exchange moves each CTA's sums once, 128 KB
+// with TN = 256 in 2 to 4 us: TN = 128 halves it.
 // Warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 4..11 epilogue (two
 // warpgroups, which take over the first one's registers: 168 a thread at launch
 // spilled the accumulators' neighbours).
@@ -25,31 +27,32 @@
 
 namespace b200moe {
 
+template <int TN_>
 struct DenseTokCfg {
   static constexpr int TM = 128;
-  static constexpr int TN = 256;
-  static constexpr int EW = 8;     // epilogue warps: 4 lane quarters x 2 column halves
-  static constexpr int COLS = 128; // columns per epilogue thread
+  static constexpr int TN = TN_;
+  static constexpr int EW = 8;          // epilogue warps: 4 lane quarters x 2 column halves
+  static constexpr int COLS = TN / 2;   // columns per epilogue thread
   static constexpr int THREADS = 128 + 32 * EW;
   // 384 threads x 168 registers at launch = 128 x (40 + 232 + 232).
   static constexpr int REGS_LOAD = 40, REGS_EPI = 232;
   static constexpr int X_BYTES = TM * 128;
   static constexpr int W_BYTES = TN * 128;
   static constexpr int TILE_BYTES = X_BYTES + W_BYTES;
-  static constexpr int NBUF = 2;
   static constexpr int TMEM_COLS = 512;
-  static constexpr int NSTAGE = 4;
+  static constexpr int NBUF = TMEM_COLS / TN;
+  static constexpr int NSTAGE = 192 * 1024 / TILE_BYTES;
   static constexpr int SUM_BYTES = TM * TN * 4;  // a CTA's sums, in the tiles' place
   static constexpr int SMEM_BYTES = 1024 + NSTAGE * TILE_BYTES + 256;
   static_assert(SUM_BYTES <= NSTAGE * TILE_BYTES, "sums reuse the tiles");
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
 
-template <int EPI>
-__global__ void __launch_bounds__(DenseTokCfg::THREADS, 1)
+template <int EPI, int TN>
+__global__ void __launch_bounds__(DenseTokCfg<TN>::THREADS, 1)
     dense_tok_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                      const DenseParams p, int splits, int n_mt, int n_nt, int group, int early_w) {
-  using C = DenseTokCfg;
+  using C = DenseTokCfg<TN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* tiles = smem;
@@ -66,7 +69,7 @@ __global__ void __launch_bounds__(DenseTokCfg::THREADS, 1)
   const int rank = (int)cluster_ctarank();  // this CTA's share of K
   int mt, nt;
   unit_coords(blockIdx.x / splits, n_mt, n_nt, group, mt, nt);
-  const int m0 = mt * C::TM, w0 = nt * C::TN;
+  const int m0 = mt * C::TM, w0 = nt * TN;
   const int kb0 = (int)((int64_t)NKB * rank / splits);
   const int nkb = (int)((int64_t)NKB * (rank + 1) / splits) - kb0;
 
@@ -220,16 +223,17 @@ __global__ void __launch_bounds__(DenseTokCfg::THREADS, 1)
     if (live) {
 #pragma unroll
       for (int c = 0; c < C::COLS / 4; ++c)
-        *reinterpret_cast<float4*>(tiles + r * 1024 + (((h * 32 + c) ^ (r & 7)) << 4)) =
+        *reinterpret_cast<float4*>(tiles + r * (TN * 4) + (((h * (C::COLS / 4) + c) ^ (r & 7)) << 4)) =
             make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
     }
     __syncwarp();
     cluster_sync_all();
     const uint32_t sums = smem_u32(tiles);
     const int rows = p.M - m0 < C::TM ? p.M - m0 : C::TM;
-    finish_tokens<EPI, 2>(p, m0, w0, splits, lane, rank + splits * ew, splits * C::EW, rows, [&](int t, int s, int hh) {
-      return mapa_shared(sums + (uint32_t)(t * 1024 + (((hh * 32 + lane) ^ (t & 7)) << 4)), s);
-    });
+    finish_tokens<EPI, TN / 128>(
+        p, m0, w0, splits, lane, rank + splits * ew, splits * C::EW, rows, [&](int t, int s, int hh) {
+          return mapa_shared(sums + (uint32_t)(t * (TN * 4) + (((hh * 32 + lane) ^ (t & 7)) << 4)), s);
+        });
   }
 
   __syncwarp();
