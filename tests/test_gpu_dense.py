@@ -52,7 +52,9 @@ SHAPES = [(1, 128, 128), (1, 4096, 1024), (2, 6144, 2048), (3, 256, 6144), (11, 
           (64, 2048, 2048), (65, 257, 512), (100, 8, 1152), (127, 1000, 256), (128, 512, 640), (129, 383, 2048),
           (255, 64, 128), (300, 1280, 768), (512, 640, 1024), (1000, 384, 512), (2100, 520, 384), (5000, 130, 256),
           # 128-column tiles: split, one each over two rounds, and pairs past that
-          (300, 1000, 1152), (777, 77, 768), (20000, 24, 256), (40000, 128, 128)]
+          (300, 1000, 1152), (777, 77, 768), (20000, 24, 256), (40000, 128, 128),
+          # pairs: whole and partial boxes of the output
+          (5000, 328, 256), (4100, 776, 512), (9000, 256, 1024)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -68,6 +70,8 @@ def test_linear(cuda_device, M, N, K):
     res = torch.randn(M, N, device=cuda_device).to(torch.bfloat16)
     with_res = fp8_block_linear(xq, wq, ws, x_scale=xs, residual=res)
     assert torch.equal(with_res, (f32 + res.float()).to(torch.bfloat16))
+    with_res32 = fp8_block_linear(xq, wq, ws, x_scale=xs, residual=res, out_dtype=torch.float32)
+    assert torch.equal(with_res32, f32 + res.float())
     into = res.clone()
     assert fp8_block_linear(x, wq, ws, residual=into, out=into) is into
     assert torch.equal(into, with_res)
@@ -145,7 +149,7 @@ def test_empty_batch(cuda_device):
     assert fp8_mlp(x[:0], w13, s13, w2, s2).shape == (0, 256)
 
 
-@pytest.mark.parametrize("M,N", [(3, 200), (130, 200), (130, 264), (70, 512)])
+@pytest.mark.parametrize("M,N", [(3, 200), (130, 200), (130, 264), (70, 512), (5000, 328)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_strides_and_surroundings(cuda_device, M, N, dtype):
     """Row strides of every operand; nothing outside the result is written."""

@@ -73,17 +73,18 @@ int make_tmap_u8(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, i
   return B200MOE_OK;
 }
 
-// 2D bf16 matrix [rows][cols] (row pitch = cols elements), boxes of 64
-// columns (128 bytes) x box_rows, 128-byte swizzle: the token-major stage-2
-// output, stored from swizzled shared-memory staging.
-int make_tmap_rows_bf16(CUtensorMap* m, void* base, int64_t rows, int64_t cols, int box_rows) {
+// 2D bf16 or fp32 matrix [rows][cols] (row pitch = ld elements), boxes of 128
+// bytes of columns x box_rows, 128-byte swizzle: outputs that are stored from
+// swizzled shared-memory staging (and the residual that is read the same way).
+int make_tmap_rows(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, bool f32, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(B200MOE_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable%s");
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
-  cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * (f32 ? 4 : 2)};
+  cuuint32_t box[2] = {f32 ? 32u : 64u, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1u, 1u};
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr,
+  CUresult r = fn(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                  const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(B200MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed%s");
@@ -255,7 +256,7 @@ int run_gemm(int epi, const uint8_t* a_q, const float* a_sT, int64_t as_ld, int6
   CUtensorMap tm_o = tm_w;
   if (epi == EPI_COMBINE && tile_tokens == 128 && !p.rows_by_slot) {
     if (!aligned16(p.out_pair)) return fail(B200MOE_ERR_UNSUPPORTED, "out_pair: 16-byte alignment required%s");
-    st = make_tmap_rows_bf16(&tm_o, p.out_pair, rows_cap, Nw, 16);
+    st = make_tmap_rows(&tm_o, p.out_pair, rows_cap, Nw, Nw, false, 16);
     if (st) return st;
   }
   const int64_t units_cap = chunks_cap * (Nw / 256);
@@ -1550,13 +1551,19 @@ int run_dense(const char* name, int epi, const DensePlan& pl, DenseInput in, int
     p.xs = in.s;
     p.ld_xs = in.ld_s;
   }
+  CUtensorMap tm_o = tm_w, tm_r = tm_w;
+  if (epi == DENSE_OUT && pl.out_box_rows > 0 && p.vec) {
+    st = make_tmap_rows(&tm_o, p.out, M, N, p.ld_out, p.out_f32 != 0, pl.out_box_rows);
+    if (!st && p.residual) st = make_tmap_rows(&tm_r, p.residual, M, N, p.ld_res, false, pl.out_box_rows);
+    if (st) return st;
+  }
   p.ws = w_scale;
   p.M = (int)M;
   p.N = (int)N;
   p.K = (int)K;
   p.err = err_word;
   p.timeout_ns = kTimeoutNs;
-  return cuda_status(launch_dense(epi, pl, tm_x, tm_w, p, chained, (cudaStream_t)stream), name);
+  return cuda_status(launch_dense(epi, pl, tm_x, tm_w, tm_o, tm_r, p, chained, (cudaStream_t)stream), name);
 }
 
 int check_dense_out(const char* name, int64_t M, int64_t N, const void* residual, int64_t ld_res, const void* out,

@@ -87,7 +87,7 @@ cudaError_t launch_tok_dense(const DensePlan& pl, const CUtensorMap& tm_x, const
 // and expert kernels do with 194 KB and more.
 constexpr int kSplitSmem = 113 * 1024, kSplitSmemMin = 78 * 1024;
 static_assert(DenseTokCfg<256>::SMEM_BYTES + kSplitSmemMin + 2048 > 228 * 1024 &&
-                  DensePairCfg::SMEM_BYTES + kSplitSmemMin + 2048 > 228 * 1024,
+                  DensePairCfg<DENSE_OUT>::SMEM_BYTES + kSplitSmemMin + 2048 > 228 * 1024,
               "no split CTA beside one that takes all of the TMEM");
 
 // Stages that fit next to the scales (and quantised rows) of nkb K blocks, or 0.
@@ -154,13 +154,14 @@ int resident_tok(int R) {
 }
 int resident_pairs() {
   static std::atomic<int> cache[kMaxDevices][9];
-  return resident_clusters(dense_pair_kernel<DENSE_OUT>, 2, DensePairCfg::THREADS, DensePairCfg::SMEM_BYTES, cache);
+  using C = DensePairCfg<DENSE_OUT>;
+  return resident_clusters(dense_pair_kernel<DENSE_OUT>, 2, C::THREADS, C::SMEM_BYTES, cache);
 }
 
 template <int EPI>
-cudaError_t launch_pair_dense(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const DenseParams& p,
-                              cudaStream_t stream) {
-  using C = DensePairCfg;
+cudaError_t launch_pair_dense(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const CUtensorMap& tm_o,
+                              const CUtensorMap& tm_r, const DenseParams& p, cudaStream_t stream) {
+  using C = DensePairCfg<EPI>;
   static std::atomic<int> done[kMaxDevices];
   auto kernel = dense_pair_kernel<EPI>;
   cudaError_t err = allow_smem(kernel, C::SMEM_BYTES, current_device(), done);
@@ -171,12 +172,12 @@ cudaError_t launch_pair_dense(const CUtensorMap& tm_x, const CUtensorMap& tm_w, 
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
   cluster_launch(cfg, attr, 2, dim3(2 * pairs), C::THREADS, C::SMEM_BYTES, stream);
-  return cudaLaunchKernelEx(&cfg, kernel, tm_x, tm_w, p, n_mt, n_nt, kTileGroup);
+  return cudaLaunchKernelEx(&cfg, kernel, tm_x, tm_w, tm_o, tm_r, p, n_mt, n_nt, kTileGroup);
 }
 
 template <int EPI>
 cudaError_t launch_epi_dense(const DensePlan& pl, const CUtensorMap& tm_x, const CUtensorMap& tm_w,
-                             const DenseParams& p, bool early_w, cudaStream_t stream) {
+                             const CUtensorMap& tm_o, const CUtensorMap& tm_r, const DenseParams& p, bool early_w, cudaStream_t stream) {
   switch (pl.cfg) {
     case 16:
       return pl.quantise_x ? launch_split_dense<EPI, 16, true>(pl, tm_x, tm_w, p, early_w, stream)
@@ -186,7 +187,7 @@ cudaError_t launch_epi_dense(const DensePlan& pl, const CUtensorMap& tm_x, const
     case 64:
       return launch_split_dense<EPI, 64, false>(pl, tm_x, tm_w, p, early_w, stream);
     case kDensePair:
-      return launch_pair_dense<EPI>(tm_x, tm_w, p, stream);
+      return launch_pair_dense<EPI>(tm_x, tm_w, tm_o, tm_r, p, stream);
     default:
       // (DENSE_SILU: a tile holds 128 gate and their 128 up rows.)
       if constexpr (EPI == DENSE_OUT)
@@ -281,8 +282,9 @@ DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K, bool x_bf16) {
   if (units > resident_tok(2) && rounds >= pair_rounds) {
     pl.cfg = kDensePair;
     pl.splits = 1;
-    pl.x_box_rows = DensePairCfg::TM;
-    pl.w_box_rows = DensePairCfg::WR;
+    pl.x_box_rows = DensePairCfg<DENSE_OUT>::TM;
+    pl.w_box_rows = DensePairCfg<DENSE_OUT>::WR;
+    pl.out_box_rows = 32;
     return pl;
   }
   pl.splits = s;
@@ -292,9 +294,10 @@ DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K, bool x_bf16) {
 }
 
 cudaError_t launch_dense(int epi, const DensePlan& pl, const CUtensorMap& tm_x, const CUtensorMap& tm_w,
-                         const DenseParams& p, bool early_w, cudaStream_t stream) {
-  return epi == DENSE_SILU ? launch_epi_dense<DENSE_SILU>(pl, tm_x, tm_w, p, early_w, stream)
-                           : launch_epi_dense<DENSE_OUT>(pl, tm_x, tm_w, p, early_w, stream);
+                         const CUtensorMap& tm_o, const CUtensorMap& tm_r, const DenseParams& p, bool early_w,
+                         cudaStream_t stream) {
+  return epi == DENSE_SILU ? launch_epi_dense<DENSE_SILU>(pl, tm_x, tm_w, tm_o, tm_r, p, early_w, stream)
+                           : launch_epi_dense<DENSE_OUT>(pl, tm_x, tm_w, tm_o, tm_r, p, early_w, stream);
 }
 
 }  // namespace b200moe

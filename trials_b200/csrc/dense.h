@@ -42,12 +42,14 @@ struct DensePlan {
   int quantise_x;  // bf16 rows are quantised inside the kernel
   int x_box_rows;
   int w_box_rows;
+  int out_box_rows;  // DENSE_OUT of vector-aligned rows (p.vec) through TMA; 0: plain stores
 };
 // x_bf16: the rows come in bf16 (quantise_x can only be set then).
 DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K, bool x_bf16);
 // early_w: the kernel ahead of this one in the stream belongs to the same call
-// and does not write w.
+// and does not write w. tm_o, tm_r: output and residual in boxes of 128 bytes x
+// out_box_rows; any map where they are not used.
 cudaError_t launch_dense(int epi, const DensePlan& pl, const CUtensorMap& tm_x, const CUtensorMap& tm_w,
-                         const DenseParams& p, bool early_w, cudaStream_t stream);
+                         const CUtensorMap& tm_o, const CUtensorMap& tm_r, const DenseParams& p, bool early_w, cudaStream_t stream);
 
 }  // namespace b200moe

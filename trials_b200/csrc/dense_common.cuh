@@ -64,78 +64,6 @@ __device__ __forceinline__ void store_codes(const float (&acc)[NC], float scale,
   }
 }
 
-// Stores 32 rows (m0.., one per lane) x NC columns (n0..) of fp32 results. They
-// pass through st (4 KB of this warp, rows of 32 columns, 16-byte pieces
-// swizzled by row), so that a store instruction covers whole 64-byte (bf16) or
-// 128-byte (f32) runs of 4 rows, or 32 consecutive columns of one row where
-// rows are not aligned.
-template <int NC>
-__device__ __forceinline__ void dense_store_tile(const DenseParams& p, int m0, int n0, const float (&acc)[NC],
-                                                 uint8_t* st, int lane) {
-  const int rows = p.M - m0 < 32 ? p.M - m0 : 32;
-#pragma unroll
-  for (int cb = 0; cb < NC / 32; ++cb) {
-    const int n1 = n0 + cb * 32;
-    if (n1 < p.N) {  // warp-uniform
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        *reinterpret_cast<float4*>(st + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-            make_float4(acc[cb * 32 + 4 * c], acc[cb * 32 + 4 * c + 1], acc[cb * 32 + 4 * c + 2],
-                        acc[cb * 32 + 4 * c + 3]);
-      __syncwarp();
-      if (p.vec) {  // N is a multiple of 8: a piece of 4 columns exists or does not
-        const int c = lane & 7, n = n1 + 4 * c;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = i * 4 + (lane >> 3);
-          if (r < rows && n < p.N) {
-            float4 v = *reinterpret_cast<const float4*>(st + r * 128 + ((c ^ (r & 7)) << 4));
-            const int64_t m = m0 + r;
-            if (p.residual) {
-              const uint2 raw = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.residual) +
-                                                                m * p.ld_res + n);
-              const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
-              const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
-              v.x += lo.x;
-              v.y += lo.y;
-              v.z += hi.x;
-              v.w += hi.y;
-            }
-            if (p.out_f32) {
-              *reinterpret_cast<float4*>(static_cast<float*>(p.out) + m * p.ld_out + n) = v;
-            } else {
-              const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
-              uint2 pk;
-              pk.x = *reinterpret_cast<const uint32_t*>(&lo);
-              pk.y = *reinterpret_cast<const uint32_t*>(&hi);
-              *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + m * p.ld_out + n) = pk;
-            }
-          }
-        }
-      } else if (n1 + lane < p.N) {
-        for (int r = 0; r < rows; ++r) {
-          float v = *reinterpret_cast<const float*>(st + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-          const int64_t m = m0 + r;
-          const int n = n1 + lane;
-          if (p.residual) v += __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[m * p.ld_res + n]);
-          if (p.out_f32) static_cast<float*>(p.out)[m * p.ld_out + n] = v;
-          else static_cast<__nv_bfloat16*>(p.out)[m * p.ld_out + n] = __float2bfloat16_rn(v);
-        }
-      }
-      __syncwarp();
-    }
-  }
-}
-
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-
 // The residual of four consecutive outputs n.. of token m, where rows are vector
 // aligned (p.vec); zero bits otherwise.
 __device__ __forceinline__ uint2 dense_residual4(const DenseParams& p, int64_t m, int n) {
@@ -163,6 +91,59 @@ __device__ __forceinline__ void dense_store4(const DenseParams& p, int64_t m, in
     pk.y = *reinterpret_cast<const uint32_t*>(&hi);
     *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + m * p.ld_out + n) = pk;
   }
+}
+
+// Stores 32 rows (m0.., one per lane) x NC columns (n0..) of fp32 results where rows
+// are not vector aligned (!p.vec). They pass through st (4 KB of this warp, rows of 32
+// columns, 16-byte pieces swizzled by row), so that a store instruction covers 32
+// consecutive columns of one row. The residuals of 8 rows are asked for together: a
+// load between stores, which may alias it, waits for the one before.
+template <int NC>
+__device__ __forceinline__ void dense_store_tile(const DenseParams& p, int m0, int n0, const float (&acc)[NC],
+                                                 uint8_t* st, int lane) {
+  const int rows = p.M - m0 < 32 ? p.M - m0 : 32;
+#pragma unroll
+  for (int cb = 0; cb < NC / 32; ++cb) {
+    const int n1 = n0 + cb * 32, n = n1 + lane;
+    if (n1 < p.N) {  // warp-uniform
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<float4*>(st + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+            make_float4(acc[cb * 32 + 4 * c], acc[cb * 32 + 4 * c + 1], acc[cb * 32 + 4 * c + 2],
+                        acc[cb * 32 + 4 * c + 3]);
+      __syncwarp();
+      for (int r1 = 0; r1 < rows; r1 += 8) {
+        float res[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          res[i] = p.residual && n < p.N && r1 + i < rows
+                       ? __bfloat162float(
+                             static_cast<const __nv_bfloat16*>(p.residual)[(int64_t)(m0 + r1 + i) * p.ld_res + n])
+                       : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = r1 + i;
+          if (n < p.N && r < rows) {
+            float v = *reinterpret_cast<const float*>(st + r * 128 + (((lane >> 2) ^ i) << 4) + (lane & 3) * 4);
+            if (p.residual) v += res[i];
+            const int64_t at = (int64_t)(m0 + r) * p.ld_out + n;
+            if (p.out_f32) static_cast<float*>(p.out)[at] = v;
+            else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
+}
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
 
 // A lane's columns 4 * lane .. of 128 -> columns lane, lane + 32, lane + 64, lane + 96.

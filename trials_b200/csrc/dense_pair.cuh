@@ -10,6 +10,15 @@
 // multicast); the leader's MMA thread commits to `empty` / `tfull` of both CTAs;
 // both CTAs' epilogue warps release a TMEM buffer on the leader's `tempty`.
 // Warps: 0 TMA producer, 1 MMA issuer (leader) and TMEM owner, 4..11 epilogue.
+//
+// The promotion of partials is what a K block waits for, so the epilogue warps leave
+// the output to TMA: they put a tile's rounded results into swizzled staging and go on
+// with the next tile; its residual was brought there the same way while its K blocks
+// were multiplied. Plain stores by the same warps took 4 us a tile and a residual read
+// beside them 12 more, one latency after another: 5772 x 7424 x 768 took 82.5 us and 202
+// with a residual, like this 52.0 and 60.5; 2048 x 6144 x 2048 41.8 and 78.1, now 35.2
+// and 38.3. With long rows of K they hide behind the power limit (8192 x 6144 x 6144:
+// 323 and 458, now 324 and 336).
 #pragma once
 
 #include "dense_common.cuh"
@@ -17,6 +26,7 @@
 
 namespace b200moe {
 
+template <int EPI>
 struct DensePairCfg {
   static constexpr int TM = 128;   // tokens per CTA
   static constexpr int TN = 256;   // weight rows per pair
@@ -30,27 +40,96 @@ struct DensePairCfg {
   static constexpr int TILE_BYTES = X_BYTES + W_BYTES;
   static constexpr int NBUF = 2;
   static constexpr int TMEM_COLS = 512;
-  static constexpr int NSTAGE = 6;
-  static constexpr int RED = 2 * 2 * TM * 4;
-  static constexpr int STAGING = EW * 32 * 128;
-  static constexpr int SMEM_BYTES = 1024 + NSTAGE * TILE_BYTES + (STAGING > RED ? STAGING : RED) + 256;
+  static constexpr int NSTAGE = EPI == DENSE_SILU ? 6 : 5;
+  static constexpr int STAGING = 32 * COLS * 2;  // of a warp: its 32 x 128 results in bf16
+  // DENSE_SILU: two buffers of row maxima; DENSE_OUT: staging.
+  static constexpr int SCRATCH = EPI == DENSE_SILU ? 2 * 2 * TM * 4 : EW * STAGING;
+  static constexpr int SMEM_BYTES = 1024 + NSTAGE * TILE_BYTES + SCRATCH + 256;
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
 
+// The epilogue of a warp's 32 tokens (m0 ..) x 128 columns (n0 ..) of DENSE_OUT. tm_o:
+// boxes of 32 rows x 128 bytes of the output; st: 8 KB in swizzled rows of 128 bytes,
+// holding the residual in two boxes of 64 columns (if any) and then the results.
+__device__ __forceinline__ void pair_store_tile(const DenseParams& p, const CUtensorMap& tm_o, int m0, int n0,
+                                                float (&acc)[128], uint8_t* st, int lane) {
+  uint8_t* row = st + lane * 128;
+  const int sw = lane & 7;
+  if (p.residual) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(row + (j >> 3) * 4096 + (((j & 7) ^ sw) << 4));
+      const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v[e]));
+        acc[j * 8 + 2 * e] += f.x;
+        acc[j * 8 + 2 * e + 1] += f.y;
+      }
+    }
+  } else {
+    if (lane == 0) bulk_wait_read_all();  // the tile before has left the staging
+  }
+  __syncwarp();
+  if (p.out_f32) {
+    // Four boxes of 32 columns, two at a time.
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half) {
+        if (lane == 0) bulk_wait_read_all();
+        __syncwarp();
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float* a = acc + half * 64 + j * 4;
+        *reinterpret_cast<float4*>(row + (j >> 3) * 4096 + (((j & 7) ^ sw) << 4)) = make_float4(a[0], a[1], a[2], a[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        for (int b = 0; b < 2; ++b)
+          if (n0 + half * 64 + b * 32 < p.N) tma_store_2d(&tm_o, st + b * 4096, n0 + half * 64 + b * 32, m0);
+        bulk_commit_group();
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      uint32_t v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat162 c = __floats2bfloat162_rn(acc[j * 8 + 2 * e], acc[j * 8 + 2 * e + 1]);
+        v[e] = *reinterpret_cast<const uint32_t*>(&c);
+      }
+      *reinterpret_cast<uint4*>(row + (j >> 3) * 4096 + (((j & 7) ^ sw) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      for (int b = 0; b < 2; ++b)
+        if (n0 + b * 64 < p.N) tma_store_2d(&tm_o, st + b * 4096, n0 + b * 64, m0);
+      bulk_commit_group();
+    }
+  }
+}
+
+// tm_o, tm_r (DENSE_OUT with p.vec): the output and, if any, the residual.
 template <int EPI>
-__global__ void __launch_bounds__(DensePairCfg::THREADS, 1)
+__global__ void __launch_bounds__(DensePairCfg<EPI>::THREADS, 1)
     dense_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                      const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ CUtensorMap tm_r,
                       const DenseParams p, int n_mt, int n_nt, int group) {
-  using C = DensePairCfg;
+  using C = DensePairCfg<EPI>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* tiles = smem;
   uint8_t* scratch = tiles + C::NSTAGE * C::TILE_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(scratch + (EPI == DENSE_SILU ? C::RED : C::STAGING));
+  uint64_t* full = reinterpret_cast<uint64_t*>(scratch + C::SCRATCH);
   uint64_t* empty = full + C::NSTAGE;
   uint64_t* tfull = empty + C::NSTAGE;
   uint64_t* tempty = tfull + C::NBUF;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + C::NBUF);
+  uint64_t* res_full = tempty + C::NBUF;  // of each epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + C::EW);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -69,6 +148,7 @@ __global__ void __launch_bounds__(DensePairCfg::THREADS, 1)
       mbar_init(&tfull[b], 1);
       mbar_init(&tempty[b], 2 * C::EW);  // leader: the epilogue warps of both CTAs
     }
+    for (int e = 0; e < C::EW; ++e) mbar_init(&res_full[e], 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -79,6 +159,7 @@ __global__ void __launch_bounds__(DensePairCfg::THREADS, 1)
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&tm_x);
     prefetch_tmap(&tm_w);
+    if (EPI == DENSE_OUT && p.vec) prefetch_tmap(&tm_o);
   }
   __syncwarp();
   tc_fence_before();
@@ -184,8 +265,10 @@ __global__ void __launch_bounds__(DensePairCfg::THREADS, 1)
     const int r = q * 32 + lane;  // token of this CTA's half tile
     const uint32_t taddr0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * C::COLS);
     int buf = 0, parity = 0;
-    uint32_t bphase = 0;
+    uint32_t bphase = 0, rphase = 0;
     bool ok = true;
+    uint8_t* st = scratch + ew * C::STAGING;
+    const bool residual = EPI == DENSE_OUT && p.vec && p.residual;
     // A warp whose wait gave up still walks all tiles (without waiting or
     // storing), so that the named barriers below keep their full count.
     for (int u = pair; u < n_units; u += n_pairs) {
@@ -201,6 +284,7 @@ __global__ void __launch_bounds__(DensePairCfg::THREADS, 1)
 #pragma unroll
       for (int j = 0; j < C::COLS; ++j) acc[j] = 0.f;
       float sc_next = __ldg(xsr) * __ldg(wsr);
+      bool asked = false;  // for the residual
       for (int kb = 0; kb < NKB && ok; ++kb) {
         const float sc = sc_next;
         float xs_n = 0.f, ws_n = 0.f;
@@ -224,6 +308,16 @@ __global__ void __launch_bounds__(DensePairCfg::THREADS, 1)
           bphase ^= 1;
         }
         sc_next = xs_n * ws_n;
+        if (kb == 0 && residual && live) {
+          asked = true;
+          if (lane == 0) {
+            bulk_wait_read_all();  // the tile before has left the staging
+            const int boxes = n0 + 64 < p.N ? 2 : 1;
+            mbar_arrive_expect_tx(&res_full[ew], boxes * 4096);
+            for (int b = 0; b < boxes; ++b)
+              tma_load_2d(st + b * 4096, &tm_r, &res_full[ew], n0 + b * 64, m0 + q * 32);
+          }
+        }
       }
       if constexpr (EPI == DENSE_SILU) {
         // The 1x128 group is both column halves. One barrier per tile: the
@@ -240,9 +334,21 @@ __global__ void __launch_bounds__(DensePairCfg::THREADS, 1)
           if (h == 0) p.s[m * p.ld_s + nt] = scale;
         }
       } else {
-        if (ok && live) dense_store_tile(p, m0 + q * 32, n0, acc, scratch + ew * 4096, lane);
+        if (asked) {  // waited for even when the tile is given up
+          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&res_full[ew], rphase, p.timeout_ns))) {
+            ok = false;
+            atomicOr(p.err, ERR_DEV_TIMEOUT);
+            *abort_flag = 1;
+          }
+          rphase ^= 1;
+        }
+        if (ok && live) {
+          if (p.vec) pair_store_tile(p, tm_o, m0 + q * 32, n0, acc, st, lane);
+          else dense_store_tile(p, m0 + q * 32, n0, acc, st, lane);
+        }
       }
     }
+    if (EPI == DENSE_OUT && lane == 0) bulk_wait_all();  // the output has arrived
   }
 
   __syncwarp();
