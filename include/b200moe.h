@@ -575,8 +575,9 @@ B200MOE_API int b200moe_combine_reduce(const void* out_pair, const int32_t* slot
  * ld_x / ld_xs are row strides in elements of x or x_q / x_scale (ld_xs is not
  * read with bf16 rows). w (N, K) fp8 with row stride ld_w bytes; w_scale
  * (ceil(N/128), K/128) contiguous. residual (M, N) bf16 or NULL; it may be out
- * itself (the same address and stride, with bf16 out). Any M >= 0 and N >= 1;
- * K % 128 == 0. Activation and weight rows start 16-byte aligned.
+ * itself (the same address and stride, with bf16 out). Otherwise out overlaps no
+ * input. Any M >= 0 and N >= 1; K % 128 == 0. Activation and weight rows start
+ * 16-byte aligned.
  *
  * b200moe_gate_up: the product with w13 (2I, H), gate/up rows interleaved (row
  * 2j = gate j, 2j+1 = up j) as in the layer, then silu(gate) * up in fp32,
@@ -585,7 +586,7 @@ B200MOE_API int b200moe_combine_reduce(const void* out_pair, const int32_t* slot
  *
  * b200moe_mlp: b200moe_gate_up followed by b200moe_linear with w2 (H, I) on its
  * result, bit for bit: a dense or shared expert, residual = the routed output
- * to add to. Weights contiguous; workspace b200moe_mlp_workspace_size() bytes,
+ * to add to; out may also be x. Weights contiguous; workspace b200moe_mlp_workspace_size() bytes,
  * 256-byte aligned.
  *
  * The calls take their twenty arguments in a struct whose members are all 8 bytes

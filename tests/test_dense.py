@@ -43,6 +43,33 @@ def test_linear_workspace(kw):
     assert linear(**kw) == _lib.ERR_WORKSPACE
 
 
+def test_output_over_an_input():
+    """Refused where the product may still read what it stores over; columns side
+    by side in one buffer are apart. (The base: P = M rows of K = N = 256.)"""
+    base = dict(N=256, ld_out=256, w=1 << 30, ws=1 << 32, out=1 << 34)
+    for kw in (dict(out=P), dict(out=P + 3 * 512 + 510, ld_out=300), dict(out=1 << 30), dict(out=1 << 32),
+               dict(x=None, xq=P, xs=1 << 36, ld_xs=2, out=1 << 36), dict(x=None, xq=P, xs=1 << 36, out=P),
+               dict(res=(1 << 34) + 2, ld_res=256), dict(res=1 << 34, ld_res=260),
+               dict(res=1 << 34, ld_res=256, f32=1), dict(ld_out=1024, out=P + 256, ld_x=1024),
+               dict(res=(1 << 34) + 768, ld_res=512, ld_out=512)):
+        assert linear(**{**base, **kw}) == _lib.ERR_INVALID_ARG, kw
+        assert b"overlap" in _lib.lib().b200moe_last_error_message()
+
+    def mlp(out, res=None, ld_res=256):
+        return call("b200moe_mlp", P, None, None, 256, 0, 4, 256, 128, 1 << 28, 1 << 29, 1 << 30, 1 << 32, res, ld_res,
+                    out, 256, P, 1 << 20, P, None)
+
+    for args in ((1 << 30,), (1 << 32,), (1 << 34, (1 << 34) + 4)):
+        assert mlp(*args) == _lib.ERR_INVALID_ARG
+
+    def gate_up(q, s):
+        return call("b200moe_gate_up", P, None, None, 256, 0, 4, 256, 128, 1 << 30, 256, 1 << 32, q, 128, s, 1, P,
+                    1 << 20, P, None)
+
+    for args in ((P, 1 << 36), (1 << 34, P), (1 << 30, 1 << 36), (1 << 34, 1 << 32)):
+        assert gate_up(*args) == _lib.ERR_INVALID_ARG
+
+
 def test_empty_batches_launch_nothing():
     L = _lib.lib()
     assert linear(M=0, x=None, out=None, work=None, nwork=0) == _lib.OK

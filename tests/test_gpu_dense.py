@@ -277,6 +277,47 @@ def test_row_quantiser_is_the_division(cuda_device):
         assert torch.equal(q.view(torch.uint8), want.view(torch.uint8))
 
 
+@pytest.mark.parametrize("M", [1, 2, 40, 200, 1300])
+def test_in_place(cuda_device, M):
+    """A residual stream updated in place; outputs beside the rows in one buffer."""
+    H, I = 512, 1024
+    x, w13, s13 = make(cuda_device, M, 2 * I, H, M)
+    _, w2, s2 = make(cuda_device, 1, H, I, M + 1)
+    want = fp8_mlp(x, w13, s13, w2, s2, residual=x)
+    h = x.clone()
+    assert fp8_mlp(h, w13, s13, w2, s2, residual=h, out=h) is h
+    assert torch.equal(h, want)
+    h = x.clone()
+    assert torch.equal(fp8_mlp(h, w13, s13, w2, s2, out=h), fp8_mlp(x, w13, s13, w2, s2))
+    _, wq, ws = make(cuda_device, 1, H, H, 5)
+    buf = torch.cat([x, x, x], 1)
+    fp8_block_linear(buf[:, :H], wq, ws, residual=buf[:, 2 * H:], out=buf[:, H:2 * H])
+    assert torch.equal(buf, torch.cat([x, fp8_block_linear(x, wq, ws, residual=x), x], 1))
+    for out, res in ((x, None), (buf[:, 1:H + 1], None if M > 1 else buf[:, :H]), (buf[:, 2:H + 2], buf[:, :H])):
+        with pytest.raises(ValueError, match="overlap"):
+            fp8_block_linear(buf[:, :H] if out is not x else x, wq, ws, residual=res, out=out)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^31 outputs, more than 2^32 bytes of rows: the last rows are the
+    rows' own product."""
+    M, N, K = 270_000, 8192, 128
+    if torch.cuda.get_device_properties(cuda_device).total_memory < 40e9:
+        pytest.skip("needs 40 GB")
+    x, wq, ws = make(cuda_device, 1000, N, K)
+    big = x.repeat(M // 1000, 1)
+    want = fp8_block_linear(x, wq, ws, residual=None)
+    out = fp8_block_linear(big, wq, ws)
+    for first in (0, M // 2, M - 1000):
+        assert torch.equal(out[first:first + 1000], want)
+    assert torch.equal(fp8_block_linear(big, wq, ws, residual=out, out=out)[-1000:],
+                       fp8_block_linear(x, wq, ws, residual=want))
+    del out, big
+    x, w13, s13 = make(cuda_device, 500, 256, 8192)
+    q, s = fp8_gate_up(x.repeat(600, 1), w13, s13)
+    assert torch.equal(q[-500:].view(torch.uint8), q[:500].view(torch.uint8)) and torch.equal(s[-500:], s[:500])
+
+
 def test_refusals_on_device(cuda_device):
     x, wq, ws = make(cuda_device, 4, 200, 256)
     with pytest.raises(ValueError):

@@ -1484,6 +1484,32 @@ struct DenseInput {
   int64_t ld_x, ld_s;
 };
 
+// A matrix in memory: `rows` rows of `width` bytes, `ld` bytes apart.
+struct Span {
+  const void* p;
+  int64_t rows, ld, width;
+};
+// Whether two of them share bytes: exact for equal strides (columns side by side in
+// one buffer do not), else by the ranges they lie in.
+bool overlap(const Span& a, const Span& b) {
+  if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0) return false;
+  const int64_t a0 = (int64_t)reinterpret_cast<uintptr_t>(a.p), b0 = (int64_t)reinterpret_cast<uintptr_t>(b.p);
+  if (a0 + (a.rows - 1) * a.ld + a.width <= b0 || b0 + (b.rows - 1) * b.ld + b.width <= a0) return false;
+  if (a.ld != b.ld) return true;
+  const int64_t d = ((b0 - a0) % a.ld + a.ld) % a.ld;
+  return d < a.width || d + b.width > a.ld;
+}
+Span rows_of(const DenseInput& in, int64_t M, int64_t K) {
+  return in.x ? Span{in.x, M, in.ld_x * 2, K * 2} : Span{in.q, M, in.ld_x, K};
+}
+Span scales_of(const DenseInput& in, int64_t M, int64_t K) {
+  return Span{in.x ? nullptr : in.s, M, in.ld_s * 4, K / 128 * 4};
+}
+// Whether an output shares bytes with what its product still reads when it is stored.
+bool overwrites(const Span& out, int64_t N, int64_t K, const uint8_t* w, int64_t ld_w, const float* w_scale) {
+  return overlap(out, Span{w, N, ld_w, K}) || overlap(out, Span{w_scale, 1, 0, (N + 127) / 128 * (K / 128) * 4});
+}
+
 int check_dense(const char* name, const DenseInput& in, int64_t M, int64_t N, int64_t K, const uint8_t* w,
                 int64_t ld_w, const float* w_scale, const int32_t* err_word) {
   if (M < 0 || N <= 0 || K <= 0 || !w || !w_scale || !err_word || ld_w < K)
@@ -1583,6 +1609,17 @@ int check_dense_out(const char* name, int64_t M, int64_t N, const void* residual
   return B200MOE_OK;
 }
 
+int check_dense_overlap(const char* name, const DenseParams& p, int64_t M, int64_t N, int64_t K, const uint8_t* w,
+                        int64_t ld_w, const float* w_scale) {
+  const int64_t esize = p.out_f32 ? 4 : 2;
+  const Span out{p.out, M, p.ld_out * esize, N * esize};
+  const bool in_place = p.residual == p.out && !p.out_f32 && (p.ld_res == p.ld_out || M == 1);
+  if (overwrites(out, N, K, w, ld_w, w_scale) ||
+      (!in_place && overlap(out, Span{p.residual, M, p.ld_res * 2, N * 2})))
+    return fail(B200MOE_ERR_INVALID_ARG, "%s: the output overlaps an input", name);
+  return B200MOE_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1605,7 +1642,12 @@ int b200moe_linear(const b200moe_linear_args* a) {
   if (M == 0) return B200MOE_OK;
   const DensePlan pl = dense_plan(DENSE_OUT, M, N, K, in.x != nullptr);
   st = check_dense_work(name, a->workspace, a->workspace_bytes, dense_bytes(pl, M, K, in.x != nullptr));
+  if (!st) st = check_dense_overlap(name, p, M, N, K, a->w, a->ld_w, a->w_scale);
   if (st) return st;
+  const int64_t esize = p.out_f32 ? 4 : 2;
+  const Span out{p.out, M, p.ld_out * esize, N * esize};
+  if (overlap(out, rows_of(in, M, K)) || overlap(out, scales_of(in, M, K)))
+    return fail(B200MOE_ERR_INVALID_ARG, "%s: the output overlaps an input", name);
   return run_dense(name, DENSE_OUT, pl, in, M, N, K, a->w, a->ld_w, a->w_scale, p, false,
                    static_cast<uint8_t*>(a->workspace), a->err_word, a->stream);
 }
@@ -1627,6 +1669,10 @@ int b200moe_gate_up(const b200moe_gate_up_args* a) {
   const DensePlan pl = dense_plan(DENSE_SILU, M, 2 * I, H, in.x != nullptr);
   st = check_dense_work(name, a->workspace, a->workspace_bytes, dense_bytes(pl, M, H, in.x != nullptr));
   if (st) return st;
+  for (const Span& out : {Span{a->q, M, a->ld_q, I}, Span{a->s, M, a->ld_s * 4, I / 128 * 4}})
+    if (overlap(out, rows_of(in, M, H)) || overlap(out, scales_of(in, M, H)) ||
+        overwrites(out, 2 * I, H, a->w13, a->ld_w, a->w13_scale))
+      return fail(B200MOE_ERR_INVALID_ARG, "%s: an output overlaps an input", name);
   DenseParams p{};
   p.q = a->q;
   p.ld_q = a->ld_q;
@@ -1681,6 +1727,8 @@ int b200moe_mlp(const b200moe_mlp_args* a) {
   if (M == 0) return B200MOE_OK;
   const MlpPlan m = plan_mlp(M, H, I, in.x != nullptr);
   st = check_dense_work(name, a->workspace, a->workspace_bytes, m.total);
+  // (x has been read when out is stored, so out may be x.)
+  if (!st) st = check_dense_overlap(name, p, M, H, I, a->w2, I, a->w2_scale);
   if (st) return st;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   uint8_t* iq = ws + m.off_inter;

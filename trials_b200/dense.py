@@ -151,7 +151,8 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     or fp8 e4m3 with x_scale (M, K/128); weight (N, K) fp8 e4m3 with
     weight_scale (ceil(N/128), K/128) f32; residual (M, N) bf16, added in fp32.
     Accumulated in fp32 and rounded once to out_dtype (bf16 or f32). Any M and
-    N; K % 128 == 0. out may be residual itself. See b200moe_linear."""
+    N; K % 128 == 0. out may be residual itself and overlaps no other input. See
+    b200moe_linear."""
     index = _device_of(x, weight, weight_scale, x_scale, residual, out)
     if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
         raise NotImplementedError("out_dtype must be bf16 or float32")
@@ -212,7 +213,7 @@ def fp8_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
             out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """(M, H) bf16 = w2 . (silu(gate) * up) (+ residual): fp8_gate_up with w13
     (2I, H), then fp8_block_linear with w2 (H, I), in one call (same bits).
-    out may be residual itself. See b200moe_mlp."""
+    out may be residual or x itself. See b200moe_mlp."""
     index = _device_of(x, w13, w13_scale, w2, w2_scale, x_scale, residual, out)
     x, x_scale, ld_x, ld_s = _input(x, x_scale)
     M, H = x.shape
