@@ -236,6 +236,33 @@ def test_other_stream_and_graph(cuda_device, M):
     assert torch.equal(outs[1], fp8_mlp(-x, w13, s13, w2, s2))
 
 
+def test_calls_at_once(cuda_device):
+    """Every kind of product on six streams at the same time."""
+    _, w13, s13 = make(cuda_device, 1, 2048, 2048)
+    _, w2, s2 = make(cuda_device, 1, 2048, 1024)
+    inputs = [make(cuda_device, M, 128, 2048, M)[0] for M in (1, 16, 64, 100, 400, 1500)]
+
+    def work(x):
+        y = fp8_mlp(x, w13, s13, w2, s2, residual=x)
+        return y, fp8_block_linear(x, w13[:1000], s13[:8], residual=y[:, :1000])
+
+    want = [work(x) for x in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    torch.cuda.synchronize()
+    got = [[] for _ in inputs]
+    for _ in range(20):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(work(inputs[k]))
+    torch.cuda.synchronize()
+    for k, outs in enumerate(got):
+        for y, z in outs:
+            assert torch.equal(y, want[k][0]) and torch.equal(z, want[k][1])
+    for s in streams:
+        with torch.cuda.stream(s):
+            assert read_device_error(layer_error_word(cuda_device)) == 0
+
+
 def test_ragged_weight_quantiser(cuda_device):
     for N in (1, 100, 128, 200, 300):
         w = torch.randn(N, 384, device=cuda_device).to(torch.bfloat16)

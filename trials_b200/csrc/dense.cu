@@ -6,6 +6,7 @@
 #include "dense_pair.cuh"
 #include "dense_split.cuh"
 #include "dense_tok.cuh"
+#include "moe_gemm_tok2.cuh"
 #include "launch.h"
 
 namespace b200moe {
@@ -86,8 +87,12 @@ cudaError_t launch_tok_dense(const DensePlan& pl, const CUtensorMap& tm_x, const
 // system's), and none beside a CTA that takes all of it, as the token-major, pair
 // and expert kernels do with 194 KB and more.
 constexpr int kSplitSmem = 113 * 1024, kSplitSmemMin = 78 * 1024;
-static_assert(DenseTokCfg<256>::SMEM_BYTES + kSplitSmemMin + 2048 > 228 * 1024 &&
-                  DensePairCfg<DENSE_OUT>::SMEM_BYTES + kSplitSmemMin + 2048 > 228 * 1024,
+constexpr bool alone(int smem) { return smem + kSplitSmemMin + 2 * 1024 > 228 * 1024; }
+static_assert(alone(DenseTokCfg<256>::SMEM_BYTES) && alone(DenseTokCfg<128>::SMEM_BYTES) &&
+                  alone(DensePairCfg<DENSE_OUT>::SMEM_BYTES) && alone(DensePairCfg<DENSE_SILU>::SMEM_BYTES) &&
+                  alone(GemmCfg<32, 1>::SMEM_BYTES) && alone(GemmCfg<64, 1>::SMEM_BYTES) &&
+                  alone(GemmCfg<64, 2>::SMEM_BYTES) && alone(TokCfgE<EPI_SILU>::SMEM_BYTES) &&
+                  alone(TokCfgE<EPI_COMBINE>::SMEM_BYTES) && alone(Tok2Cfg::SMEM_BYTES),
               "no split CTA beside one that takes all of the TMEM");
 
 // Stages that fit next to the scales (and quantised rows) of nkb K blocks, or 0.
