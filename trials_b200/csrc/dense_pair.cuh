@@ -16,9 +16,9 @@
 // with the next tile; its residual was brought there the same way while its K blocks
 // were multiplied. Plain stores by the same warps took 4 us a tile and a residual read
 // beside them 12 more, one latency after another: 5772 x 7424 x 768 took 82.5 us and 202
-// with a residual, like this 52.0 and 60.5; 2048 x 6144 x 2048 41.8 and 78.1, now 35.2
-// and 38.3. With long rows of K they hide behind the power limit (8192 x 6144 x 6144:
-// 323 and 458, now 324 and 336).
+// with a residual, like this 49 and 63; 2048 x 6144 x 2048 41.8 and 78.1, now 34 and
+// 38; 8192 x 6144 x 6144 323 and 458, now 321 and 332. Five stages carry this as well as
+// six with half the staging, stored in two steps (52 and 61 to 54 and 65).
 #pragma once
 
 #include "dense_common.cuh"
@@ -284,7 +284,18 @@ __global__ void __launch_bounds__(DensePairCfg<EPI>::THREADS, 1)
 #pragma unroll
       for (int j = 0; j < C::COLS; ++j) acc[j] = 0.f;
       float sc_next = __ldg(xsr) * __ldg(wsr);
-      bool asked = false;  // for the residual
+      // The residual is asked for here although the tile before has just been stored: a
+      // branch for it in the loop, after the first K block, slowed every K block (2048 x
+      // 7168 x 18432: 337 us against 316; 5772 x 7424 x 768 with its six: 60.5, here 63).
+      const bool asked = residual && live;
+      if (asked && lane == 0) {
+        bulk_wait_read_all();  // the tile before has left the staging
+        const int boxes = n0 + 64 < p.N ? 2 : 1;
+        mbar_arrive_expect_tx(&res_full[ew], boxes * 4096);
+        for (int b = 0; b < boxes; ++b)
+          tma_load_2d(st + b * 4096, &tm_r, &res_full[ew], n0 + b * 64, m0 + q * 32);
+      }
+      __syncwarp();
       for (int kb = 0; kb < NKB && ok; ++kb) {
         const float sc = sc_next;
         float xs_n = 0.f, ws_n = 0.f;
@@ -308,16 +319,6 @@ __global__ void __launch_bounds__(DensePairCfg<EPI>::THREADS, 1)
           bphase ^= 1;
         }
         sc_next = xs_n * ws_n;
-        if (kb == 0 && residual && live) {
-          asked = true;
-          if (lane == 0) {
-            bulk_wait_read_all();  // the tile before has left the staging
-            const int boxes = n0 + 64 < p.N ? 2 : 1;
-            mbar_arrive_expect_tx(&res_full[ew], boxes * 4096);
-            for (int b = 0; b < boxes; ++b)
-              tma_load_2d(st + b * 4096, &tm_r, &res_full[ew], n0 + b * 64, m0 + q * 32);
-          }
-        }
       }
       if constexpr (EPI == DENSE_SILU) {
         // The 1x128 group is both column halves. One barrier per tile: the
