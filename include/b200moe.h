@@ -110,11 +110,19 @@ B200MOE_API int b200moe_router_topk(const void* logits, int logits_bf16, int64_t
  * the selected scores sum to 0, the weights are 0. num_experts % num_groups
  * == 0, topk <= topk_groups * num_experts / num_groups, at most 32 groups. The
  * reference runs one group (measure_xcd_imbalance.py:50-55); more are what
- * other checkpoints of this layer's geometries route with. */
-B200MOE_API int b200moe_router_topk_grouped(const void* logits, int logits_bf16, int64_t M, int num_experts,
-                                            int num_groups, int topk_groups, int topk, int scoring,
-                                            const float* correction_bias, int renormalize, float scaling,
-                                            float* topk_weights, int32_t* topk_ids, void* stream);
+ * other checkpoints of this layer's geometries route with. The arguments come in
+ * a struct whose members are all 8 bytes wide, as those of b200moe_linear. */
+typedef struct b200moe_router_grouped_args {
+  const void* logits;
+  int64_t logits_bf16, M, num_experts, num_groups, topk_groups, topk, scoring;
+  const float* correction_bias;
+  int64_t renormalize;
+  double scaling;
+  float* topk_weights;
+  int32_t* topk_ids;
+  void* stream;
+} b200moe_router_grouped_args;
+B200MOE_API int b200moe_router_topk_grouped(const b200moe_router_grouped_args* args);
 
 /* ------------------------------------------------------------------------
  * Activation quantisation: per_token_group_quant_fp8(x, 128).

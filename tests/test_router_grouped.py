@@ -1,4 +1,6 @@
 """Refusals of group-limited routing, checked on the host (no GPU needed)."""
+import struct
+
 import pytest
 import torch
 
@@ -8,17 +10,18 @@ P = 256
 
 
 def call(M=4, E=64, G=8, T=3, k=6, scoring=1, bias=P, logits=P, w=P, ids=P):
-    return _lib.lib().b200moe_router_topk_grouped(logits, 0, M, E, G, T, k, scoring, bias, 1, 1.0, w, ids, None)
+    args = (logits, 0, M, E, G, T, k, scoring, bias, 1, 1.0, w, ids, None)
+    return _lib.lib().b200moe_router_topk_grouped(struct.pack("10qd3q", *(0 if a is None else a for a in args)))
 
 
 @pytest.mark.parametrize("kw", [
     dict(M=-1), dict(E=0), dict(k=0), dict(k=65), dict(scoring=2), dict(scoring=0), dict(logits=None), dict(w=None),
-    dict(ids=None), dict(G=0), dict(G=7), dict(G=-8), dict(T=0), dict(T=9), dict(T=1, k=9)])
+    dict(ids=None), dict(E=-(1 << 32)), dict(T=(1 << 32) + 3), dict(G=0), dict(G=7), dict(G=-8), dict(T=0), dict(T=9), dict(T=1, k=9)])
 def test_invalid_arguments(kw):
     assert call(**kw) == _lib.ERR_INVALID_ARG
 
 
-@pytest.mark.parametrize("kw", [dict(E=2048), dict(k=17, T=8), dict(G=64, T=64)])
+@pytest.mark.parametrize("kw", [dict(E=2048), dict(E=(1 << 32) + 64, k=1), dict(k=17, T=8), dict(G=64, T=64)])
 def test_unsupported_sizes(kw):
     assert call(**kw) == _lib.ERR_UNSUPPORTED
 
@@ -33,6 +36,7 @@ def test_fused_entries_check_the_groups_too():
 
 def test_empty_batch_launches_nothing():
     assert call(M=0, logits=None, w=None, ids=None) == _lib.OK
+    assert _lib.lib().b200moe_router_topk_grouped(None) == _lib.ERR_INVALID_ARG
 
 
 def test_python_arguments():

@@ -1457,15 +1457,19 @@ int b200moe_router_topk(const void* logits, int logits_bf16, int64_t M, int num_
   return cuda_status(launch_router_topk(r, M, (cudaStream_t)stream), "router_topk");
 }
 
-int b200moe_router_topk_grouped(const void* logits, int logits_bf16, int64_t M, int num_experts, int num_groups,
-                                int topk_groups, int topk, int scoring, const float* correction_bias, int renormalize,
-                                float scaling, float* topk_weights, int32_t* topk_ids, void* stream) {
-  int st = check_router_grouped("b200moe_router_topk_grouped", logits, M, num_experts, num_groups, topk_groups, topk,
-                                scoring, correction_bias, topk_weights, topk_ids);
+int b200moe_router_topk_grouped(const b200moe_router_grouped_args* a) {
+  const char* name = "b200moe_router_topk_grouped";
+  if (!a) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
+  // Sizes as int; what does not fit stays too large or negative.
+  auto size = [](int64_t v) { return (int)(v < -1 ? -1 : v > (1 << 30) ? (1 << 30) : v); };
+  const int E = size(a->num_experts), G = size(a->num_groups), T = size(a->topk_groups), k = size(a->topk);
+  const int scoring = size(a->scoring);
+  const int st = check_router_grouped(name, a->logits, a->M, E, G, T, k, scoring, a->correction_bias, a->topk_weights,
+                                      a->topk_ids);
   if (st) return st;
-  const RouterArgs r = grouped_router(logits, logits_bf16, num_experts, num_groups, topk_groups, topk, scoring,
-                                      correction_bias, renormalize, scaling, topk_weights, topk_ids);
-  return cuda_status(launch_router_topk(r, M, (cudaStream_t)stream), "router_topk_grouped");
+  const RouterArgs r = grouped_router(a->logits, a->logits_bf16 != 0, E, G, T, k, scoring, a->correction_bias,
+                                      a->renormalize != 0, (float)a->scaling, a->topk_weights, a->topk_ids);
+  return cuda_status(launch_router_topk(r, a->M, (cudaStream_t)a->stream), "router_topk_grouped");
 }
 
 }  // extern "C"
