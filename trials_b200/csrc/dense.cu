@@ -215,18 +215,24 @@ DensePlan split_plan(int epi, int64_t M, int64_t N, int nkb, bool x_bf16) {
   const int T = tt <= 16 ? 16 : (tt <= 32 ? 32 : 64);
   const int64_t units = (N + 128 * halves - 1) / (128 * halves) * n_tt;
   const int sms = sm_count_of(current_device());
-  // More than 64 tokens read the weights more than once, which only pays when
-  // the tiles are so few that 8 CTAs each still run in one wave (two CTAs an SM
-  // less what clusters of 8 cannot use): 100 x 576 x 7168 takes 7.7 us this way
-  // and 11.0 token-major, 100 x 4096 x 6144 15.3 and 12.8.
-  if (M > 64 && units * halves * 8 > (int64_t)sms * 7 / 4) return pl;
-  // CTAs along K, at least two K blocks each. Up to 4/3 of the SMs measured best:
-  // one token of 6144 x 2048 (48 tiles) takes 6.2 us with 4, 6.8 with 2 and, in
-  // two waves, 10.8 with 6; 4096 x 6144 (32 tiles) 8.9 with 4 and 9.0 with 8, 64
-  // tokens of it 11.4 and 11.9.
+  // CTAs along K, at least two K blocks each.
   int s = 8 / halves;
-  const int64_t most = M > 64 ? (int64_t)sms * 7 / 4 : (int64_t)sms * 4 / 3;
-  while (s > 1 && (s * 2 > nkb || units * halves * s > most)) s /= 2;
+  while (s > 1 && s * 2 > nkb) s /= 2;
+  if (M > 64) {
+    // More than 64 tokens read the weights more than once, which pays while the tiles'
+    // clusters run in one wave, two CTAs an SM less what clusters cannot use (gate/up of
+    // 200 x 2048 x 256 5.9 us, token-major 8.7; 1500 x 1024 x 256 6.2 and 7.8). With long
+    // K and DENSE_OUT the token-major tiles of 128 columns are the better ones as soon as
+    // two CTAs share an SM (200 x 576 x 7168, 160 CTAs: 10.0 and 8.5; 300 x 100 x 6144,
+    // 40 CTAs: 6.7 and 7.5; 500 x 1000 x 1024, 256 CTAs: 7.2 and 6.6).
+    const int64_t most = epi == DENSE_SILU || s <= 2 ? (int64_t)sms * 7 / 4 : sms;
+    if (units * halves * s > most) return pl;
+  } else {
+    // Up to 4/3 of the SMs measured best: one token of 6144 x 2048 (48 tiles) takes 6.2
+    // us with 4 CTAs along K, 6.8 with 2 and, in two waves, 10.8 with 6; 4096 x 6144 (32
+    // tiles) 8.9 with 4 and 9.0 with 8, 64 tokens of it 11.4 and 11.9.
+    while (s > 1 && units * halves * s > (int64_t)sms * 4 / 3) s /= 2;
+  }
   const int per = (nkb + s - 1) / s;
   // A token or two: a CTA can quantise its own K blocks of bf16 rows.
   const bool qx = x_bf16 && T == 16 && M * per <= kQuantGroups && split_stages<16>(per, tt, true) > 0;
@@ -273,10 +279,12 @@ DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K, bool x_bf16) {
       return pl;
     }
   }
-  // Token-major tiles of 256 columns while a cluster of two or more CTAs can share
-  // each (512 x 4096 x 6144: 20.9 us against 30.7 with pairs); then whichever takes
-  // fewer rounds, a K block of either costing about the same (89 tokens leave half of
-  // a pair's tile empty), and pairs if neither does (1024 x 4096 x 6144: 31.5 against
+  // Token-major tiles of 256 columns while a cluster of two or more CTAs can share each
+  // (512 x 4096 x 6144: 20.9 us against 30.7 with pairs), unless two of them share so
+  // few K blocks that their exchange costs more (gate/up 300 x 1024 x 2048, 8 K blocks:
+  // 11.5 against 10.0 with pairs; 300 x 2048 x 2048, 16: 13.4 and 13.8); then whichever
+  // takes fewer rounds, a K block of either costing about the same (89 tokens leave half
+  // of a pair's tile empty), and pairs if neither does (1024 x 4096 x 6144: 31.5 against
   // 32.9; 2048: 59.5 against 64.3).
   using T = DenseTokCfg<256>;
   const int64_t n_nt = (N + T::TN - 1) / T::TN;
@@ -284,7 +292,7 @@ DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K, bool x_bf16) {
   const int s = most_splits(units);
   const int64_t rounds = (units + resident_tok(1) - 1) / resident_tok(1);
   const int64_t pair_rounds = (pair_units + resident_pairs() - 1) / resident_pairs();
-  if (units > resident_tok(2) && rounds >= pair_rounds) {
+  if ((s == 1 || (s == 2 && nkb <= 8)) && rounds >= pair_rounds) {
     pl.cfg = kDensePair;
     pl.splits = 1;
     pl.x_box_rows = DensePairCfg<DENSE_OUT>::TM;
