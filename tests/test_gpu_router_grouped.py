@@ -60,7 +60,10 @@ def check(logits, groups, topk_group, k, scoring, bias=None, renorm=True, scale=
 SHAPES = [  # M, E, groups, topk_group, k
     (1, 256, 8, 4, 8), (300, 256, 8, 4, 8), (77, 160, 8, 3, 6), (33, 64, 4, 1, 6), (129, 1024, 32, 5, 16),
     (64, 512, 16, 16, 10), (50, 60, 6, 2, 4), (50, 60, 5, 3, 16), (9, 8, 8, 2, 2), (20, 96, 3, 2, 6), (10, 30, 15, 4, 3),
-    (40, 7, 1, 1, 7), (16, 1, 1, 1, 1), (25, 330, 2, 1, 8), (31, 1000, 10, 3, 16), (2000, 128, 4, 2, 5)]
+    (40, 7, 1, 1, 7), (16, 1, 1, 1, 1), (25, 330, 2, 1, 8), (31, 1000, 10, 3, 16), (2000, 128, 4, 2, 5),
+    # lanes not all full, lanes across groups
+    (60, 250, 5, 2, 9), (55, 312, 4, 1, 16), (80, 336, 16, 9, 7), (30, 992, 31, 4, 8), (40, 1020, 17, 5, 8),
+    (21, 900, 12, 4, 8), (64, 40, 8, 2, 2)]
 
 
 @pytest.mark.parametrize("M,E,G,T,k", SHAPES)

@@ -293,11 +293,7 @@ RouterArgs grouped_router(const void* logits, int logits_bf16, int num_experts, 
   r.topk_groups = topk_groups;
   r.vec = aligned16(logits) && num_experts * (logits_bf16 ? 2 : 4) % 16 == 0;
   r.vec_bias = aligned16(correction_bias);
-  r.per = grouped_per_lane(num_experts, num_groups);
-  r.gs = num_experts / num_groups;
-  r.span_log2 = -1;
-  for (int j = 0; j < 6; ++j)
-    if (r.per << j == r.gs) r.span_log2 = j;
+  grouped_lanes(r);
   return r;
 }
 

@@ -371,7 +371,7 @@ cudaError_t launch_route_logits_impl(const AlignArgs& a_in, const RouterArgs& r,
   a.topk_ids = r.out_ids;
   a.seg_align = r.topk;
   const int C = route_ctas(a.n);
-  const int per = router_per_lane(r.E);
+  const int per = GROUPED ? grouped_per_lane(r) : router_per_lane(r.E);
   if (C > 1 && a.heavy_rows == 0) {
     if (per == 8) return launch_route_multi<true, 8, GROUPED>(a, r, C, counts, stream);
     if (per == 16) return launch_route_multi<true, 16, GROUPED>(a, r, C, counts, stream);

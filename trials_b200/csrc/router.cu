@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(kRouterWarps * 32) router_topk_kernel(const Ro
 template <bool GROUPED>
 cudaError_t launch_router_per(const RouterArgs& r, int64_t M, cudaStream_t stream) {
   const unsigned blocks = (unsigned)((M + kRouterWarps - 1) / kRouterWarps);
-  switch (router_per_lane(r.E)) {
+  switch (GROUPED ? grouped_per_lane(r) : router_per_lane(r.E)) {
     case 8:
       router_topk_kernel<8, GROUPED><<<blocks, kRouterWarps * 32, 0, stream>>>(r, M);
       break;

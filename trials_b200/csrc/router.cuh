@@ -34,9 +34,9 @@ struct RouterArgs {
   int topk_groups;     // groups whose experts may be selected
   int vec;             // rows of logits start 16-byte aligned (E * element size too)
   int vec_bias;        // bias 16-byte aligned
-  int per;             // with groups: consecutive experts a lane owns (grouped_per_lane)
+  int per;             // with groups: most experts a lane owns (grouped_lanes)
   int gs;              // experts of a group
-  int span_log2;       // log2 of the whole lanes a group fills, -1: groups do not fill lanes
+  int span_log2;       // log2 of the lanes of a group, -1: lanes own experts of several groups
 };
 
 __device__ __forceinline__ float router_logit(const RouterArgs& r, int64_t t, int e) {
@@ -163,13 +163,17 @@ __device__ __forceinline__ void route_token_warp(const RouterArgs& r, int64_t t,
 // candidates, which are put in order by their exact values in fp64; where groups
 // are that close, their scores are computed again in fp64.
 //
-// One warp per token; lane l owns the experts [l * per, (l + 1) * per) (per chosen
-// so that groups fill a power of two of whole lanes wherever it can be), so the
-// lowest lane holding a value also holds its lowest id. What bounds it is the
-// number of instructions a warp issues: a round of the selection is one redux
-// and one ballot on the lanes' best keys, the lists behind them sorted once.
-// 8,192 tokens of 256 experts in 8 groups: 10.9 us with a bias (25.7 with every
-// value compared in turn and each close token redone in fp64), 8.7 without.
+// One warp per token; a lane owns up to `per` consecutive experts, ascending with
+// the lanes, so the lowest lane holding a value also holds its lowest id. A group
+// has a power of two of lanes to itself, the last of them not always full, wherever
+// that leaves no lane more than 32 (5,580 tokens of 312 experts in 4 groups with a
+// bias: 15.9 us, 23.5 with lanes across groups). What bounds it is the number of
+// instructions a warp issues, 880 with a bias (issue slots 69% busy, the integer
+// pipe 80%; fewer registers for more warps measured 0-8% slower): a round of the
+// selection is one redux and one ballot on the lanes' best keys, the lists behind
+// them sorted once. 8,192 tokens of 256 experts in 8 groups: 10.9 us with a bias
+// (25.7 with every value compared in turn and each close token redone in fp64),
+// 8.7 without.
 // ---------------------------------------------------------------------------
 constexpr int kRouterMaxGroups = 32;
 // Bound of the error of two values c together: the sigmoid's (exp 6e-8 where its
@@ -186,6 +190,20 @@ __device__ __forceinline__ float order_value(uint32_t k) {
   return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
 }
 
+// The experts of a lane: n from e0 on.
+__device__ __forceinline__ void lane_experts(const RouterArgs& r, int lane, int& e0, int& n) {
+  int left;
+  if (r.span_log2 >= 0) {
+    const int g = lane >> r.span_log2, first = (lane & ((1 << r.span_log2) - 1)) * r.per;
+    e0 = g * r.gs + first;
+    left = g < r.groups ? r.gs - first : 0;
+  } else {
+    e0 = lane * r.per;
+    left = r.E - e0;
+  }
+  n = left < 0 ? 0 : (left < r.per ? left : r.per);
+}
+
 template <typename T>
 __device__ __forceinline__ void merge_top2(T& a1, T& a2, T b1, T b2) {
   const T lo = a1 < b1 ? a1 : b1;
@@ -195,18 +213,20 @@ __device__ __forceinline__ void merge_top2(T& a1, T& a2, T b1, T b2) {
 }
 
 // Scores of the groups, group g's in lane g (-inf in the lanes past the last),
-// from this lane's per values c. size: the magnitudes added in the score.
+// from this lane's n values c (experts e0 ..; -inf past them). size: the magnitudes
+// added in the score.
 template <typename T, int PER>
-__device__ __forceinline__ T group_scores(const RouterArgs& r, const T (&c)[PER], bool two, int lane, T& size) {
+__device__ __forceinline__ T group_scores(const RouterArgs& r, const T (&c)[PER], bool two, int lane, int e0, int n,
+                                          T& size) {
   const T ninf = -INFINITY;
-  const int groups = r.groups, gs = r.gs, per = r.per;
+  const int groups = r.groups, gs = r.gs;
   two = two && gs > 1;
   T s1 = ninf, s2 = ninf;
   if (r.span_log2 >= 0) {
     const int span = 1 << r.span_log2;
     T a1 = c[0], a2 = ninf;
 #pragma unroll
-    for (int i = 1; i < PER; ++i) {  // values past `per` are -inf
+    for (int i = 1; i < PER; ++i) {
       const T lo = a1 < c[i] ? a1 : c[i];
       a1 = a1 < c[i] ? c[i] : a1;
       a2 = a2 < lo ? lo : a2;
@@ -222,8 +242,8 @@ __device__ __forceinline__ T group_scores(const RouterArgs& r, const T (&c)[PER]
       T a1 = ninf, a2 = ninf;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int e = lane * per + i;
-        if (i < per && e >= g * gs && e < (g + 1) * gs) merge_top2(a1, a2, c[i], ninf);
+        const int e = e0 + i;
+        if (i < n && e >= g * gs && e < (g + 1) * gs) merge_top2(a1, a2, c[i], ninf);
       }
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) {
@@ -257,13 +277,12 @@ __device__ __forceinline__ double grouped_value_f64(const RouterArgs& r, int64_t
 template <int PER>
 __device__ __noinline__ uint32_t grouped_taken_f64(const RouterArgs r, int64_t t, int lane) {
   double c[PER];
+  int e0, n;
+  lane_experts(r, lane, e0, n);
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = lane * r.per + i;
-    c[i] = i < r.per && e < r.E ? grouped_value_f64(r, t, e) : -INFINITY;
-  }
+  for (int i = 0; i < PER; ++i) c[i] = i < n ? grouped_value_f64(r, t, e0 + i) : -INFINITY;
   double size;
-  const double score = group_scores<double, PER>(r, c, r.bias != nullptr, lane, size);
+  const double score = group_scores<double, PER>(r, c, r.bias != nullptr, lane, e0, n, size);
   int rank = 0;
   for (int h = 0; h < r.groups; ++h) {
     const double other = __shfl_sync(0xffffffffu, score, h);
@@ -277,13 +296,14 @@ __device__ __noinline__ uint32_t grouped_taken_f64(const RouterArgs r, int64_t t
 template <int PER>
 __device__ __noinline__ int grouped_select_f64(const RouterArgs r, int64_t t, uint32_t taken, int lane) {
   double c[PER];
-  uint32_t open = 0;  // bit i: expert lane * per + i may still be selected
+  uint32_t open = 0;  // bit i: expert e0 + i may still be selected
+  int e0, n;
+  lane_experts(r, lane, e0, n);
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int e = lane * r.per + i;
     c[i] = -INFINITY;
-    if (i < r.per && e < r.E && ((taken >> (e / r.gs)) & 1u)) {
-      c[i] = grouped_value_f64(r, t, e);
+    if (i < n && ((taken >> ((e0 + i) / r.gs)) & 1u)) {
+      c[i] = grouped_value_f64(r, t, e0 + i);
       open |= 1u << i;
     }
   }
@@ -295,7 +315,7 @@ __device__ __noinline__ int grouped_select_f64(const RouterArgs r, int64_t t, ui
     for (int i = 0; i < PER; ++i)
       if (((open >> i) & 1u) && (bi == 0x7fffffff || c[i] > bv)) {
         bv = c[i];
-        bi = lane * r.per + i;
+        bi = e0 + i;
       }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
@@ -307,7 +327,7 @@ __device__ __noinline__ int grouped_select_f64(const RouterArgs r, int64_t t, ui
         bi = oi;
       }
     }
-    if (bi / r.per == lane) open &= ~(1u << (bi - lane * r.per));
+    if (bi >= e0 && bi < e0 + n) open &= ~(1u << (bi - e0));
     if (lane == k) id = bi;
   }
   return id;
@@ -374,9 +394,10 @@ __device__ __forceinline__ void route_token_grouped(const RouterArgs& r, int64_t
   constexpr float kEps = BIASED ? kValueEps : 0.f;
   constexpr float kEpsRel = BIASED ? kValueEpsRel + PER * 1.2e-7f : 0.f;
   const int E = r.E, topk = r.topk, groups = r.groups;
-  const int per = r.per, gs = r.gs;
-  const int e0 = lane * per;
-  const bool whole = per == PER && E == 32 * PER && r.vec;  // every lane full, rows aligned for vector loads
+  const int gs = r.gs;
+  int e0, own;  // this lane's experts
+  lane_experts(r, lane, e0, own);
+  const bool whole = r.per == PER && E == 32 * PER && r.vec;  // every lane full, rows aligned for vector loads
   float x[PER];  // logits, then the values that are compared
   if (whole && !r.bf16) {
     const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(r.logits) + t * E + e0);
@@ -402,7 +423,7 @@ __device__ __forceinline__ void route_token_grouped(const RouterArgs& r, int64_t
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] = i < per && e0 + i < E ? router_logit(r, t, e0 + i) : -INFINITY;
+    for (int i = 0; i < PER; ++i) x[i] = i < own ? router_logit(r, t, e0 + i) : -INFINITY;
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) x[i] = x[i] == x[i] ? x[i] : -INFINITY;
@@ -432,11 +453,11 @@ __device__ __forceinline__ void route_token_grouped(const RouterArgs& r, int64_t
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) b[i] = i < per && e0 + i < E ? __ldg(&r.bias[e0 + i]) : 0.f;
+      for (int i = 0; i < PER; ++i) b[i] = i < own ? __ldg(&r.bias[e0 + i]) : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (whole || (i < per && e0 + i < E)) {
+      if (whole || i < own) {
         const float d = 1.0f + __expf(-x[i]);
         const float c = (d < 1e30f ? __fdividef(1.0f, d) : 0.0f) + b[i];
         x[i] = c == c ? c : -INFINITY;
@@ -448,7 +469,7 @@ __device__ __forceinline__ void route_token_grouped(const RouterArgs& r, int64_t
   if (r.topk_groups < groups) {
     taken = 0;
     float size;
-    const float score = group_scores<float, PER>(r, x, BIASED, lane, size);
+    const float score = group_scores<float, PER>(r, x, BIASED, lane, e0, own, size);
     uint32_t sk = lane < groups ? order_key(score) : 0u;
     uint32_t m = 0;
     for (int k = 0; k < r.topk_groups; ++k) {
@@ -471,12 +492,12 @@ __device__ __forceinline__ void route_token_grouped(const RouterArgs& r, int64_t
     const bool in = (taken >> (lane >> r.span_log2)) & 1u;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      key[i] = in && (whole || (i < per && e0 + i < E)) ? ((order_key(x[i]) & ~kPlace) | (kPlace - i)) : 0u;
+      key[i] = in && (whole || i < own) ? ((order_key(x[i]) & ~kPlace) | (kPlace - i)) : 0u;
   } else {
     int g = e0 / gs, left = (g + 1) * gs - e0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      key[i] = i < per && e0 + i < E && ((taken >> (g & 31)) & 1u) ? ((order_key(x[i]) & ~kPlace) | (kPlace - i)) : 0u;
+      key[i] = i < own && ((taken >> (g & 31)) & 1u) ? ((order_key(x[i]) & ~kPlace) | (kPlace - i)) : 0u;
       if (--left == 0) {
         ++g;
         left = gs;
@@ -520,7 +541,9 @@ __device__ __forceinline__ void route_token_grouped(const RouterArgs& r, int64_t
     const float next = __shfl_down_sync(0xffffffffu, v, 1);
     order = __any_sync(0xffffffffu, lane + 1 < n && !(v - next > kEps + kEpsRel * fabsf(v)));
   }
-  int my_id = my_src * per + (int)(kPlace - (my_key & kPlace));
+  int src_e0, src_n;
+  lane_experts(r, my_src, src_e0, src_n);
+  int my_id = src_e0 + (int)(kPlace - (my_key & kPlace));
   int place = lane;  // of this lane's expert in the output (topk and more: none)
   if (many) my_id = grouped_select_f64<PER>(r, t, taken, lane);  // warp-uniform
   else if (order) place = grouped_order_f64(r, t, my_id, n, lane);
@@ -560,18 +583,20 @@ __device__ __forceinline__ void route_token(const RouterArgs& r, int64_t t, int 
 // Values per lane for E experts (see route_token_warp).
 __host__ __device__ __forceinline__ int router_per_lane(int E) { return E <= 256 ? 8 : (E <= 512 ? 16 : 32); }
 
-// Consecutive experts a lane owns in group-limited routing: at least ceil(E / 32)
-// and at most router_per_lane(E), a group's size divided by a power of two if one
-// fits.
-inline int grouped_per_lane(int E, int groups) {
-  const int least = (E + 31) / 32;
-  int fit = 0;
-  for (int per = E / groups;; per /= 2) {
-    if (per < least) break;
-    if (per <= router_per_lane(E)) fit = per;
-    if (per % 2) break;
+// Values per lane in group-limited routing (r.per of them used).
+inline int grouped_per_lane(const RouterArgs& r) { return r.per <= 8 ? 8 : (r.per <= 16 ? 16 : 32); }
+
+// How the experts of r.groups groups are dealt to the lanes (lane_experts).
+inline void grouped_lanes(RouterArgs& r) {
+  r.gs = r.E / r.groups;
+  int log2 = 0;
+  while (r.groups << (log2 + 1) <= 32) ++log2;
+  r.span_log2 = log2;
+  r.per = (r.gs + (1 << log2) - 1) >> log2;
+  if (r.per > 32) {  // more than 512 experts in groups that are no power of two
+    r.span_log2 = -1;
+    r.per = (r.E + 31) / 32;
   }
-  return fit ? fit : least;
 }
 
 }  // namespace b200moe
