@@ -34,7 +34,9 @@ __device__ __forceinline__ void promote(float (&acc)[NC], uint32_t taddr, float 
 }
 
 // silu(gate) * up of a token's NC / 2 (gate, up) pairs into acc[0 .. NC/2 - 1];
-// returns their largest magnitude.
+// returns their largest magnitude. (A reciprocal shared by four values, for half the
+// load of the special-function unit, needs a branch for large gates and measured 4-12%
+// slower: 62 us to 70 for 5772 x 768 x 3584.)
 template <int NC>
 __device__ __forceinline__ float silu_pairs(float (&acc)[NC]) {
   float mx = 0.f;
@@ -93,45 +95,81 @@ __device__ __forceinline__ void dense_store4(const DenseParams& p, int64_t m, in
   }
 }
 
+// Element (row r, column c) of 32 rows x 64 fp32 columns in shared memory, 16-byte
+// pieces swizzled by row.
+__device__ __forceinline__ float* staged(uint8_t* st, int r, int c) {
+  return reinterpret_cast<float*>(st + r * 256 + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4);
+}
+
+// Columns n1 .. n1 + nc - 1 (nc <= 64) of staged rows m0 ..: whole aligned 16-byte
+// pieces, and the elements before and behind them one by one.
+template <bool F32>
+__device__ __forceinline__ void store_staged(const DenseParams& p, int m0, int n1, int nc, int rows, uint8_t* st,
+                                             int lane) {
+  constexpr int ES = F32 ? 4 : 2, EP = 16 / ES, L = 64 / EP;  // bytes; elements and lanes: of a piece, of a row
+  for (int r = lane / L; r < rows; r += 32 / L) {
+    uint8_t* row = static_cast<uint8_t*>(p.out) + ((int64_t)(m0 + r) * p.ld_out + n1) * ES;
+    const int ahead = (int)((0 - reinterpret_cast<uintptr_t>(row)) & 15) / ES;
+    const int lead = ahead < nc ? ahead : nc, pieces = (nc - lead) / EP, tail = lead + pieces * EP;
+    const int j = lane % L;
+    if (j < pieces) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = lead + j * EP + i * (EP / 4);
+        if (F32) {
+          w[i] = __float_as_uint(*staged(st, r, c));
+        } else {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(*staged(st, r, c), *staged(st, r, c + 1));
+          w[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+      }
+      *reinterpret_cast<uint4*>(row + (lead + j * EP) * ES) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    for (int e = j; e < lead + nc - tail; e += L) {
+      const int c = e < lead ? e : tail + e - lead;
+      if (F32) reinterpret_cast<float*>(row)[c] = *staged(st, r, c);
+      else reinterpret_cast<__nv_bfloat16*>(row)[c] = __float2bfloat16_rn(*staged(st, r, c));
+    }
+  }
+}
+
 // Stores 32 rows (m0.., one per lane) x NC columns (n0..) of fp32 results where rows
-// are not vector aligned (!p.vec). They pass through st (4 KB of this warp, rows of 32
-// columns, 16-byte pieces swizzled by row), so that a store instruction covers 32
-// consecutive columns of one row. The residuals of 8 rows are asked for together: a
-// load between stores, which may alias it, waits for the one before.
+// are not vector aligned (!p.vec), 64 columns at a time through st (8 KB of this
+// warp). The residuals of all of them are asked for together: a load between stores,
+// which may alias it, waits for the one before. (1349 x 1467 x 1024: 13.3 us, 15.6 with
+// 32 columns of a row to a store of 2 bytes a lane; 9.5 for 1464 columns.)
 template <int NC>
 __device__ __forceinline__ void dense_store_tile(const DenseParams& p, int m0, int n0, const float (&acc)[NC],
                                                  uint8_t* st, int lane) {
   const int rows = p.M - m0 < 32 ? p.M - m0 : 32;
 #pragma unroll
-  for (int cb = 0; cb < NC / 32; ++cb) {
-    const int n1 = n0 + cb * 32, n = n1 + lane;
-    if (n1 < p.N) {  // warp-uniform
+  for (int cb = 0; cb < NC / 64; ++cb) {
+    const int n1 = n0 + cb * 64, nc = p.N - n1 < 64 ? p.N - n1 : 64;
+    if (nc > 0) {  // warp-uniform
 #pragma unroll
-      for (int c = 0; c < 8; ++c)
-        *reinterpret_cast<float4*>(st + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-            make_float4(acc[cb * 32 + 4 * c], acc[cb * 32 + 4 * c + 1], acc[cb * 32 + 4 * c + 2],
-                        acc[cb * 32 + 4 * c + 3]);
+      for (int c = 0; c < 16; ++c)
+        *reinterpret_cast<float4*>(staged(st, lane, 4 * c)) =
+            make_float4(acc[cb * 64 + 4 * c], acc[cb * 64 + 4 * c + 1], acc[cb * 64 + 4 * c + 2],
+                        acc[cb * 64 + 4 * c + 3]);
       __syncwarp();
-      for (int r1 = 0; r1 < rows; r1 += 8) {
-        float res[8];
+      if (p.residual) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          res[i] = p.residual && n < p.N && r1 + i < rows
-                       ? __bfloat162float(
-                             static_cast<const __nv_bfloat16*>(p.residual)[(int64_t)(m0 + r1 + i) * p.ld_res + n])
-                       : 0.f;
+        for (int h = 0; h < 2; ++h) {
+          const int c = h * 32 + lane;
+          const __nv_bfloat16* src =
+              static_cast<const __nv_bfloat16*>(p.residual) + (int64_t)m0 * p.ld_res + n1 + c;
+          __nv_bfloat16 res[32];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = r1 + i;
-          if (n < p.N && r < rows) {
-            float v = *reinterpret_cast<const float*>(st + r * 128 + (((lane >> 2) ^ i) << 4) + (lane & 3) * 4);
-            if (p.residual) v += res[i];
-            const int64_t at = (int64_t)(m0 + r) * p.ld_out + n;
-            if (p.out_f32) static_cast<float*>(p.out)[at] = v;
-            else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-          }
+          for (int r = 0; r < 32; ++r) res[r] = c < nc && r < rows ? src[r * p.ld_res] : __nv_bfloat16();
+#pragma unroll
+          for (int r = 0; r < 32; ++r)
+            if (c < nc && r < rows) *staged(st, r, c) += __bfloat162float(res[r]);
         }
+        __syncwarp();
       }
+      if (p.out_f32) store_staged<true>(p, m0, n1, nc, rows, st, lane);
+      else store_staged<false>(p, m0, n1, nc, rows, st, lane);
       __syncwarp();
     }
   }
