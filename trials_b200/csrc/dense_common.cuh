@@ -51,16 +51,14 @@ __device__ __forceinline__ float silu_pairs(float (&acc)[NC]) {
 // acc[0 .. NC/2 - 1] quantised with `scale` to consecutive codes (16-byte aligned).
 template <int NC>
 __device__ __forceinline__ void store_codes(const float (&acc)[NC], float scale, uint8_t* q) {
-  const float rcp = __frcp_rn(scale);
+  const CodeScale cs = code_scale(scale);
 #pragma unroll
   for (int k = 0; k < NC / 32; ++k) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = 0;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        w[i] |= quant_e4m3x2_by(acc[k * 16 + i * 4 + 2 * t], acc[k * 16 + i * 4 + 2 * t + 1], scale, rcp) << (16 * t);
+      const float* v = acc + k * 16 + i * 4;
+      w[i] = quant_e4m3x4<true>(v[0], v[1], v[2], v[3], cs);
     }
     reinterpret_cast<uint4*>(q)[k] = make_uint4(w[0], w[1], w[2], w[3]);
   }
@@ -269,13 +267,13 @@ __device__ __forceinline__ void finish_tokens_of(const DenseParams& p, int64_t m
         float mx = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float scale = group_scale(mx), rcp = __frcp_rn(scale);
+        const float scale = group_scale(mx);
+        const CodeScale cs = code_scale(scale);
         const int unit = n0 >> 8;
         uint8_t* dst = p.q + m * p.ld_q + unit * 128 + lane * 2;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<uint16_t*>(dst + h * 64) =
-              (uint16_t)quant_e4m3x2_by(y[2 * h], y[2 * h + 1], scale, rcp);
+          *reinterpret_cast<uint16_t*>(dst + h * 64) = quant_e4m3x2(y[2 * h], y[2 * h + 1], cs);
         if (lane == 0) p.s[m * p.ld_s + unit] = scale;
       } else {
 #pragma unroll

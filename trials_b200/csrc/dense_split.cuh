@@ -241,10 +241,11 @@ __global__ void __launch_bounds__(DenseSplitCfg<T>::THREADS, 2)
         }
 #pragma unroll
         for (int o = 8; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float scale = group_scale(mx), rcp = __frcp_rn(scale);
-        uint32_t w[2] = {0, 0};
+        const float scale = group_scale(mx);
+        const CodeScale cs = code_scale(scale);
+        uint32_t w[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i >> 1] |= quant_e4m3x2_by(v[2 * i], v[2 * i + 1], scale, rcp) << (16 * (i & 1));
+        for (int i = 0; i < 2; ++i) w[i] = quant_e4m3x4<true>(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], cs);
         if (g < total) {
           *reinterpret_cast<uint2*>(xq + kb * tt * 128 + t * 128 + (((sub >> 1) ^ (t & 7)) << 4) + (sub & 1) * 8) =
               make_uint2(w[0], w[1]);

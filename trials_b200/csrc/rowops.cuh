@@ -76,23 +76,11 @@ __device__ __forceinline__ void quant_row_segment(const QuantArgs& a, int64_t ro
     return;
   }
   const __nv_bfloat16* xr = reinterpret_cast<const __nv_bfloat16*>(a.x) + src * a.ldx;
-  float v[kQuantSegSteps][8];
+  uint4 raw[kQuantSegSteps];
 #pragma unroll
   for (int i = 0; i < kQuantSegSteps; ++i) {
     const int64_t c = seg0 + i * 256 + lane * 8;
-    if (c < seg_end) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(xr + c));
-      const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f2 = __bfloat1622float2(h2[j]);
-        v[i][2 * j] = f2.x;
-        v[i][2 * j + 1] = f2.y;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    }
+    raw[i] = c < seg_end ? __ldg(reinterpret_cast<const uint4*>(xr + c)) : make_uint4(0, 0, 0, 0);
   }
   uint2 packed[kQuantSegSteps];
   float scl[kQuantSegSteps];
@@ -101,19 +89,35 @@ __device__ __forceinline__ void quant_row_segment(const QuantArgs& a, int64_t ro
     packed[i] = make_uint2(0, 0);
     scl[i] = 0.f;
     if (seg0 + i * 256 >= seg_end) continue;  // warp-uniform
-    float m = 0.f;
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    // Magnitudes of bf16 compare as integers, two at a time; NaN above infinity.
+    uint32_t mm = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                           __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[i][j]));
+    for (int o = 8; o >= 1; o >>= 1) mm = __vmaxu2(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    mm = mm >> 16 > (mm & 0xffffu) ? mm & 0xffff0000u : mm << 16;
+    float v[8];
 #pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    uint32_t lo = 0, hi = 0;
-    const float scale = group_scale(m), rcp = __frcp_rn(scale);
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(w[j] << 16);
+      v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+    if (__any_sync(0xffffffffu, mm >= 0x7f800000u)) {
+      // Infinities or NaN: the largest number counts, NaN becomes -448.
+      float m = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) lo |= quant_e4m3x2_by(v[i][2 * j], v[i][2 * j + 1], scale, rcp) << (16 * j);
+      for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
 #pragma unroll
-    for (int j = 0; j < 2; ++j) hi |= quant_e4m3x2_by(v[i][4 + 2 * j], v[i][5 + 2 * j], scale, rcp) << (16 * j);
-    packed[i] = make_uint2(lo, hi);
-    scl[i] = scale;
+      for (int o = 8; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      scl[i] = group_scale(m);
+      const CodeScale cs = code_scale(scl[i]);
+      packed[i] = make_uint2(quant_e4m3x4<true>(v[0], v[1], v[2], v[3], cs), quant_e4m3x4<true>(v[4], v[5], v[6], v[7], cs));
+    } else {
+      scl[i] = group_scale(__uint_as_float(mm));
+      const CodeScale cs = code_scale(scl[i]);
+      packed[i] =
+          make_uint2(quant_e4m3x4<false>(v[0], v[1], v[2], v[3], cs), quant_e4m3x4<false>(v[4], v[5], v[6], v[7], cs));
+    }
   }
   auto put = [&](int64_t d) {
     uint8_t* qr = a.q + d * a.ldq;
