@@ -215,9 +215,10 @@ DensePlan split_plan(int epi, int64_t M, int64_t N, int nkb, bool x_bf16) {
   const int T = tt <= 16 ? 16 : (tt <= 32 ? 32 : 64);
   const int64_t units = (N + 128 * halves - 1) / (128 * halves) * n_tt;
   const int sms = sm_count_of(current_device());
-  // CTAs along K, at least two K blocks each.
+  // CTAs along K, at least two K blocks each, four where 8 CTAs would exchange the sums of
+  // more than 32 tokens (64 of 2304 x 2048: 6.4 us with 4 CTAs, 7.7 with 8).
   int s = 8 / halves;
-  while (s > 1 && s * 2 > nkb) s /= 2;
+  while (s > 1 && s * (T == 64 && M <= 64 && s == 8 ? 4 : 2) > nkb) s /= 2;
   if (M > 64) {
     // More than 64 tokens read the weights more than once, which pays while the tiles'
     // clusters run in one wave, two CTAs an SM less what clusters cannot use (gate/up of
@@ -228,10 +229,18 @@ DensePlan split_plan(int epi, int64_t M, int64_t N, int nkb, bool x_bf16) {
     const int64_t most = epi == DENSE_SILU || s <= 2 ? (int64_t)sms * 7 / 4 : sms;
     if (units * halves * s > most) return pl;
   } else {
-    // Up to 4/3 of the SMs measured best: one token of 6144 x 2048 (48 tiles) takes 6.2
-    // us with 4 CTAs along K, 6.8 with 2 and, in two waves, 10.8 with 6; 4096 x 6144 (32
-    // tiles) 8.9 with 4 and 9.0 with 8, 64 tokens of it 11.4 and 11.9.
-    while (s > 1 && units * halves * s > (int64_t)sms * 4 / 3) s /= 2;
+    // Two CTAs an SM where that leaves more than 8 K blocks to each (one token of 8192 x
+    // 8192 14.6 us, 16.4 with half of them; 64 tokens of 7168 x 18432 28.8 and 38.4), else
+    // up to 4/3 of the SMs: one token of 6144 x 2048 (48 tiles) takes 6.2 us with 4 CTAs
+    // along K, 6.8 with 2 and, in two waves, 10.8 with 6; 64 tokens of 4096 x 6144 (32
+    // tiles) 10.8 with 4, 11.5 with 8. One an SM where more than 32 tokens would leave
+    // fewer than 8 K blocks (64 of 6144 x 2048: 8.1 with 2, 9.2 with 4).
+    auto fits = [&](int k) {
+      const int64_t ctas = units * halves * k;
+      if (nkb > 8 * k) return ctas <= (int64_t)sms * 2;
+      return ctas <= (T == 64 && nkb < 8 * k ? sms : (int64_t)sms * 4 / 3);
+    };
+    while (s > 1 && !fits(s)) s /= 2;
   }
   const int per = (nkb + s - 1) / s;
   // A token or two: a CTA can quantise its own K blocks of bf16 rows.
