@@ -64,10 +64,10 @@ __device__ __forceinline__ void store_codes(const float (&acc)[NC], float scale,
   }
 }
 
-// The residual of four consecutive outputs n.. of token m, where rows are vector
-// aligned (p.vec); zero bits otherwise.
+// The residual (four bf16) of four consecutive outputs n.. of token m, where rows are
+// vector aligned (p.vec).
 __device__ __forceinline__ uint2 dense_residual4(const DenseParams& p, int64_t m, int n) {
-  if (!p.vec || !p.residual || n >= p.N) return make_uint2(0, 0);
+  if (!p.residual || n >= p.N) return make_uint2(0, 0);
   return *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.residual) + m * p.ld_res + n);
 }
 
@@ -196,14 +196,24 @@ __device__ __forceinline__ float4 spread_cols(float4 v, int lane) {
 }
 
 // Rows that are not vector aligned: outputs n, n + 32, n + 64, n + 96 of token m,
-// so that a store instruction of the warp covers 32 consecutive ones.
-__device__ __forceinline__ void dense_store_cols(const DenseParams& p, int64_t m, int n, float4 v) {
+// so that a store instruction of the warp covers 32 consecutive ones, and the
+// residual of them (four bf16).
+__device__ __forceinline__ uint2 dense_residual_cols(const DenseParams& p, int64_t m, int n) {
+  if (!p.residual) return make_uint2(0, 0);
+  const uint16_t* src = static_cast<const uint16_t*>(p.residual) + m * p.ld_res + n;
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = n + 32 * i < p.N ? src[32 * i] : 0;
+  return make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
+}
+__device__ __forceinline__ void dense_store_cols(const DenseParams& p, int64_t m, int n, float4 v, uint2 res) {
   const float a[4] = {v.x, v.y, v.z, v.w};
+  const uint32_t r[4] = {res.x << 16, res.x & 0xffff0000u, res.y << 16, res.y & 0xffff0000u};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (n + 32 * i < p.N) {
       float y = a[i];
-      if (p.residual) y += __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[m * p.ld_res + n + 32 * i]);
+      if (p.residual) y += __uint_as_float(r[i]);
       if (p.out_f32) static_cast<float*>(p.out)[m * p.ld_out + n + 32 * i] = y;
       else static_cast<__nv_bfloat16*>(p.out)[m * p.ld_out + n + 32 * i] = __float2bfloat16_rn(y);
     }
@@ -233,7 +243,9 @@ __device__ __forceinline__ void finish_tokens_of(const DenseParams& p, int64_t m
 #pragma unroll
           for (int s = 0; s < MAXS; ++s)
             if (s < splits) v[b][h][s] = ld_cluster_f4(at(t, s, h));
-          if (EPI == DENSE_OUT) res[b][h] = dense_residual4(p, m0 + t, n0 + 128 * h + lane * 4);
+          if (EPI == DENSE_OUT)
+            res[b][h] = p.vec ? dense_residual4(p, m0 + t, n0 + 128 * h + lane * 4)
+                              : dense_residual_cols(p, m0 + t, n0 + 128 * h + lane);
         }
       }
     }
@@ -279,7 +291,7 @@ __device__ __forceinline__ void finish_tokens_of(const DenseParams& p, int64_t m
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
           if (p.vec) dense_store4(p, m, n0 + 128 * h + lane * 4, sum[h], res[b][h]);
-          else dense_store_cols(p, m, n0 + 128 * h + lane, spread_cols(sum[h], lane));
+          else dense_store_cols(p, m, n0 + 128 * h + lane, spread_cols(sum[h], lane), res[b][h]);
         }
       }
     }
