@@ -222,11 +222,14 @@ DensePlan split_plan(int epi, int64_t M, int64_t N, int nkb, bool x_bf16) {
   if (M > 64) {
     // More than 64 tokens read the weights more than once, which pays while the tiles'
     // clusters run in one wave, two CTAs an SM less what clusters cannot use (gate/up of
-    // 200 x 2048 x 256 5.9 us, token-major 8.7; 1500 x 1024 x 256 6.2 and 7.8). With long
-    // K and DENSE_OUT the token-major tiles of 128 columns are the better ones as soon as
-    // two CTAs share an SM (200 x 576 x 7168, 160 CTAs: 10.0 and 8.5; 300 x 100 x 6144,
-    // 40 CTAs: 6.7 and 7.5; 500 x 1000 x 1024, 256 CTAs: 7.2 and 6.6).
-    const int64_t most = epi == DENSE_SILU || s <= 2 ? (int64_t)sms * 7 / 4 : sms;
+    // 200 x 2048 x 256 5.9 us, token-major 8.7; 1500 x 1024 x 256 6.2 and 7.8), with one
+    // CTA an SM where K is long: token-major clusters then wait less for their operands
+    // (gate/up of 128 x 6144 x 2048, 256 CTAs of 12 K blocks: 14.7 and 13.9; 128 x 4096 x
+    // 2048, of 8: 12.3 and 12.9), with DENSE_OUT, whose tiles of 128 columns exchange
+    // little, from 4 CTAs along K on (500 x 1000 x 1024, 256 CTAs: 7.2 and 6.6; 200 x 576
+    // x 7168, 160: 10.0 and 8.5; 300 x 100 x 6144, 40: 6.7 and 7.5).
+    const bool two_an_sm = epi == DENSE_SILU ? nkb <= 8 * s : s <= 2;
+    const int64_t most = two_an_sm ? (int64_t)sms * 7 / 4 : sms;
     if (units * halves * s > most) return pl;
   } else {
     // Two CTAs an SM where that leaves more than 8 K blocks to each (one token of 8192 x
