@@ -129,6 +129,12 @@ def test_refusals_on_device(cuda_device):
             moe.select_experts(x, 4, "sigmoid", **kw)
     with pytest.raises(ValueError):  # a bias that does not cover the experts
         moe.select_experts(x, 4, "sigmoid", torch.zeros(32, device=cuda_device), num_expert_group=8, topk_group=2)
+    with pytest.raises(ValueError):
+        stages.route_logits(x, 4, 32, correction_bias=torch.zeros(32, device=cuda_device), num_expert_group=8,
+                            topk_group=2)
+    with pytest.raises(ValueError):
+        stages.LayerPipeline(8, 256, 128, 64, 4, device=cuda_device,
+                             router={"correction_bias": torch.zeros(32), "num_expert_group": 8, "topk_group": 2})
     with pytest.raises(NotImplementedError):
         moe.select_experts(x.half(), 4, "sigmoid", num_expert_group=8, topk_group=2)
 

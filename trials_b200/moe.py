@@ -137,8 +137,10 @@ def _check_groups(num_expert_group: Optional[int], topk_group: Optional[int]) ->
     return num_expert_group is not None
 
 
-def _router_bias(bias: Optional[torch.Tensor], dev: torch.device, index: int, E: int) -> Optional[torch.Tensor]:
-    """The correction bias as the kernels read it: E contiguous f32 on the device."""
+def _router_bias(bias: Optional[torch.Tensor], dev: torch.device, index: Optional[int],
+                 E: int) -> Optional[torch.Tensor]:
+    """The correction bias as the kernels read it: E contiguous f32 on the device
+    (index: the device's, None if unknown)."""
     if bias is None:
         return None
     if bias.numel() != E:

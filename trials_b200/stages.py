@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .moe import FP8, _check_groups, _ptr, _require_cuda, _stream
+from .moe import FP8, _check_groups, _ptr, _require_cuda, _router_bias, _stream
 
 
 @dataclass
@@ -106,7 +106,7 @@ def route_logits(logits: torch.Tensor, top_k: int, tile_tokens: int, scoring_fun
         expert_map = expert_map.to(device=dev, dtype=torch.int32).contiguous()
     ns = L.b200moe_route_logits_scratch_ints(numel, E)
     scratch = torch.zeros(ns, dtype=torch.int32, device=dev)
-    bias = None if correction_bias is None else correction_bias.to(device=dev, dtype=torch.float32).contiguous()
+    bias = _router_bias(correction_bias, dev, logits.get_device(), E_router)
     scoring = {"softmax": 0, "sigmoid": 1}[scoring_func]
     head = (_ptr(logits), int(logits.dtype == torch.bfloat16), M, E_router)
     tail = (top_k, scoring, _ptr(bias), int(renormalize), float(routed_scaling_factor), _ptr(tw), _ptr(ids),
@@ -369,9 +369,8 @@ class LayerPipeline:
         self.router = None
         if router is not None:
             r = dict(router)
-            bias = r.get("correction_bias")
             self.router = (({"softmax": 0, "sigmoid": 1}[r.get("scoring_func", "sigmoid")]),
-                           None if bias is None else bias.to(device=device, dtype=torch.float32).contiguous(),
+                           _router_bias(r.get("correction_bias"), device, None, num_experts),
                            int(r.get("renormalize", True)), float(r.get("routed_scaling_factor", 1.0)))
             self.groups = (r.get("num_expert_group"), r.get("topk_group"))
             if not _check_groups(*self.groups):
