@@ -53,6 +53,8 @@ SHAPES = [(1, 128, 128), (1, 4096, 1024), (2, 6144, 2048), (3, 256, 6144), (11, 
           (255, 64, 128), (300, 1280, 768), (512, 640, 1024), (1000, 384, 512), (2100, 520, 384), (5000, 130, 256),
           # 128-column tiles: split, one each over two rounds, and pairs past that
           (300, 1000, 1152), (777, 77, 768), (20000, 24, 256), (40000, 128, 128),
+          # rows quantised in the product, as many as there may be
+          (4, 4096, 6144), (12, 5000, 1024),
           # pairs: whole and partial boxes of the output
           (5000, 328, 256), (4100, 776, 512), (9000, 256, 1024)]
 

@@ -246,7 +246,7 @@ DensePlan split_plan(int epi, int64_t M, int64_t N, int nkb, bool x_bf16) {
     while (s > 1 && !fits(s)) s /= 2;
   }
   const int per = (nkb + s - 1) / s;
-  // A token or two: a CTA can quantise its own K blocks of bf16 rows.
+  // A few tokens: a CTA can quantise its own K blocks of bf16 rows.
   const bool qx = x_bf16 && T == 16 && M * per <= kQuantGroups && split_stages<16>(per, tt, true) > 0;
   const int stages = qx ? 1
                         : (T == 16 ? split_stages<16>(per, tt, false)

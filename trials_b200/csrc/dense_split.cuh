@@ -30,9 +30,11 @@
 
 namespace b200moe {
 
-// Most (token, K block) groups a CTA quantises itself (QX): from about there on
-// the launch that quantises every row once is cheaper.
-constexpr int kQuantGroups = 32;
+// Most (token, K block) groups a CTA quantises itself (QX). Up to 24 it is faster than
+// the launch that quantises every row once (one token of 6144 x 2048 6.5 us, 8.0); at 48
+// (4 of 4096 x 6144) 11.4 us on the GPU against 10.8 but 12.1 a call against 15.7, at 64
+// (16 of 6144 x 2048) 9.8 against 8.4.
+constexpr int kQuantGroups = 48;
 
 template <int T_>
 struct DenseSplitCfg {
