@@ -14,6 +14,7 @@ the current torch stream of its tensors' device; there is no fallback path.
 """
 from __future__ import annotations
 
+import functools
 import struct
 from typing import Optional
 
@@ -26,6 +27,7 @@ from .moe import FP8, _require_cuda, _stream, _workspaces
 # below read each attribute once and build no intermediate objects, and the C
 # entries get their arguments packed as one struct of 8-byte members (0 = NULL).
 _PACK = {n: struct.Struct(f"{n}q").pack for n in (19, 20)}
+_F32, _BF16 = torch.float32, torch.bfloat16
 
 
 def _device_of(x: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
@@ -55,6 +57,8 @@ def _call(fn, where: str, index: int, *args: int) -> None:
 
 def _rows(t: torch.Tensor, what: str) -> int:
     """Row stride in elements of a 2-D tensor whose rows are contiguous."""
+    if t.is_contiguous():
+        return t.shape[1]
     s0, s1 = t.stride()
     n, m = t.shape
     if m > 1 and s1 != 1:
@@ -67,17 +71,19 @@ def _rows(t: torch.Tensor, what: str) -> int:
 
 
 def _input(x: torch.Tensor, x_scale: Optional[torch.Tensor]):
-    """Checked activation rows and scales and their row strides, copied only where
-    their layout asks for it: (x, x_scale, stride of x, stride of x_scale)."""
-    if x.dim() != 2:
+    """Checked activation rows and scales, copied only where their layout asks for
+    it: (x, x_scale, M, K, stride of x, stride of x_scale)."""
+    shape = x.shape
+    if len(shape) != 2:
         raise ValueError("x must be (M, K)")
-    M, K = x.shape
+    M, K = shape
+    dtype = x.dtype
     ld_s = 0
-    if x.dtype == FP8:
-        size = 1
+    if dtype is FP8:
+        align = 16
         if x_scale is None or x_scale.shape != (M, K // 128):
             raise ValueError("fp8 x needs x_scale of shape (M, K/128) (1x128 per-token-group scales)")
-        if x_scale.dtype != torch.float32:
+        if x_scale.dtype is not _F32:
             raise NotImplementedError("x_scale must be float32")
         ld_s, s1 = x_scale.stride()
         if s1 != 1 or (M > 1 and ld_s < K // 128):
@@ -85,8 +91,8 @@ def _input(x: torch.Tensor, x_scale: Optional[torch.Tensor]):
             ld_s = K // 128
         elif M <= 1:
             ld_s = K // 128
-    elif x.dtype == torch.bfloat16:
-        size = 2
+    elif dtype is _BF16:
+        align = 8
         if x_scale is not None:
             raise ValueError("x_scale is only meaningful with fp8 x")
     else:
@@ -96,42 +102,60 @@ def _input(x: torch.Tensor, x_scale: Optional[torch.Tensor]):
     s0, s1 = x.stride()
     if M <= 1:
         s0 = K
-    if s1 != 1 or s0 < K or s0 * size % 16 or x.data_ptr() % 16:
+    if s1 != 1 or s0 < K or s0 % align or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
         s0 = K
-    return x, x_scale, s0, ld_s
+    return x, x_scale, M, K, s0, ld_s
 
 
 def _weight(w: torch.Tensor, scale: torch.Tensor, K: int, what: str):
-    """(row stride of the weight, contiguous scales), checked."""
-    if w.dtype != FP8:
+    """(row stride of the weight, contiguous scales, rows), checked."""
+    if w.dtype is not FP8:
         raise NotImplementedError(f"{what} must be float8_e4m3fn with 128x128 block scales")
-    if w.dim() != 2 or w.shape[1] != K or w.shape[0] == 0:
-        raise ValueError(f"{what} must be (N, {K}), got {tuple(w.shape)}")
-    if scale.dtype != torch.float32:
+    shape = w.shape
+    if len(shape) != 2 or shape[1] != K or shape[0] == 0:
+        raise ValueError(f"{what} must be (N, {K}), got {tuple(shape)}")
+    N = shape[0]
+    if scale.dtype is not _F32:
         raise NotImplementedError(f"{what}_scale must be float32")
-    if scale.shape != ((w.shape[0] + 127) // 128, K // 128):
+    if scale.shape != ((N + 127) >> 7, K >> 7):
         raise ValueError(f"{what}_scale must be (ceil(N/128), K/128), got {tuple(scale.shape)}")
-    return _rows(w, what), scale if scale.is_contiguous() else scale.contiguous()
+    if w.is_contiguous():
+        ld = K
+    else:
+        ld = _rows(w, what)
+    return ld, scale if scale.is_contiguous() else scale.contiguous(), N
 
 
 def _output(out: Optional[torch.Tensor], residual: Optional[torch.Tensor], M: int, N: int, dtype: torch.dtype,
             dev: torch.device):
     """(out, its row stride, the residual's row stride), checked."""
     if out is None:
-        out = torch.empty(M, N, dtype=dtype, device=dev)
+        out = torch.empty((M, N), dtype=dtype, device=dev)
         ld = N
     else:
-        if out.shape != (M, N) or out.dtype != dtype:
+        if out.shape != (M, N) or out.dtype is not dtype:
             raise ValueError(f"out must be ({M}, {N}) {dtype}")
         ld = _rows(out, "out")
     if residual is None:
         return out, ld, 0
-    if residual.dtype != torch.bfloat16:
+    if residual.dtype is not _BF16:
         raise NotImplementedError("residual must be bf16")
     if residual.shape != (M, N):
         raise ValueError(f"residual must be ({M}, {N})")
     return out, ld, _rows(residual, "residual")
+
+
+# Sizes of workspaces by sizes of the call (and its device): asking the library each
+# time is a tenth of a one-token call.
+@functools.lru_cache(maxsize=4096)
+def _linear_bytes(index: int, M: int, N: int, K: int, gate_up: int) -> int:
+    return _lib.lib().b200moe_linear_workspace_size(M, N, K, 1, gate_up)
+
+
+@functools.lru_cache(maxsize=4096)
+def _mlp_bytes(index: int, M: int, H: int, I: int, bf16: bool) -> int:
+    return _lib.lib().b200moe_mlp_workspace_size(M, H, I, bf16)
 
 
 def _workspace(nbytes: int, dev: torch.device):
@@ -140,7 +164,7 @@ def _workspace(nbytes: int, dev: torch.device):
     graphs have theirs."""
     if nbytes == 0:
         return None, 0, 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
     return ws, ws.data_ptr(), nbytes
 
 
@@ -154,19 +178,17 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     N; K % 128 == 0. out may be residual itself and overlaps no other input. See
     b200moe_linear."""
     index = _device_of(x, weight, weight_scale, x_scale, residual, out)
-    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
+    if out_dtype is not _BF16 and out_dtype is not _F32:
         raise NotImplementedError("out_dtype must be bf16 or float32")
-    x, x_scale, ld_x, ld_s = _input(x, x_scale)
-    M, K = x.shape
-    N = weight.shape[0]
+    x, x_scale, M, K, ld_x, ld_s = _input(x, x_scale)
     dev = x.device
-    ld_w, weight_scale = _weight(weight, weight_scale, K, "weight")
+    ld_w, weight_scale, N = _weight(weight, weight_scale, K, "weight")
     out, ld_out, ld_res = _output(out, residual, M, N, out_dtype, dev)
     if M == 0:
         return out
     L = _lib.lib()
     if x_scale is None:
-        ws, ws_ptr, ws_bytes = _workspace(L.b200moe_linear_workspace_size(M, N, K, 1, 0), dev)
+        ws, ws_ptr, ws_bytes = _workspace(_linear_bytes(index, M, N, K, 0), dev)
         rows = (x.data_ptr(), 0, 0)
     else:
         ws_ptr, ws_bytes = 0, 0
@@ -174,7 +196,7 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     _call(L.b200moe_linear, "fp8_block_linear", index,
           *rows, ld_x, ld_s, M, N, K, weight.data_ptr(), ld_w, weight_scale.data_ptr(),
           0 if residual is None else residual.data_ptr(), ld_res, out.data_ptr(), ld_out,
-          out_dtype is torch.float32, ws_ptr, ws_bytes)
+          out_dtype is _F32, ws_ptr, ws_bytes)
     return out
 
 
@@ -184,20 +206,19 @@ def fp8_gate_up(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, x_s
     up j). x as in fp8_block_linear; w13 (2I, H) fp8 e4m3, w13_scale (2I/128,
     H/128) f32; I % 128 == 0. See b200moe_gate_up."""
     index = _device_of(x, w13, w13_scale, x_scale)
-    x, x_scale, ld_x, ld_s = _input(x, x_scale)
-    M, H = x.shape
+    x, x_scale, M, H, ld_x, ld_s = _input(x, x_scale)
     dev = x.device
-    ld_w, w13_scale = _weight(w13, w13_scale, H, "w13")
-    if w13.shape[0] % 256:
+    ld_w, w13_scale, N = _weight(w13, w13_scale, H, "w13")
+    if N % 256:
         raise NotImplementedError("w13 must have 2I rows with I a multiple of 128")
-    I = w13.shape[0] // 2
-    q = torch.empty(M, I, dtype=FP8, device=dev)
-    s = torch.empty(M, I // 128, dtype=torch.float32, device=dev)
+    I = N // 2
+    q = torch.empty((M, I), dtype=FP8, device=dev)
+    s = torch.empty((M, I // 128), dtype=_F32, device=dev)
     if M == 0:
         return q, s
     L = _lib.lib()
     if x_scale is None:
-        ws, ws_ptr, ws_bytes = _workspace(L.b200moe_linear_workspace_size(M, 2 * I, H, 1, 1), dev)
+        ws, ws_ptr, ws_bytes = _workspace(_linear_bytes(index, M, 2 * I, H, 1), dev)
         rows = (x.data_ptr(), 0, 0)
     else:
         ws_ptr, ws_bytes = 0, 0
@@ -215,23 +236,22 @@ def fp8_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
     (2I, H), then fp8_block_linear with w2 (H, I), in one call (same bits).
     out may be residual or x itself. See b200moe_mlp."""
     index = _device_of(x, w13, w13_scale, w2, w2_scale, x_scale, residual, out)
-    x, x_scale, ld_x, ld_s = _input(x, x_scale)
-    M, H = x.shape
+    x, x_scale, M, H, ld_x, ld_s = _input(x, x_scale)
     dev = x.device
-    ld13, w13_scale = _weight(w13, w13_scale, H, "w13")
-    if w13.shape[0] % 256:
+    ld13, w13_scale, N = _weight(w13, w13_scale, H, "w13")
+    if N % 256:
         raise NotImplementedError("w13 must have 2I rows with I a multiple of 128")
-    I = w13.shape[0] // 2
-    ld2, w2_scale = _weight(w2, w2_scale, I, "w2")
-    if w2.shape[0] != H:
+    I = N // 2
+    ld2, w2_scale, rows2 = _weight(w2, w2_scale, I, "w2")
+    if rows2 != H:
         raise ValueError(f"w2 must be ({H}, {I}), got {tuple(w2.shape)}")
     if ld13 != H or ld2 != I:
         raise ValueError("w13 and w2 must be contiguous")
-    out, ld_out, ld_res = _output(out, residual, M, H, torch.bfloat16, dev)
+    out, ld_out, ld_res = _output(out, residual, M, H, _BF16, dev)
     if M == 0:
         return out
     L = _lib.lib()
-    ws, ws_ptr, ws_bytes = _workspace(L.b200moe_mlp_workspace_size(M, H, I, x_scale is None), dev)
+    ws, ws_ptr, ws_bytes = _workspace(_mlp_bytes(index, M, H, I, x_scale is None), dev)
     rows = (x.data_ptr(), 0, 0) if x_scale is None else (0, x.data_ptr(), x_scale.data_ptr())
     _call(L.b200moe_mlp, "fp8_mlp", index,
           *rows, ld_x, ld_s, M, H, I, w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(),
