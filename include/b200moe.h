@@ -597,7 +597,7 @@ B200MOE_API int b200moe_combine_reduce(const void* out_pair, const int32_t* slot
  * to add to; out may also be x. Weights contiguous; workspace b200moe_mlp_workspace_size() bytes,
  * 256-byte aligned.
  *
- * The calls take their twenty arguments in a struct whose members are all 8 bytes
+ * The calls take their arguments in a struct whose members are all 8 bytes
  * wide (set every one; a foreign-function interface fills it in one step). A
  * pipeline wait that gives up sets B200MOE_DEVERR_TIMEOUT in err_word (required)
  * and leaves the outputs undefined.
