@@ -31,7 +31,9 @@ int sm_count_of(int dev) {
   return n;
 }
 
-// Raises the kernel's shared memory limit once per device.
+// Raises the kernel's shared memory limit once per device, to a size that is the same in
+// every call of a kernel: a limit that went by the call could be lowered again by another
+// host thread between here and the launch.
 template <typename K>
 cudaError_t allow_smem(K kernel, int bytes, int dev, std::atomic<int> (&done)[kMaxDevices]) {
   if (dev >= 0 && dev < kMaxDevices && done[dev].load() >= bytes) return cudaSuccess;
@@ -119,7 +121,7 @@ cudaError_t launch_split_dense(const DensePlan& pl, const CUtensorMap& tm_x, con
   if (nstage == 0) return cudaErrorInvalidValue;
   int smem = C::smem_bytes(nstage, nkb, pl.tokens, QX);
   if (smem < kSplitSmemMin) smem = kSplitSmemMin;
-  cudaError_t err = allow_smem(kernel, smem, current_device(), done);
+  cudaError_t err = allow_smem(kernel, kSplitSmem, current_device(), done);
   if (err != cudaSuccess) return err;
   const int R = HALVES * pl.splits;
   cudaLaunchConfig_t cfg;
