@@ -64,3 +64,60 @@ def run(script):
 
 def test_first_products_of_several_threads(cuda_device):
     run(DENSE)
+
+
+ROUTING = """
+import threading
+import torch
+from trials_b200 import stages
+
+dev = torch.device("cuda", 0)
+calls = []
+for E in (16, 64, 256, 512, 1024):
+    for M in (4, 4096):            # one CTA, and several
+        calls.append((torch.randn(M, E, device=dev), dict(num_expert_group=8, topk_group=4)))
+        calls.append((calls[-1][0], {}))
+torch.cuda.synchronize()
+
+
+def call(x, groups):
+    r, w, ids = stages.route_logits(x, 8, 32, "sigmoid", **groups)
+    return r.sorted_ids, r.slot_pos, w, ids, stages.route(ids, x.shape[1], 32).slot_pos
+
+
+threads = 10
+gate = threading.Barrier(threads)
+got, failed = [None] * threads, []
+
+
+def work(k):
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            mine = list(range(len(calls)))
+            mine = mine[2 * k:] + mine[:2 * k]
+            gate.wait()
+            for _ in range(20):
+                out = {i: call(*calls[i]) for i in mine}
+            torch.cuda.current_stream().synchronize()
+        got[k] = out
+    except Exception as e:
+        failed.append(e)
+
+
+all_ = [threading.Thread(target=work, args=(k,)) for k in range(threads)]
+for t in all_:
+    t.start()
+for t in all_:
+    t.join()
+assert not failed, failed
+for i, c in enumerate(calls):
+    want = call(*c)
+    for k in range(threads):
+        for a, b in zip(got[k][i], want):
+            assert torch.equal(a, b)
+print("fine")
+"""
+
+
+def test_routing_of_several_threads(cuda_device):
+    run(ROUTING)

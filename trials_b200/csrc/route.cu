@@ -76,9 +76,18 @@ __global__ void __launch_bounds__(kRouteThreads, 1) unpack_align_kernel(const Al
 
 size_t align_smem_bytes(int E) { return (size_t)align_smem_ints(E, kRouteWarps) * sizeof(int32_t); }
 
+// Raises a kernel's shared memory limit to what the most experts need, whatever this call
+// needs: a limit that went by the call could be lowered again by another host thread
+// between here and the launch.
+constexpr int kRouteMaxExperts = 1024;
+template <typename K>
+static cudaError_t allow_smem(K kernel, size_t most) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+}
+
 cudaError_t launch_align_packed(const AlignArgs& a, const PackedMeta& pm, cudaStream_t stream) {
   const size_t smem = align_smem_bytes(a.E);
-  cudaError_t err = cudaFuncSetAttribute(unpack_align_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t err = allow_smem(unpack_align_kernel, align_smem_bytes(kRouteMaxExperts));
   if (err != cudaSuccess) return err;
   unpack_align_kernel<<<1, kRouteThreads, smem, stream>>>(a, pm);
   return cudaGetLastError();
@@ -86,7 +95,7 @@ cudaError_t launch_align_packed(const AlignArgs& a, const PackedMeta& pm, cudaSt
 
 cudaError_t launch_align(const AlignArgs& a, cudaStream_t stream) {
   const size_t smem = align_smem_bytes(a.E);
-  cudaError_t err = cudaFuncSetAttribute(align_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t err = allow_smem(align_kernel, align_smem_bytes(kRouteMaxExperts));
   if (err != cudaSuccess) return err;
   align_kernel<<<1, kRouteThreads, smem, stream>>>(a);
   return cudaGetLastError();
@@ -337,12 +346,11 @@ namespace {
 template <bool ROUTER, int PER, bool GROUPED = false>
 cudaError_t launch_route_multi(const AlignArgs& a, const RouterArgs& r, int C, int32_t* scratch,
                                cudaStream_t stream) {
-  const size_t smem1 = (size_t)kRouteWarps * a.E * sizeof(int32_t);
-  const size_t smem2 = (size_t)(kRouteWarps * a.E + 5 * a.E + 2) * sizeof(int32_t);
-  cudaError_t err = cudaFuncSetAttribute(route_count_kernel<ROUTER, PER, GROUPED>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem1);
-  if (err == cudaSuccess)
-    err = cudaFuncSetAttribute(route_scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem2);
+  auto count_bytes = [](int E) { return (size_t)kRouteWarps * E * sizeof(int32_t); };
+  auto scatter_bytes = [](int E) { return (size_t)(kRouteWarps * E + 5 * E + 2) * sizeof(int32_t); };
+  const size_t smem1 = count_bytes(a.E), smem2 = scatter_bytes(a.E);
+  cudaError_t err = allow_smem(route_count_kernel<ROUTER, PER, GROUPED>, count_bytes(kRouteMaxExperts));
+  if (err == cudaSuccess) err = allow_smem(route_scatter_kernel, scatter_bytes(kRouteMaxExperts));
   if (err != cudaSuccess) return err;
   route_count_kernel<ROUTER, PER, GROUPED><<<C, kRouteThreads, smem1, stream>>>(a, scratch, r);
   err = cudaGetLastError();
@@ -384,7 +392,7 @@ cudaError_t launch_route_logits_impl(const AlignArgs& a_in, const RouterArgs& r,
   const int64_t ctas = M > 0 ? (M + tpc - 1) / tpc : 1;
   auto kernel = per == 8 ? router_align_kernel<8, GROUPED>
                          : (per == 16 ? router_align_kernel<16, GROUPED> : router_align_kernel<32, GROUPED>);
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t err = allow_smem(kernel, align_smem_bytes(kRouteMaxExperts));
   if (err != cudaSuccess) return err;
   kernel<<<(unsigned)ctas, kRouteThreads, smem, stream>>>(a, r, M, tpc, counter);
   return cudaGetLastError();
