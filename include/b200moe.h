@@ -236,6 +236,46 @@ B200MOE_API int b200moe_layer_quantized(const uint8_t* hidden_q, const float* hi
                                         const int32_t* expert_map, int num_local_experts, void* out,
                                         void* workspace, size_t workspace_bytes, void* stream);
 
+/* The four entries above in one, with the header apart from the workspace: a
+ * caller whose workspace moves when it has to grow keeps one header, so that an
+ * error word is not lost and a captured graph goes on reporting into the one
+ * that is read. Either hidden, or hidden_q with hidden_scale, as in
+ * b200moe_layer_quantized. With router_logits NULL topk_weights and topk_ids are
+ * inputs, else outputs; num_groups 0 = no groups. header: 256 bytes as the first
+ * 256 of a workspace (those of this workspace are not used), 256-byte aligned,
+ * for one call at a time like the workspace. All members are 8 bytes wide. */
+typedef struct b200moe_layer_args {
+  const void* hidden;
+  const uint8_t* hidden_q;
+  const float* hidden_scale;
+  int64_t M, H, I, num_experts, topk;
+  const void* router_logits;
+  int64_t logits_bf16, num_groups, topk_groups, scoring;
+  const float* correction_bias;
+  int64_t renormalize;
+  double scaling;
+  const uint8_t* w13;
+  const float* w13_scale;
+  const uint8_t* w2;
+  const float* w2_scale;
+  float* topk_weights;
+  int32_t* topk_ids;
+  const int32_t* expert_map;
+  int64_t num_local_experts;
+  void* out;
+  int32_t* header;
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} b200moe_layer_args;
+B200MOE_API int b200moe_layer_call(const b200moe_layer_args* args);
+
+/* *header = 256 zeroed bytes on the current device (a header, or the error word
+ * of the dense products), there until the process exits. Synchronises with the
+ * host, and may be called while a stream is being captured: nothing of it becomes
+ * part of the graph. */
+B200MOE_API int b200moe_header_create(int32_t** header);
+
 /* ------------------------------------------------------------------------
  * Expert parallelism over G ranks: rank r owns experts [r*E/G, (r+1)*E/G).
  * Replaces the dispatch/combine that the reference consumes from DeepEP/Mori

@@ -50,6 +50,8 @@ SIGNATURES = {
     "b200moe_layer_logits_grouped": (_I, [_P, _L, _L, _L, _I, _I, _P, _I, _I, _I, _I, _P, _I, ctypes.c_float, _P, _P,
                                           _P, _P, _P, _I, _P, _P, _P, _P, _S, _P]),
     "b200moe_layer_quantized": (_I, [_P, _P, _L, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _S, _P]),
+    "b200moe_layer_call": (_I, [ctypes.c_char_p]),  # a packed argument struct
+    "b200moe_header_create": (_I, [_P]),
     "b200moe_ep_row_bytes": (_L, [_L, _I]),
     "b200moe_ep_dispatch": (_I, [_P, _P, _P, _P, _L, _L, _I, _I, _I, _I, _P, _I, _I, _L, _P, _P, _P, _P, _P, _P]),
     "b200moe_layer_packed_workspace_size": (_S, [_L, _L, _L, _I, _I]),

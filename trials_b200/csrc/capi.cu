@@ -273,6 +273,9 @@ int record_error(int status, const char* message) { return fail(status, "%s", me
 
 namespace {
 
+// A size of an argument struct as int; what does not fit stays too large or negative.
+int int_size(int64_t v) { return (int)(v < -1 ? -1 : v > (1 << 30) ? (1 << 30) : v); }
+
 // Host checks of the router arguments (b200moe_router_topk and routing from logits).
 int check_router(const char* name, const void* logits, int64_t M, int num_experts, int topk, int scoring,
                  const float* correction_bias, const float* topk_weights, const int32_t* topk_ids) {
@@ -1049,7 +1052,7 @@ int layer_core(const char* name, const LayerInput& in, int64_t M, int64_t H, int
                const float* topk_weights, const int32_t* topk_ids, const int32_t* expert_map, int num_local_experts,
                void* out, void* workspace, size_t workspace_bytes, size_t workspace_offset, void* stream,
                const EpPeerArgs* peer_out = nullptr, int32_t* peer_counter = nullptr, int64_t tile_numel = -1,
-               const RouterArgs* router = nullptr, const PackedMeta* packed = nullptr) {
+               const RouterArgs* router = nullptr, const PackedMeta* packed = nullptr, int32_t* header = nullptr) {
   int st = check_gemm_shapes(H, I);
   if (st) return st;
   if (M < 0 || topk <= 0 || num_experts <= 0) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
@@ -1066,7 +1069,7 @@ int layer_core(const char* name, const LayerInput& in, int64_t M, int64_t H, int
   const LayerPlan pl = plan_layer(M, H, I, E, topk, tile_numel >= 0 ? pick_tile_tokens(tile_numel, E) : 0);
   if (workspace_bytes < workspace_offset + pl.total) return fail(B200MOE_ERR_WORKSPACE, "%s: workspace too small", name);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  int32_t* err = reinterpret_cast<int32_t*>(ws);
+  int32_t* err = header ? header : reinterpret_cast<int32_t*>(ws);
   uint8_t* wl = ws + workspace_offset;  // layer regions (the error word stays at offset 0)
   int32_t* sorted = reinterpret_cast<int32_t*>(wl + pl.off_sorted);
   int32_t* pos = reinterpret_cast<int32_t*>(wl + pl.off_pos);
@@ -1195,6 +1198,56 @@ int b200moe_layer_logits_grouped(const void* hidden, int64_t M, int64_t H, int64
   return layer_core("b200moe_layer_logits_grouped", in, M, H, I, num_experts, topk, w13, w13_scale, w2, w2_scale,
                     topk_weights, topk_ids, expert_map, num_local_experts, out, workspace, workspace_bytes, 0, stream,
                     nullptr, nullptr, -1, &r);
+}
+
+int b200moe_layer_call(const b200moe_layer_args* a) {
+  if (!a) return fail(B200MOE_ERR_INVALID_ARG, "b200moe_layer_call: bad argument%s");
+  const bool logits = a->router_logits != nullptr, grouped = logits && a->num_groups != 0;
+  const char* name = grouped ? "b200moe_layer_logits_grouped" : logits ? "b200moe_layer_logits"
+                     : a->hidden_q ? "b200moe_layer_quantized" : "b200moe_layer";
+  if (a->M > 0 && ((a->hidden != nullptr) == (a->hidden_q != nullptr) || (a->hidden_q && !a->hidden_scale) ||
+                   !a->header || (reinterpret_cast<uintptr_t>(a->header) & 255) != 0))
+    return fail(B200MOE_ERR_INVALID_ARG, "%s: bad activations or header", name);
+  const int E = int_size(a->num_experts), k = int_size(a->topk), scoring = int_size(a->scoring);
+  RouterArgs r{};
+  if (logits) {
+    const int G = int_size(a->num_groups), T = int_size(a->topk_groups);
+    const int st = grouped ? check_router_grouped(name, a->router_logits, a->M, E, G, T, k, scoring, a->correction_bias,
+                                                  a->topk_weights, a->topk_ids)
+                           : check_router(name, a->router_logits, a->M, E, k, scoring, a->correction_bias,
+                                          a->topk_weights, a->topk_ids);
+    if (st) return st;
+    const int bf16 = a->logits_bf16 != 0, renorm = a->renormalize != 0;
+    r = grouped ? grouped_router(a->router_logits, bf16, E, G, T, k, scoring, a->correction_bias, renorm,
+                                 (float)a->scaling, a->topk_weights, a->topk_ids)
+                : RouterArgs{a->router_logits, bf16, E, k, scoring, renorm, a->correction_bias, (float)a->scaling,
+                             a->topk_weights, a->topk_ids};
+  }
+  const LayerInput in{a->hidden, a->hidden_q, a->H, a->hidden_scale, a->H / 128};
+  return layer_core(name, in, a->M, a->H, a->I, E, k, a->w13, a->w13_scale, a->w2, a->w2_scale, a->topk_weights,
+                    a->topk_ids, a->expert_map, int_size(a->num_local_experts), a->out, a->workspace,
+                    a->workspace_bytes, 0, a->stream, nullptr, nullptr, -1, logits ? &r : nullptr, nullptr, a->header);
+}
+
+int b200moe_header_create(int32_t** header) {
+  if (!header) return fail(B200MOE_ERR_INVALID_ARG, "b200moe_header_create: null pointer%s");
+  // A capture in progress (of this thread or another) neither forbids these calls in relaxed
+  // mode nor records them, as the stream is none that is captured.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  int st = cuda_status(cudaThreadExchangeStreamCaptureMode(&mode), "header_create");
+  if (st) return st;
+  void* p = nullptr;
+  cudaStream_t s = nullptr;
+  cudaError_t e = cudaMalloc(&p, 256);
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, 256, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (s) cudaStreamDestroy(s);
+  if (e != cudaSuccess && p) cudaFree(p);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  st = cuda_status(e, "header_create");
+  if (!st) *header = static_cast<int32_t*>(p);
+  return st;
 }
 
 int64_t b200moe_ep_row_bytes(int64_t H, int topk) { return round_up(H + (H / 128) * 4 + 8 * (int64_t)topk, 16); }
@@ -1456,10 +1509,8 @@ int b200moe_router_topk(const void* logits, int logits_bf16, int64_t M, int num_
 int b200moe_router_topk_grouped(const b200moe_router_grouped_args* a) {
   const char* name = "b200moe_router_topk_grouped";
   if (!a) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
-  // Sizes as int; what does not fit stays too large or negative.
-  auto size = [](int64_t v) { return (int)(v < -1 ? -1 : v > (1 << 30) ? (1 << 30) : v); };
-  const int E = size(a->num_experts), G = size(a->num_groups), T = size(a->topk_groups), k = size(a->topk);
-  const int scoring = size(a->scoring);
+  const int E = int_size(a->num_experts), G = int_size(a->num_groups), T = int_size(a->topk_groups);
+  const int k = int_size(a->topk), scoring = int_size(a->scoring);
   const int st = check_router_grouped(name, a->logits, a->M, E, G, T, k, scoring, a->correction_bias, a->topk_weights,
                                       a->topk_ids);
   if (st) return st;

@@ -44,13 +44,12 @@ def _device_of(x: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
 def _call(fn, where: str, index: int, *args: int) -> None:
     """Calls a C entry on the current stream of device `index` (kernels launch on
     the current device); args are its arguments up to the error word and the
-    stream. The error word is the cached one of (device, stream)
-    (moe.layer_error_word)."""
+    stream. The error word is the one of (device, stream), moe.layer_error_word."""
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
             return _call(fn, where, index, *args)
     stream = torch._C._cuda_getCurrentRawStream(index)
-    status = fn(_PACK[len(args) + 2](*args, _workspaces.error_ptr(index, stream), stream))
+    status = fn(_PACK[len(args) + 2](*args, _workspaces.header_ptr(index, stream), stream))
     if status:
         _lib.check(status, where)
 

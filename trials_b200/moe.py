@@ -54,38 +54,63 @@ def _require_cuda(*tensors: torch.Tensor) -> torch.device:
 
 
 class _Workspaces:
-    """Grow-only per-(device, stream) workspace buffers. Their first 256 bytes
-    are zeroed at allocation: the device error word (int 0), then the router's
-    CTA counter and the whole-layer launch's sync words (ints 1..3, left at
-    zero by every call)."""
+    """What calls on one (device, stream) share: a header of 256 zeroed bytes (the
+    device error word, int 0, then the router's CTA counter and the whole-layer
+    launch's sync words, ints 1..3, left at zero by every call) and the layer's
+    grow-only scratch. A header is there until the process exits, since captured
+    graphs keep its address, and is zeroed outside any capture, or a graph's replay
+    would clear it. A scratch that a captured graph may use is kept when a larger
+    one takes its place."""
 
     def __init__(self):
+        self._headers = {}
         self._bufs = {}
+        self._captured = set()  # keys whose scratch a captured call was given
+        self._kept = []
         self._lock = threading.Lock()
 
     def get(self, device: torch.device, nbytes: int) -> torch.Tensor:
-        return self.get_for(device, _stream(device), nbytes)
-
-    def get_for(self, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-        """The buffer of (device, stream), `stream` being the device's current one."""
-        key = (device.index, stream)
+        """The scratch of (device, its current stream)."""
+        key = (device.index, _stream(device))
+        capturing = torch.cuda.is_current_stream_capturing()
         with self._lock:
             buf = self._bufs.get(key)
             if buf is None or buf.numel() < nbytes:
-                buf = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
-                buf[:256].zero_()
+                if key in self._captured:
+                    self._kept.append(buf)
+                    self._captured.discard(key)
+                buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
                 self._bufs[key] = buf
+            if capturing:
+                self._captured.add(key)
             return buf
 
-    def error_ptr(self, index: int, stream: int) -> int:
-        """Address of the error word of (device index, its current stream)."""
-        buf = self._bufs.get((index, stream))
-        return (self.get_for(torch.device("cuda", index), stream, 256) if buf is None else buf).data_ptr()
+    def header_ptr(self, index: int, stream: int) -> int:
+        """Address of the header of (device index, its current stream)."""
+        ptr = self._headers.get((index, stream))
+        return self._new_header(index, stream) if ptr is None else ptr
+
+    def _new_header(self, index: int, stream: int) -> int:
+        with self._lock:
+            if (index, stream) not in self._headers:
+                out = ctypes.c_void_p()
+                with torch.cuda.device(index):
+                    _lib.check(_lib.lib().b200moe_header_create(ctypes.byref(out)), "header_create")
+                self._headers[index, stream] = out.value
+            return self._headers[index, stream]
+
+
+class _DeviceInts:
+    """Device memory as the CUDA array interface describes it."""
+
+    def __init__(self, ptr: int, n: int):
+        self.__cuda_array_interface__ = {"shape": (n,), "typestr": "<i4", "data": (ptr, False), "version": 2}
 
 
 _workspaces = _Workspaces()
 _SCORING = {"softmax": 0, "sigmoid": 1}
 _PACK_GROUPED = struct.Struct("10qd3q").pack  # b200moe_router_grouped_args
+_PACK_LAYER = struct.Struct("15qd13q").pack  # b200moe_layer_args
 
 
 def read_device_error(err_word: torch.Tensor, clear: bool = True) -> int:
@@ -97,9 +122,11 @@ def read_device_error(err_word: torch.Tensor, clear: bool = True) -> int:
 
 
 def layer_error_word(device: Optional[torch.device] = None) -> torch.Tensor:
-    """The error word of the cached layer workspace for (device, current stream)."""
-    device = device or torch.device("cuda", torch.cuda.current_device())
-    return _workspaces.get(device, 256)[:4].view(torch.int32)
+    """The error word of the calls on (device, its current stream), graphs captured
+    on that stream among them; the same word until the process exits."""
+    index = torch.cuda.current_device() if device is None or device.index is None else device.index
+    ptr = _workspaces.header_ptr(index, torch._C._cuda_getCurrentRawStream(index))
+    return torch.as_tensor(_DeviceInts(ptr, 1), device=torch.device("cuda", index))
 
 
 # ----------------------------------------------------------------------------
@@ -124,9 +151,10 @@ def moe_align_block_size(topk_ids: torch.Tensor, block_size: int, num_experts: i
     sorted_ids = torch.empty(cap, dtype=torch.int32, device=dev)
     expert_ids = torch.empty(cap_b, dtype=torch.int32, device=dev)
     ntp = torch.empty(1, dtype=torch.int32, device=dev)
-    err = err_word if err_word is not None else layer_error_word(dev)
+    stream = _stream(dev)
+    err = _workspaces.header_ptr(ids.get_device(), stream) if err_word is None else _ptr(err_word)
     _lib.check(L.b200moe_align(_ptr(ids), M, topk, num_experts, block_size, _ptr(expert_map), E or 0,
-                               _ptr(sorted_ids), cap, _ptr(expert_ids), cap_b, _ptr(ntp), _ptr(err), _stream(dev)),
+                               _ptr(sorted_ids), cap, _ptr(expert_ids), cap_b, _ptr(ntp), err, stream),
                "moe_align_block_size")
     return sorted_ids, expert_ids, ntp
 
@@ -134,6 +162,8 @@ def moe_align_block_size(topk_ids: torch.Tensor, block_size: int, num_experts: i
 def _check_groups(num_expert_group: Optional[int], topk_group: Optional[int]) -> bool:
     if (num_expert_group is None) != (topk_group is None):
         raise ValueError("num_expert_group and topk_group go together")
+    if num_expert_group is not None and num_expert_group < 1:
+        raise ValueError("num_expert_group must be positive")
     return num_expert_group is not None
 
 
@@ -262,6 +292,20 @@ def _check_layer_args(hidden, w13, w13_scale, w2, w2_scale, topk_weights, topk_i
     return dev, M, H, I, E
 
 
+_NO_ROUTER = (0, 0, 0, 0, 0, 0, 0, 0.0)
+
+
+def _layer_call(where: str, dev: torch.device, ws_bytes: int, rows, sizes, router, tensors, n_local: int,
+                out: torch.Tensor) -> None:
+    """b200moe_layer_call on the current stream of `dev`, with its header and scratch."""
+    ws = _workspaces.get(dev, ws_bytes)
+    stream = _stream(dev)
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    _lib.check(_lib.lib().b200moe_layer_call(_PACK_LAYER(
+        *rows, *sizes, *router, *(_ptr(t) or 0 for t in tensors), n_local, _ptr(out),
+        _workspaces.header_ptr(index, stream), _ptr(ws), ws.numel(), stream)), where)
+
+
 def _run_layer(hidden, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids, expert_map, num_experts, out=None,
                a1_scale=None):
     dev, M, H, I, E_w = _check_layer_args(hidden, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids, a1_scale)
@@ -276,21 +320,15 @@ def _run_layer(hidden, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids, exp
     L = _lib.lib()
     n_local = E_w
     ws_bytes = L.b200moe_layer_workspace_size(M, H, I, num_experts, n_local, topk)
-    ws = _workspaces.get(dev, ws_bytes)
     # Contiguous copies are bound to names so that they live until the call
     # returns: a copy whose pointer alone were passed could be freed, and its
     # memory reused by the next copy, before the kernels read it.
     w13_scale, w2_scale = w13_scale.contiguous(), w2_scale.contiguous()
-    if hidden.dtype == FP8:
-        a1 = a1_scale.to(torch.float32).contiguous()
-        _lib.check(L.b200moe_layer_quantized(_ptr(hidden), _ptr(a1), M, H, I, num_experts, topk, _ptr(w13),
-                                             _ptr(w13_scale), _ptr(w2), _ptr(w2_scale),
-                                             _ptr(tw), _ptr(ids), _ptr(expert_map), n_local, _ptr(out), _ptr(ws),
-                                             ws.numel(), _stream(dev)), "b200moe_layer_quantized")
-        return out
-    _lib.check(L.b200moe_layer(_ptr(hidden), M, H, I, num_experts, topk, _ptr(w13), _ptr(w13_scale),
-                               _ptr(w2), _ptr(w2_scale), _ptr(tw), _ptr(ids), _ptr(expert_map),
-                               n_local, _ptr(out), _ptr(ws), ws.numel(), _stream(dev)), "b200moe_layer")
+    fp8 = hidden.dtype == FP8
+    a1 = a1_scale.to(torch.float32).contiguous() if fp8 else None
+    _layer_call("b200moe_layer_quantized" if fp8 else "b200moe_layer", dev, ws_bytes,
+                (0, _ptr(hidden), _ptr(a1)) if fp8 else (_ptr(hidden), 0, 0), (M, H, I, num_experts, topk), _NO_ROUTER,
+                (w13, w13_scale, w2, w2_scale, tw, ids, expert_map), n_local, out)
     return out
 
 
@@ -425,17 +463,13 @@ def moe_layer_from_logits(hidden_states: torch.Tensor, router_logits: torch.Tens
     hidden = hidden_states.contiguous()
     w13_scale, w2_scale = w13_scale.contiguous(), w2_scale.contiguous()  # held through the call
     L = _lib.lib()
-    ws = _workspaces.get(dev, L.b200moe_layer_workspace_size(M, H, I, E_router, E_w, top_k))
-    args = (_ptr(bias), int(renormalize), float(routed_scaling_factor), _ptr(w13_fp8), _ptr(w13_scale), _ptr(w2_fp8),
-            _ptr(w2_scale), _ptr(expert_map), E_w, _ptr(tw), _ptr(ids), _ptr(out), _ptr(ws), ws.numel(), _stream(dev))
-    if grouped:
-        _lib.check(L.b200moe_layer_logits_grouped(_ptr(hidden), M, H, I, E_router, top_k, _ptr(logits),
-                                                  int(logits.dtype == torch.bfloat16), num_expert_group, topk_group,
-                                                  scoring, *args), "b200moe_layer_logits_grouped")
-    else:
-        _lib.check(L.b200moe_layer_logits(_ptr(hidden), M, H, I, E_router, top_k, _ptr(logits),
-                                          int(logits.dtype == torch.bfloat16), scoring, *args),
-                   "b200moe_layer_logits")
+    _layer_call("b200moe_layer_logits_grouped" if grouped else "b200moe_layer_logits", dev,
+                L.b200moe_layer_workspace_size(M, H, I, E_router, E_w, top_k), (_ptr(hidden), 0, 0),
+                (M, H, I, E_router, top_k),
+                (_ptr(logits), logits.dtype == torch.bfloat16, num_expert_group if grouped else 0,
+                 topk_group if grouped else 0, scoring, _ptr(bias) or 0, bool(renormalize),
+                 float(routed_scaling_factor)),
+                (w13_fp8, w13_scale, w2_fp8, w2_scale, tw, ids, expert_map), E_w, out)
     if shared_expert is not None:
         from .dense import fp8_mlp
 
