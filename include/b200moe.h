@@ -618,7 +618,7 @@ B200MOE_API int b200moe_combine_reduce(const void* out_pair, const int32_t* slot
  *               * sum_{k in block kb} x_q[m, k] * w[n, k]  (+ residual[m, n])
  * in fp32, rounded once to bf16 (out_f32 = 0) or stored as f32 (1).
  * Activations: either x (M, K) bf16, quantised first as b200moe_quant_1x128
- * does, or x_q (M, K) fp8 with x_scale (M, K/128); pass NULL for the other.
+ * does (but see NaN below), or x_q (M, K) fp8 with x_scale (M, K/128); pass NULL for the other.
  * workspace: b200moe_linear_workspace_size() bytes (may be 0), 256-byte aligned.
  * ld_x / ld_xs are row strides in elements of x or x_q / x_scale (ld_xs is not
  * read with bf16 rows). w (N, K) fp8 with row stride ld_w bytes; w_scale
@@ -636,6 +636,12 @@ B200MOE_API int b200moe_combine_reduce(const void* out_pair, const int32_t* slot
  * result, bit for bit: a dense or shared expert, residual = the routed output
  * to add to; out may also be x. Weights contiguous; workspace b200moe_mlp_workspace_size() bytes,
  * 256-byte aligned.
+ *
+ * NaN: here a NaN is kept. One in a bf16 row makes the scale and codes of its
+ * 128-group NaN, an infinity makes the scale infinite and its own code NaN, and
+ * either makes the token's outputs NaN; so do NaN codes and scales that come in.
+ * A NaN of silu(gate) * up makes its group of q and s NaN, an infinity s infinite.
+ * (b200moe_quant_1x128 and the routed layer code a NaN as -448.)
  *
  * The calls take their arguments in a struct whose members are all 8 bytes
  * wide (set every one; a foreign-function interface fills it in one step). A

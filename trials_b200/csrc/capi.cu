@@ -1586,7 +1586,18 @@ size_t dense_quant_bytes(int64_t M, int64_t K) {
 int dense_quantise(DenseInput& in, int64_t M, int64_t K, uint8_t* ws, void* stream) {
   uint8_t* q = ws;
   float* s = reinterpret_cast<float*>(ws + round_up(M * K, 256));
-  const int st = b200moe_quant_1x128(in.x, M, K, in.ld_x, q, K, s, K / 128, 1, stream);
+  QuantArgs a{};  // as b200moe_quant_1x128, a NaN kept
+  a.x = in.x;
+  a.ldx = in.ld_x;
+  a.K = K;
+  a.rows = M;
+  a.q = q;
+  a.ldq = K;
+  a.s = s;
+  a.s_row = K / 128;
+  a.s_grp = 1;
+  a.keep_nan = 1;
+  const int st = cuda_status(launch_quant_1x128(a, (cudaStream_t)stream), "quant_1x128");
   if (st) return st;
   in = DenseInput{nullptr, q, s, K, K / 128};
   return B200MOE_OK;

@@ -32,8 +32,8 @@ __device__ __forceinline__ uint8_t quant_e4m3(float x, float scale) {
 // far below the smallest code and rounds to zero either way. It is computed negated,
 // qn = -q with nrcp = -rcp, which gives a zero the quotient's sign, and the codes'
 // signs are turned over. An infinite scale (nrcp = -0, its place taken by 0) gives
-// x * 0 as the division does. The conversion saturates at 448 by itself; CLAMP: the
-// values may hold NaN, which becomes -448. 8,192 x 6,144 bf16 values quantised 1x128:
+// x * 0 as the division does. The conversion saturates at 448 by itself and gives NaN its
+// own code; CLAMP: NaN becomes -448. 8,192 x 6,144 bf16 values quantised 1x128:
 // 47.7 us with the division, 39.4 with scalar fmas, sign and range put right for each
 // value, 32.1 like this.
 struct CodeScale {
@@ -60,8 +60,9 @@ __device__ __forceinline__ uint32_t negated_codes(float x0, float x1, CodeScale 
   }
   return __nv_cvt_float2_to_fp8x2(make_float2(q0, q1), __NV_SATFINITE, __NV_E4M3);
 }
+template <bool CLAMP>
 __device__ __forceinline__ uint16_t quant_e4m3x2(float x0, float x1, CodeScale c) {
-  return (uint16_t)(negated_codes<true>(x0, x1, c) ^ 0x8080u);
+  return (uint16_t)(negated_codes<CLAMP>(x0, x1, c) ^ 0x8080u);
 }
 template <bool CLAMP>
 __device__ __forceinline__ uint32_t quant_e4m3x4(float x0, float x1, float x2, float x3, CodeScale c) {
@@ -70,6 +71,17 @@ __device__ __forceinline__ uint32_t quant_e4m3x4(float x0, float x1, float x2, f
 
 // Group scale: max(amax / 448, 1e-12) in fp32 (phase5_orchestrator.py:29-30).
 __device__ __forceinline__ float group_scale(float amax) { return fmaxf(__fdiv_rn(amax, 448.0f), 1e-12f); }
+
+// The larger of two, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// The same scale where a NaN among the magnitudes has to reach it, as it does through
+// torch's amax and clamp: with an unclamped code_scale conversion all codes of the group
+// become NaN, and an infinity (scale infinite) leaves zeros and NaN in its own place.
+__device__ __forceinline__ float group_scale_nan(float amax) { return max_nan(__fdiv_rn(amax, 448.0f), 1e-12f); }
 
 // Work-unit order of the grouped GEMMs. A unit is (chunk, weight tile nt).
 // Chunks are taken in groups of `group` consecutive chunks, and inside a group

@@ -33,8 +33,18 @@ __device__ __forceinline__ void promote(float (&acc)[NC], uint32_t taddr, float 
   }
 }
 
+// silu_f32 with a NaN kept (there d < 1e30 fails for it and gives -0).
+__device__ __forceinline__ float silu_nan(float g) {
+#if B200MOE_FAST_SILU
+  const float d = 1.0f + __expf(-g);
+  return d >= 1e30f ? -0.0f : __fdividef(g, d);
+#else
+  return silu_f32(g);
+#endif
+}
+
 // silu(gate) * up of a token's NC / 2 (gate, up) pairs into acc[0 .. NC/2 - 1];
-// returns their largest magnitude. (A reciprocal shared by four values, for half the
+// returns their largest magnitude, NaN if one is. (A reciprocal shared by four values, for half the
 // load of the special-function unit, needs a branch for large gates and measured 4-12%
 // slower: 62 us to 70 for 5772 x 768 x 3584.)
 template <int NC>
@@ -42,8 +52,8 @@ __device__ __forceinline__ float silu_pairs(float (&acc)[NC]) {
   float mx = 0.f;
 #pragma unroll
   for (int i = 0; i < NC / 2; ++i) {
-    acc[i] = silu_f32(acc[2 * i]) * acc[2 * i + 1];
-    mx = fmaxf(mx, fabsf(acc[i]));
+    acc[i] = silu_nan(acc[2 * i]) * acc[2 * i + 1];
+    mx = max_nan(mx, fabsf(acc[i]));
   }
   return mx;
 }
@@ -58,7 +68,7 @@ __device__ __forceinline__ void store_codes(const float (&acc)[NC], float scale,
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float* v = acc + k * 16 + i * 4;
-      w[i] = quant_e4m3x4<true>(v[0], v[1], v[2], v[3], cs);
+      w[i] = quant_e4m3x4<false>(v[0], v[1], v[2], v[3], cs);
     }
     reinterpret_cast<uint4*>(q)[k] = make_uint4(w[0], w[1], w[2], w[3]);
   }
@@ -273,19 +283,19 @@ __device__ __forceinline__ void finish_tokens_of(const DenseParams& p, int64_t m
         float y[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          y[2 * h] = silu_f32(sum[h].x) * sum[h].y;
-          y[2 * h + 1] = silu_f32(sum[h].z) * sum[h].w;
+          y[2 * h] = silu_nan(sum[h].x) * sum[h].y;
+          y[2 * h + 1] = silu_nan(sum[h].z) * sum[h].w;
         }
-        float mx = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+        float mx = max_nan(max_nan(fabsf(y[0]), fabsf(y[1])), max_nan(fabsf(y[2]), fabsf(y[3])));
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float scale = group_scale(mx);
+        for (int o = 16; o >= 1; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float scale = group_scale_nan(mx);
         const CodeScale cs = code_scale(scale);
         const int unit = n0 >> 8;
         uint8_t* dst = p.q + m * p.ld_q + unit * 128 + lane * 2;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<uint16_t*>(dst + h * 64) = quant_e4m3x2(y[2 * h], y[2 * h + 1], cs);
+          *reinterpret_cast<uint16_t*>(dst + h * 64) = quant_e4m3x2<false>(y[2 * h], y[2 * h + 1], cs);
         if (lane == 0) p.s[m * p.ld_s + unit] = scale;
       } else {
 #pragma unroll

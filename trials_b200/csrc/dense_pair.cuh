@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(DensePairCfg<EPI>::THREADS, 1)
         parity ^= 1;
         rb[h * C::TM + r] = silu_pairs(acc);
         named_bar_sync(1, C::EW * 32);
-        const float scale = group_scale(fmaxf(rb[r], rb[C::TM + r]));
+        const float scale = group_scale_nan(max_nan(rb[r], rb[C::TM + r]));
         if (ok && m < p.M) {
           store_codes(acc, scale, p.q + m * p.ld_q + nt * 128 + h * 64);
           if (h == 0) p.s[m * p.ld_s + nt] = scale;

@@ -14,7 +14,7 @@
 // silu(gate) * up values.
 //
 // QX: x comes in bf16 and every CTA quantises its K blocks of it itself (the
-// arithmetic of b200moe_quant_1x128), straight into the swizzled operand tiles:
+// arithmetic of b200moe_quant_1x128, NaN kept), straight into the swizzled operand tiles:
 // for a few tokens that is cheaper than a launch.
 //
 // With `early_w` the kernel ahead of it in the stream is one of this call's own
@@ -239,15 +239,15 @@ __global__ void __launch_bounds__(DenseSplitCfg<T>::THREADS, 2)
           const float2 f = __bfloat1622float2(h2[i]);
           v[2 * i] = f.x;
           v[2 * i + 1] = f.y;
-          mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+          mx = max_nan(mx, max_nan(fabsf(f.x), fabsf(f.y)));
         }
 #pragma unroll
-        for (int o = 8; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float scale = group_scale(mx);
+        for (int o = 8; o >= 1; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float scale = group_scale_nan(mx);
         const CodeScale cs = code_scale(scale);
         uint32_t w[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) w[i] = quant_e4m3x4<true>(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], cs);
+        for (int i = 0; i < 2; ++i) w[i] = quant_e4m3x4<false>(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], cs);
         if (g < total) {
           *reinterpret_cast<uint2*>(xq + kb * tt * 128 + t * 128 + (((sub >> 1) ^ (t & 7)) << 4) + (sub & 1) * 8) =
               make_uint2(w[0], w[1]);

@@ -117,6 +117,7 @@ struct QuantArgs {
   // slot_pos / sorted_ids were written earlier in the same launch: read them
   // through L2 instead of the read-only path.
   int meta_l2;
+  int keep_nan;  // a NaN makes its group NaN (the dense products); else it becomes -448
   int32_t sentinel;
   uint8_t* q;
   int64_t ldq;

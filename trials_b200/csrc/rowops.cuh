@@ -103,15 +103,22 @@ __device__ __forceinline__ void quant_row_segment(const QuantArgs& a, int64_t ro
       v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
     }
     if (__any_sync(0xffffffffu, mm >= 0x7f800000u)) {
-      // Infinities or NaN: the largest number counts, NaN becomes -448.
+      // Infinities or NaN. keep_nan: a NaN reaches its group's scale and codes, an
+      // infinity's code is NaN; else the largest number counts and NaN becomes -448.
       float m = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+      for (int j = 0; j < 8; ++j) m = a.keep_nan ? max_nan(m, fabsf(v[j])) : fmaxf(m, fabsf(v[j]));
 #pragma unroll
-      for (int o = 8; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      scl[i] = group_scale(m);
+      for (int o = 8; o >= 1; o >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, m, o);
+        m = a.keep_nan ? max_nan(m, other) : fmaxf(m, other);
+      }
+      scl[i] = a.keep_nan ? group_scale_nan(m) : group_scale(m);
       const CodeScale cs = code_scale(scl[i]);
-      packed[i] = make_uint2(quant_e4m3x4<true>(v[0], v[1], v[2], v[3], cs), quant_e4m3x4<true>(v[4], v[5], v[6], v[7], cs));
+      packed[i] = a.keep_nan ? make_uint2(quant_e4m3x4<false>(v[0], v[1], v[2], v[3], cs),
+                                          quant_e4m3x4<false>(v[4], v[5], v[6], v[7], cs))
+                             : make_uint2(quant_e4m3x4<true>(v[0], v[1], v[2], v[3], cs),
+                                          quant_e4m3x4<true>(v[4], v[5], v[6], v[7], cs));
     } else {
       scl[i] = group_scale(__uint_as_float(mm));
       const CodeScale cs = code_scale(scl[i]);

@@ -9,7 +9,9 @@ layer's number formats.
 
 The reference has no counterpart: its serving framework fuses the shared expert
 as one more routed slot (runner.fuse_shared_expert), which needs the routed
-experts' intermediate size. Every op runs the CUDA kernels of libb200moe.so on
+experts' intermediate size. A NaN in a token's row, or in silu(gate) * up, is kept:
+it makes its 128-group and the outputs behind it NaN (per_token_group_quant_fp8 and
+the routed layer code it as -448). Every op runs the CUDA kernels of libb200moe.so on
 the current torch stream of its tensors' device; there is no fallback path.
 """
 from __future__ import annotations
