@@ -165,3 +165,56 @@ def test_python_weight_and_output_checks():
             dense._output(o, r, 3, 5, torch.bfloat16, out.device)
     with pytest.raises(NotImplementedError):
         dense._output(None, out.float(), 3, 5, torch.bfloat16, out.device)
+
+
+class TwoDevices:
+    """A stand-in for a process with two unlike GPUs, device 0 current and the
+    tensors on device 1: what the library is asked, and on which device."""
+
+    def __init__(self, monkeypatch):
+        self.current, self.asked = 0, []
+        outer = self
+
+        class Guard:
+            def __init__(self, index):
+                self.index = index
+
+            def __enter__(self):
+                self.back, outer.current = outer.current, self.index
+
+            def __exit__(self, *a):
+                outer.current = self.back
+
+        class Lib:
+            b200moe_linear = b200moe_gate_up = b200moe_mlp = staticmethod(lambda packed: outer.note("call"))
+            b200moe_linear_workspace_size = staticmethod(lambda *a: outer.note("size") or 256 * (outer.current + 1))
+            b200moe_mlp_workspace_size = b200moe_linear_workspace_size
+
+        monkeypatch.setattr(torch.cuda, "device", Guard)
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: self.current)
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+        monkeypatch.setattr(dense._lib, "lib", lambda: Lib)
+        monkeypatch.setattr(dense, "_device_of", lambda *t: 1)
+        monkeypatch.setattr(dense._workspaces, "header_ptr", lambda index, stream: P)
+        dense._linear_bytes.cache_clear()
+        dense._mlp_bytes.cache_clear()
+
+    def note(self, what):
+        self.asked.append((what, self.current))
+        return 0
+
+
+def test_everything_is_asked_on_the_tensors_device(monkeypatch):
+    both = TwoDevices(monkeypatch)
+    x = torch.zeros(3000, 256, dtype=torch.bfloat16)
+    w, s = torch.zeros(512, 256).to(FP8), torch.ones(4, 2)
+    w2, s2 = torch.zeros(256, 256).to(FP8), torch.ones(2, 2)
+    fp8_block_linear(x, w, s)
+    fp8_gate_up(x, w, s)
+    fp8_mlp(x, w, s, w2, s2)
+    assert both.asked == [("size", 1), ("call", 1)] * 3 and both.current == 0
+    # and sizes kept for one device are not given to another
+    both.current = 1
+    assert dense._linear_bytes(1, 3000, 512, 256, 0) == 512
+    dense._linear_bytes.cache_clear()
+    dense._mlp_bytes.cache_clear()

@@ -44,12 +44,9 @@ def _device_of(x: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
 
 
 def _call(fn, where: str, index: int, *args: int) -> None:
-    """Calls a C entry on the current stream of device `index` (kernels launch on
-    the current device); args are its arguments up to the error word and the
-    stream. The error word is the one of (device, stream), moe.layer_error_word."""
-    if torch.cuda.current_device() != index:
-        with torch.cuda.device(index):
-            return _call(fn, where, index, *args)
+    """Calls a C entry on the current stream of device `index`, the current one; args
+    are its arguments up to the error word and the stream. The error word is the one
+    of (device, stream), moe.layer_error_word."""
     stream = torch._C._cuda_getCurrentRawStream(index)
     status = fn(_PACK[len(args) + 2](*args, _workspaces.header_ptr(index, stream), stream))
     if status:
@@ -147,8 +144,8 @@ def _output(out: Optional[torch.Tensor], residual: Optional[torch.Tensor], M: in
     return out, ld, _rows(residual, "residual")
 
 
-# Sizes of workspaces by sizes of the call (and its device): asking the library each
-# time is a tenth of a one-token call.
+# Sizes of workspaces by sizes of the call and its device, which is the current one:
+# asking the library each time is a tenth of a one-token call.
 @functools.lru_cache(maxsize=4096)
 def _linear_bytes(index: int, M: int, N: int, K: int, gate_up: int) -> int:
     return _lib.lib().b200moe_linear_workspace_size(M, N, K, 1, gate_up)
@@ -179,6 +176,9 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     N; K % 128 == 0. out may be residual itself and overlaps no other input. See
     b200moe_linear."""
     index = _device_of(x, weight, weight_scale, x_scale, residual, out)
+    if torch.cuda.current_device() != index:  # plans, sizes and launches go by the current device
+        with torch.cuda.device(index):
+            return fp8_block_linear(x, weight, weight_scale, x_scale, residual, out, out_dtype)
     if out_dtype is not _BF16 and out_dtype is not _F32:
         raise NotImplementedError("out_dtype must be bf16 or float32")
     x, x_scale, M, K, ld_x, ld_s = _input(x, x_scale)
@@ -207,6 +207,9 @@ def fp8_gate_up(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, x_s
     up j). x as in fp8_block_linear; w13 (2I, H) fp8 e4m3, w13_scale (2I/128,
     H/128) f32; I % 128 == 0. See b200moe_gate_up."""
     index = _device_of(x, w13, w13_scale, x_scale)
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return fp8_gate_up(x, w13, w13_scale, x_scale)
     x, x_scale, M, H, ld_x, ld_s = _input(x, x_scale)
     dev = x.device
     ld_w, w13_scale, N = _weight(w13, w13_scale, H, "w13")
@@ -237,6 +240,9 @@ def fp8_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: tor
     (2I, H), then fp8_block_linear with w2 (H, I), in one call (same bits).
     out may be residual or x itself. See b200moe_mlp."""
     index = _device_of(x, w13, w13_scale, w2, w2_scale, x_scale, residual, out)
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return fp8_mlp(x, w13, w13_scale, w2, w2_scale, x_scale, residual, out)
     x, x_scale, M, H, ld_x, ld_s = _input(x, x_scale)
     dev = x.device
     ld13, w13_scale, N = _weight(w13, w13_scale, H, "w13")
