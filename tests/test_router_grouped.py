@@ -46,3 +46,16 @@ def test_python_arguments():
             moe._check_groups(*pair)
     with pytest.raises(ValueError, match="CUDA"):
         moe.select_experts(torch.zeros(2, 8), 2, num_expert_group=2, topk_group=1)
+
+
+def test_router_bias_covers_the_experts():
+    """A bias may be longer than the experts (padded); the kernels read the first ones."""
+    long = torch.arange(96, dtype=torch.float32)
+    got = moe._router_bias(long, torch.device("cpu"), long.get_device(), 64)
+    assert torch.equal(got[:64], long[:64])
+    odd = torch.arange(192, dtype=torch.bfloat16)[::2]
+    got = moe._router_bias(odd, torch.device("cpu"), None, 64)
+    assert got.dtype == torch.float32 and got.is_contiguous() and torch.equal(got[:64], odd[:64].float())
+    assert moe._router_bias(None, torch.device("cpu"), None, 64) is None
+    with pytest.raises(ValueError, match="64"):
+        moe._router_bias(long[:63], torch.device("cpu"), None, 64)

@@ -169,11 +169,11 @@ def _check_groups(num_expert_group: Optional[int], topk_group: Optional[int]) ->
 
 def _router_bias(bias: Optional[torch.Tensor], dev: torch.device, index: Optional[int],
                  E: int) -> Optional[torch.Tensor]:
-    """The correction bias as the kernels read it: E contiguous f32 on the device
-    (index: the device's, None if unknown)."""
+    """The correction bias as the kernels read it: E contiguous f32 on the device, or
+    more, of which the first E count (index: the device's, None if unknown)."""
     if bias is None:
         return None
-    if bias.numel() != E:
+    if bias.numel() < E:
         raise ValueError(f"correction_bias must have {E} entries, got {tuple(bias.shape)}")
     if bias.dtype is torch.float32 and bias.get_device() == index and bias.is_contiguous():
         return bias
