@@ -1,6 +1,7 @@
 """Refusals of the dense FP8 products (fp8_block_linear, fp8_gate_up, fp8_mlp):
 checked on the host before anything is launched, so no GPU is needed."""
 import struct
+from pathlib import Path
 
 import pytest
 import torch
@@ -218,3 +219,13 @@ def test_everything_is_asked_on_the_tensors_device(monkeypatch):
     assert dense._linear_bytes(1, 3000, 512, 256, 0) == 512
     dense._linear_bytes.cache_clear()
     dense._mlp_bytes.cache_clear()
+
+
+@pytest.mark.parametrize("name", ["dense_common.cuh", "dense_split.cuh", "dense_tok.cuh", "dense_pair.cuh",
+                                  "rowops.cuh"])
+def test_inputs_are_not_read_through_the_read_only_path(name):
+    """Kernels that start before the one ahead of them has ended (programmatic
+    launch) may not read what it writes as memory nobody writes."""
+    src = (Path(dense.__file__).parent / "csrc" / name).read_text()
+    code = "\n".join(line.split("//")[0] for line in src.splitlines())
+    assert "__ldg" not in code and "ld.global.nc" not in code and "__restrict__" not in code

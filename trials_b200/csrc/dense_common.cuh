@@ -1,4 +1,9 @@
 // Parts shared by the dense FP8 block-scaled product kernels.
+//
+// Rows, scales and residuals are read with plain loads, not through the read-only path
+// (__ldg): under programmatic launch the kernel that writes them can still be running
+// when this one has started, and that path is for memory that nobody writes while the
+// kernel lives.
 #pragma once
 
 #include "common.cuh"

@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(DensePairCfg<EPI>::THREADS, 1)
       float acc[C::COLS];
 #pragma unroll
       for (int j = 0; j < C::COLS; ++j) acc[j] = 0.f;
-      float sc_next = __ldg(xsr) * __ldg(wsr);
+      float sc_next = *xsr * *wsr;
       // The residual is asked for here although the tile before has just been stored: a
       // branch for it in the loop, after the first K block, slowed every K block (2048 x
       // 7168 x 18432: 337 us against 316; 5772 x 7424 x 768 with its six: 60.5, here 63).
@@ -300,8 +300,8 @@ __global__ void __launch_bounds__(DensePairCfg<EPI>::THREADS, 1)
         const float sc = sc_next;
         float xs_n = 0.f, ws_n = 0.f;
         if (kb + 1 < NKB) {
-          xs_n = __ldg(xsr + kb + 1);
-          ws_n = __ldg(wsr + kb + 1);
+          xs_n = xsr[kb + 1];
+          ws_n = wsr[kb + 1];
         }
         if (*abort_flag || !mbar_wait_bounded(&tfull[buf], bphase, p.timeout_ns)) {
           ok = false;

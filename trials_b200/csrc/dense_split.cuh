@@ -223,8 +223,8 @@ __global__ void __launch_bounds__(DenseSplitCfg<T>::THREADS, 2)
         const int t = g / nkb, kb = g - t * nkb;
         raw[u] = make_uint4(0, 0, 0, 0);
         if (g < total)
-          raw[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.xb) +
-                                                        (int64_t)(t0 + t) * p.ld_xb + (kb0 + kb) * 128 + sub * 8));
+          raw[u] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.xb) +
+                                                   (int64_t)(t0 + t) * p.ld_xb + (kb0 + kb) * 128 + sub * 8);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -251,16 +251,30 @@ __global__ void __launch_bounds__(DenseSplitCfg<T>::THREADS, 2)
         if (g < total) {
           *reinterpret_cast<uint2*>(xq + kb * tt * 128 + t * 128 + (((sub >> 1) ^ (t & 7)) << 4) + (sub & 1) * 8) =
               make_uint2(w[0], w[1]);
-          if (sub == 0) sx[kb * tt + t] = scale * __ldg(wsr + kb);
+          if (sub == 0) sx[kb * tt + t] = scale * wsr[kb];
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(xfull);
     } else {
-      for (int i = tid; i < nkb * live; i += C::EW * 32) {
-        const int t = i / nkb, kb = i - t * nkb;  // consecutive threads: consecutive K blocks of one token
-        sx[kb * tt + t] = __ldg(p.xs + (int64_t)(t0 + t) * p.ld_xs + kb0 + kb) * __ldg(wsr + kb);
+      // Consecutive threads: consecutive K blocks of one token; the loads of eight products
+      // go out together, as none passes a store that may alias it.
+      constexpr int U = 8, STEP = C::EW * 32;
+      const int total = nkb * live;
+      for (int i0 = tid; i0 < total; i0 += U * STEP) {
+        float a[U], b[U];
+        int at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + u * STEP, t = i / nkb, kb = i - t * nkb;
+          at[u] = i < total ? kb * tt + t : -1;
+          a[u] = i < total ? p.xs[(int64_t)(t0 + t) * p.ld_xs + kb0 + kb] : 0.f;
+          b[u] = i < total ? wsr[kb] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (at[u] >= 0) sx[at[u]] = a[u] * b[u];
       }
     }
     named_bar_sync(1, C::EW * 32);

@@ -194,13 +194,13 @@ __global__ void __launch_bounds__(DenseTokCfg<TN>::THREADS, 1)
     for (int j = 0; j < C::COLS; ++j) acc[j] = 0.f;
     int buf = 0;
     uint32_t bphase = 0;
-    float sc_next = __ldg(xsr) * __ldg(wsr);
+    float sc_next = *xsr * *wsr;
     for (int kb = 0; kb < nkb; ++kb) {
       const float sc = sc_next;
       float xs_n = 0.f, ws_n = 0.f;
       if (kb + 1 < nkb) {
-        xs_n = __ldg(xsr + kb + 1);
-        ws_n = __ldg(wsr + kb + 1);
+        xs_n = xsr[kb + 1];
+        ws_n = wsr[kb + 1];
       }
       if (*abort_flag || !mbar_wait_bounded(&tfull[buf], bphase, p.timeout_ns)) {
         atomicOr(p.err, ERR_DEV_TIMEOUT);

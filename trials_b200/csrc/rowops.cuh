@@ -13,9 +13,12 @@ constexpr int kQuantSegSteps = 4;
 constexpr int kQuantSegCols = 256 * kQuantSegSteps;
 
 __device__ __forceinline__ int32_t ld_index(const QuantArgs& a, const int32_t* p) {
-  return a.meta_l2 ? __ldcg(p) : __ldg(p);
+  return a.meta_l2 ? __ldcg(p) : *p;
 }
 
+// Inputs are read with plain loads and not through the read-only path (__ldg), as
+// under programmatic launch the kernel that writes them may overlap this one.
+//
 // One warp: launch row `row` of `a` (see QuantArgs), columns seg0 .. seg0+1023.
 // Each lane converts 8 consecutive bf16 per 16-byte load, a half-warp covers
 // one 128-column group, and the warp issues the loads of its four 256-column
@@ -47,11 +50,11 @@ __device__ __forceinline__ void quant_row_segment(const QuantArgs& a, int64_t ro
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int64_t b = seg0 + lane * 16 + i * 512;
-      if (b < seg_end) v[i] = __ldg(reinterpret_cast<const uint4*>(sq + b));
+      if (b < seg_end) v[i] = *reinterpret_cast<const uint4*>(sq + b);
     }
     const int64_t g = (seg0 >> 7) + lane;
     const bool gs = lane < kQuantSegCols / 128 && g * 128 < seg_end;
-    const float sv = gs ? __ldg(&a.xs[src * a.ldxs + g]) : 0.f;
+    const float sv = gs ? a.xs[src * a.ldxs + g] : 0.f;
     auto put = [&](int64_t d) {
       uint8_t* qr = a.q + d * a.ldq;
 #pragma unroll
@@ -80,7 +83,7 @@ __device__ __forceinline__ void quant_row_segment(const QuantArgs& a, int64_t ro
 #pragma unroll
   for (int i = 0; i < kQuantSegSteps; ++i) {
     const int64_t c = seg0 + i * 256 + lane * 8;
-    raw[i] = c < seg_end ? __ldg(reinterpret_cast<const uint4*>(xr + c)) : make_uint4(0, 0, 0, 0);
+    raw[i] = c < seg_end ? *reinterpret_cast<const uint4*>(xr + c) : make_uint4(0, 0, 0, 0);
   }
   uint2 packed[kQuantSegSteps];
   float scl[kQuantSegSteps];
