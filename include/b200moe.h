@@ -625,7 +625,7 @@ B200MOE_API int b200moe_combine_reduce(const void* out_pair, const int32_t* slot
  * (ceil(N/128), K/128) contiguous. residual (M, N) bf16 or NULL; it may be out
  * itself (the same address and stride, with bf16 out). Otherwise out overlaps no
  * input. Any M >= 0 and N >= 1; K % 128 == 0. Activation and weight rows start
- * 16-byte aligned.
+ * 16-byte aligned, everything else at a multiple of its element's size.
  *
  * b200moe_gate_up: the product with w13 (2I, H), gate/up rows interleaved (row
  * 2j = gate j, 2j+1 = up j) as in the layer, then silu(gate) * up in fp32,

@@ -229,3 +229,23 @@ def test_inputs_are_not_read_through_the_read_only_path(name):
     src = (Path(dense.__file__).parent / "csrc" / name).read_text()
     code = "\n".join(line.split("//")[0] for line in src.splitlines())
     assert "__ldg" not in code and "ld.global.nc" not in code and "__restrict__" not in code
+
+
+@pytest.mark.parametrize("off", [1, 2])
+def test_scales_and_words_must_be_aligned(off):
+    """A float or word at an address that is no multiple of 4 would fault on the GPU."""
+    assert linear(ws=P + off) == _lib.ERR_UNSUPPORTED
+    assert linear(x=None, xq=P, xs=P + off) == _lib.ERR_UNSUPPORTED
+    assert linear(err=P + off) == _lib.ERR_UNSUPPORTED
+
+    def gate_up(x=P, xq=None, xs=None, ws=P, s=1 << 40, err=P):
+        return call("b200moe_gate_up", x, xq, xs, 256, 2, 4, 256, 128, 1 << 30, 256, ws, 1 << 34, 128, s, 1, P,
+                    1 << 20, err, None)
+
+    def mlp(ws=P, w2s=P, err=P):
+        return call("b200moe_mlp", P, None, None, 256, 0, 4, 256, 128, 1 << 28, ws, 1 << 30, w2s, None, 0, 1 << 34, 256,
+                    P, 1 << 20, err, None)
+
+    for got in (gate_up(ws=P + off), gate_up(x=None, xq=P, xs=P + off), gate_up(s=P + off), gate_up(err=P + off),
+                mlp(ws=P + off), mlp(w2s=P + off), mlp(err=P + off)):
+        assert got == _lib.ERR_UNSUPPORTED

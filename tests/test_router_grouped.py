@@ -59,3 +59,8 @@ def test_router_bias_covers_the_experts():
     assert moe._router_bias(None, torch.device("cpu"), None, 64) is None
     with pytest.raises(ValueError, match="64"):
         moe._router_bias(long[:63], torch.device("cpu"), None, 64)
+
+
+@pytest.mark.parametrize("kw", [dict(logits=P + 2), dict(logits=P + 1), dict(bias=P + 2), dict(w=P + 1), dict(ids=P + 2)])
+def test_pointers_must_be_aligned(kw):
+    assert call(**kw) == _lib.ERR_UNSUPPORTED

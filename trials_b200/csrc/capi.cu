@@ -34,6 +34,7 @@ int cuda_status(cudaError_t e, const char* where) {
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
@@ -301,8 +302,8 @@ RouterArgs grouped_router(const void* logits, int logits_bf16, int num_experts, 
 }
 
 // The same plus the groups of group-limited routing.
-int check_router_grouped(const char* name, const void* logits, int64_t M, int num_experts, int num_groups,
-                         int topk_groups, int topk, int scoring, const float* correction_bias,
+int check_router_grouped(const char* name, const void* logits, int logits_bf16, int64_t M, int num_experts,
+                         int num_groups, int topk_groups, int topk, int scoring, const float* correction_bias,
                          const float* topk_weights, const int32_t* topk_ids) {
   const int st = check_router(name, logits, M, num_experts, topk, scoring, correction_bias, topk_weights, topk_ids);
   if (st) return st;
@@ -310,6 +311,9 @@ int check_router_grouped(const char* name, const void* logits, int64_t M, int nu
       topk > topk_groups * (num_experts / num_groups))
     return fail(B200MOE_ERR_INVALID_ARG, "%s: groups must split the experts evenly and the selected ones hold top-k",
                 name);
+  if (!aligned4(topk_weights) || !aligned4(topk_ids) || !aligned4(correction_bias) ||
+      (reinterpret_cast<uintptr_t>(logits) & (logits_bf16 ? 1 : 3)) != 0)
+    return fail(B200MOE_ERR_UNSUPPORTED, "%s: misaligned logits, bias or outputs", name);
   if (num_groups > kRouterMaxGroups) return fail(B200MOE_ERR_UNSUPPORTED, "%s: at most 32 groups", name);
   return B200MOE_OK;
 }
@@ -599,8 +603,8 @@ int b200moe_route_logits_grouped(const void* logits, int logits_bf16, int64_t M,
                                  int32_t* chunk_row0, int32_t* chunk_rows, int64_t chunks_capacity, int32_t* n_chunks,
                                  int32_t* num_rows, int32_t* slot_pos, int32_t* chunk_ready, int32_t* route_scratch,
                                  int64_t route_scratch_ints, int32_t* err_word, void* stream) {
-  int st = check_router_grouped("b200moe_route_logits_grouped", logits, M, num_experts, num_groups, topk_groups, topk,
-                                scoring, correction_bias, topk_weights, topk_ids);
+  int st = check_router_grouped("b200moe_route_logits_grouped", logits, logits_bf16, M, num_experts, num_groups,
+                                topk_groups, topk, scoring, correction_bias, topk_weights, topk_ids);
   if (st) return st;
   const RouterArgs r = grouped_router(logits, logits_bf16, num_experts, num_groups, topk_groups, topk, scoring,
                                       correction_bias, renormalize, scaling, topk_weights, topk_ids);
@@ -1189,8 +1193,8 @@ int b200moe_layer_logits_grouped(const void* hidden, int64_t M, int64_t H, int64
                                  const int32_t* expert_map, int num_local_experts, float* topk_weights,
                                  int32_t* topk_ids, void* out, void* workspace, size_t workspace_bytes, void* stream) {
   if (!hidden && M > 0) return fail(B200MOE_ERR_INVALID_ARG, "b200moe_layer_logits_grouped: null hidden%s");
-  int st = check_router_grouped("b200moe_layer_logits_grouped", router_logits, M, num_experts, num_groups, topk_groups,
-                                topk, scoring, correction_bias, topk_weights, topk_ids);
+  int st = check_router_grouped("b200moe_layer_logits_grouped", router_logits, logits_bf16, M, num_experts, num_groups,
+                                topk_groups, topk, scoring, correction_bias, topk_weights, topk_ids);
   if (st) return st;
   const RouterArgs r = grouped_router(router_logits, logits_bf16, num_experts, num_groups, topk_groups, topk, scoring,
                                       correction_bias, renormalize, scaling, topk_weights, topk_ids);
@@ -1212,8 +1216,8 @@ int b200moe_layer_call(const b200moe_layer_args* a) {
   RouterArgs r{};
   if (logits) {
     const int G = int_size(a->num_groups), T = int_size(a->topk_groups);
-    const int st = grouped ? check_router_grouped(name, a->router_logits, a->M, E, G, T, k, scoring, a->correction_bias,
-                                                  a->topk_weights, a->topk_ids)
+    const int st = grouped ? check_router_grouped(name, a->router_logits, a->logits_bf16 != 0, a->M, E, G, T, k,
+                                                  scoring, a->correction_bias, a->topk_weights, a->topk_ids)
                            : check_router(name, a->router_logits, a->M, E, k, scoring, a->correction_bias,
                                           a->topk_weights, a->topk_ids);
     if (st) return st;
@@ -1511,8 +1515,8 @@ int b200moe_router_topk_grouped(const b200moe_router_grouped_args* a) {
   if (!a) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
   const int E = int_size(a->num_experts), G = int_size(a->num_groups), T = int_size(a->topk_groups);
   const int k = int_size(a->topk), scoring = int_size(a->scoring);
-  const int st = check_router_grouped(name, a->logits, a->M, E, G, T, k, scoring, a->correction_bias, a->topk_weights,
-                                      a->topk_ids);
+  const int st = check_router_grouped(name, a->logits, a->logits_bf16 != 0, a->M, E, G, T, k, scoring,
+                                      a->correction_bias, a->topk_weights, a->topk_ids);
   if (st) return st;
   const RouterArgs r = grouped_router(a->logits, a->logits_bf16 != 0, E, G, T, k, scoring, a->correction_bias,
                                       a->renormalize != 0, (float)a->scaling, a->topk_weights, a->topk_ids);
@@ -1575,6 +1579,8 @@ int check_dense(const char* name, const DenseInput& in, int64_t M, int64_t N, in
   if (!aligned16(w) || ld_w % 16 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "%s: weight rows must be 16-byte aligned", name);
   const bool rows_ok = in.x ? (aligned16(in.x) && in.ld_x % 8 == 0) : (aligned16(in.q) && in.ld_x % 16 == 0);
   if (M > 0 && !rows_ok) return fail(B200MOE_ERR_UNSUPPORTED, "%s: activation rows must be 16-byte aligned", name);
+  if (!aligned4(w_scale) || (in.q && !aligned4(in.s)) || !aligned4(err_word))
+    return fail(B200MOE_ERR_UNSUPPORTED, "%s: misaligned scales or error word", name);
   return B200MOE_OK;
 }
 
@@ -1725,6 +1731,7 @@ int b200moe_gate_up(const b200moe_gate_up_args* a) {
   if (M > 0 && (!a->q || !a->s || a->ld_q < I || a->ld_s < I / 128))
     return fail(B200MOE_ERR_INVALID_ARG, "%s: bad output", name);
   if (I % 128 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "%s: I must be a multiple of 128", name);
+  if (!aligned4(a->s)) return fail(B200MOE_ERR_UNSUPPORTED, "%s: misaligned scales", name);
   if (!aligned16(a->q) || a->ld_q % 16 != 0)
     return fail(B200MOE_ERR_UNSUPPORTED, "%s: output rows must be 16-byte aligned", name);
   if (M == 0) return B200MOE_OK;
@@ -1783,6 +1790,7 @@ int b200moe_mlp(const b200moe_mlp_args* a) {
   if (I % 128 != 0) return fail(B200MOE_ERR_UNSUPPORTED, "%s: I must be a multiple of 128", name);
   if (!a->w2 || !a->w2_scale) return fail(B200MOE_ERR_INVALID_ARG, "%s: bad argument", name);
   if (!aligned16(a->w2)) return fail(B200MOE_ERR_UNSUPPORTED, "%s: weight rows must be 16-byte aligned", name);
+  if (!aligned4(a->w2_scale)) return fail(B200MOE_ERR_UNSUPPORTED, "%s: misaligned scales or error word", name);
   DenseParams p{};
   st = check_dense_out(name, M, H, a->residual, a->ld_res, a->out, a->ld_out, 0, p);
   if (st) return st;
