@@ -107,7 +107,7 @@ B200MOE_API int b200moe_router_topk(const void* logits, int logits_bf16, int64_t
  * that exact arithmetic on the given values makes. NaN logits count as -inf
  * (score 0; without a bias selected last, in id order); a +inf logit of a
  * softmax shares the whole weight with its equals; when renormalize is set and
- * the selected scores sum to 0, the weights are 0. num_experts % num_groups
+ * the selected scores are all 0 (sigmoids: in 64 bits, below -709), the weights are 0. num_experts % num_groups
  * == 0, topk <= topk_groups * num_experts / num_groups, at most 32 groups. The
  * reference runs one group (measure_xcd_imbalance.py:50-55); more are what
  * other checkpoints of this layer's geometries route with. The arguments come in

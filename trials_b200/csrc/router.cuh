@@ -150,7 +150,7 @@ __device__ __forceinline__ void route_token_warp(const RouterArgs& r, int64_t t,
 //   group score: without a bias the largest c, with one the sum of the two
 //   largest; best groups, then best experts, equal values lower index first.
 // NaN logits count as -inf (score 0), NaN c as -inf; a row whose selected
-// scores sum to 0 has weights 0 when renormalised.
+// scores are all 0 has weights 0 when renormalised.
 //
 // The selection is the one exact arithmetic on the given f32 (bf16) values
 // makes. Without a bias s is monotone in x, so x itself is compared. With one, c
@@ -345,6 +345,15 @@ static __device__ __noinline__ int grouped_order_f64(const RouterArgs r, int64_t
     rank += (other > c || (other == c && oid < id)) ? 1 : 0;
   }
   return rank;
+}
+
+// This lane's sigmoid over the sum of those of the lanes that are `mine`, in fp64; 0 if
+// they are all 0 there.
+static __device__ __noinline__ float grouped_ratio_f64(float v, bool mine) {
+  const double s = mine && v == v ? 1.0 / (1.0 + exp(-(double)v)) : 0.0;
+  double sum = s;
+  for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum > 0.0 ? (float)(s / sum) : 0.f;
 }
 
 // Descending order of N keys (N = 8: a 19-exchange network; else halves, merged).
@@ -548,13 +557,16 @@ __device__ __forceinline__ void route_token_grouped(const RouterArgs& r, int64_t
   if (many) my_id = grouped_select_f64<PER>(r, t, taken, lane);  // warp-uniform
   else if (order) place = grouped_order_f64(r, t, my_id, n, lane);
   const bool mine = place < topk && (many || lane < n);
-  float w = 0.f;
+  float w = 0.f, v = 0.f;
   if (mine) {
-    const float v = router_logit(r, t, my_id);
+    v = router_logit(r, t, my_id);
     if (r.scoring == 1) w = v == v ? 1.0f / (1.0f + expf(-v)) : 0.f;
     else if (v == v && v != -INFINITY) w = v == xmax ? 1.0f : expf(v - xmax);
   }
-  if (r.renormalize) {
+  // Sigmoids that fp32 does not hold although fp64 does still have a ratio.
+  if (r.scoring == 1 && r.renormalize && __any_sync(0xffffffffu, v < -87.0f && v > -710.0f)) {
+    w = grouped_ratio_f64(v, mine);
+  } else if (r.renormalize) {
     float sum = w;
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
