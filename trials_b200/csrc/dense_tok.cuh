@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(DenseTokCfg<TN>::THREADS, 1)
       sc_next = xs_n * ws_n;
     }
     // The last partial is out of the tensor core, so the tiles are free: this
-    // CTA's sums, rows of 256 columns in 16-byte pieces swizzled by row.
+    // CTA's sums, rows of TN columns in 16-byte pieces swizzled by row.
     if (live) {
 #pragma unroll
       for (int c = 0; c < C::COLS / 4; ++c)
