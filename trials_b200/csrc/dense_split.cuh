@@ -217,11 +217,13 @@ __global__ void __launch_bounds__(DenseSplitCfg<T>::THREADS, 2)
       const int hw = tid >> 4, sub = tid & 15;
       const int total = live * nkb;
       uint4 raw[U];
+      float wv[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int g = u * C::EW * 2 + hw;
         const int t = g / nkb, kb = g - t * nkb;
         raw[u] = make_uint4(0, 0, 0, 0);
+        wv[u] = g < total ? wsr[kb] : 0.f;
         if (g < total)
           raw[u] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.xb) +
                                                    (int64_t)(t0 + t) * p.ld_xb + (kb0 + kb) * 128 + sub * 8);
@@ -251,7 +253,7 @@ __global__ void __launch_bounds__(DenseSplitCfg<T>::THREADS, 2)
         if (g < total) {
           *reinterpret_cast<uint2*>(xq + kb * tt * 128 + t * 128 + (((sub >> 1) ^ (t & 7)) << 4) + (sub & 1) * 8) =
               make_uint2(w[0], w[1]);
-          if (sub == 0) sx[kb * tt + t] = scale * wsr[kb];
+          if (sub == 0) sx[kb * tt + t] = scale * wv[u];
         }
       }
       fence_proxy_async_smem();
@@ -261,16 +263,30 @@ __global__ void __launch_bounds__(DenseSplitCfg<T>::THREADS, 2)
       // Consecutive threads: consecutive K blocks of one token; the loads of eight products
       // go out together, as none passes a store that may alias it.
       constexpr int U = 8, STEP = C::EW * 32;
-      const int total = nkb * live;
-      for (int i0 = tid; i0 < total; i0 += U * STEP) {
+      // tid / nkb and STEP / nkb: (n + 0.5) / nkb is 0.5 / nkb away from every integer, far
+      // more than the rounding of so small a number.
+      const float inv = __fdividef(1.0f, (float)nkb);
+      const int dt = (int)(((float)STEP + 0.5f) * inv), dk = STEP - dt * nkb;
+      int t = (int)(((float)tid + 0.5f) * inv), kb = tid - t * nkb;
+      for (int i0 = 0; i0 < nkb * live; i0 += U * STEP) {
         float a[U], b[U];
         int at[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int i = i0 + u * STEP, t = i / nkb, kb = i - t * nkb;
-          at[u] = i < total ? kb * tt + t : -1;
-          a[u] = i < total ? p.xs[(int64_t)(t0 + t) * p.ld_xs + kb0 + kb] : 0.f;
-          b[u] = i < total ? wsr[kb] : 0.f;
+          at[u] = -1;
+          if (i0 + u * STEP < nkb * live) {  // uniform
+            if (t < live) {
+              at[u] = kb * tt + t;
+              a[u] = p.xs[(int64_t)(t0 + t) * p.ld_xs + kb0 + kb];
+              b[u] = wsr[kb];
+            }
+            t += dt;
+            kb += dk;
+            if (kb >= nkb) {
+              kb -= nkb;
+              ++t;
+            }
+          }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
