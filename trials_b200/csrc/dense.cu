@@ -81,20 +81,19 @@ cudaError_t launch_tok_dense(const DensePlan& pl, const CUtensorMap& tm_x, const
                             early_w && B200MOE_PDL ? 1 : 0);
 }
 
-// Shared memory of a CTA of the split kernel. A CTA that waits for TMEM holds its
-// place in its cluster, and two clusters that wait for each other's TMEM never
-// end: so the CTAs that fit on an SM together (of one launch or of several
-// streams) must also have TMEM enough. The sizes see to it: at most two CTAs of
-// this kernel, with half of the TMEM each (3 x 79 KB > 228 KB, 1 KB of each the
-// system's), and none beside a CTA that takes all of it, as the token-major, pair
-// and expert kernels do with 194 KB and more. That is said of this library's kernels: a
-// clustered kernel of another one that takes more than half of the TMEM with less than
-// 148 KB can meet a split CTA on an SM, and neither the allocation nor a cluster barrier
-// has a time limit. (113 KB for every call would leave such kernels 113 KB and measured
-// slower: 8 tokens of 300 x 256 4.1 us against 3.8, the expert on 64 tokens of 2048 x 768
-// 14.4 against 13.7.)
-constexpr int kSplitSmem = 113 * 1024, kSplitSmemMin = 78 * 1024;
-constexpr bool alone(int smem) { return smem + kSplitSmemMin + 2 * 1024 > 228 * 1024; }
+// Shared memory of a CTA of the split kernel, whatever it needs of it. A CTA that waits
+// for TMEM holds its place in its cluster, and two clusters that wait for each other's
+// TMEM never end: so the CTAs that fit on an SM together (of one launch or of several
+// streams) must also have TMEM enough. The size sees to it: two CTAs of this kernel,
+// with half of the TMEM each, fill the SM (2 x 114 KB = 228, 1 KB of each the system's),
+// and none stands beside a CTA that takes all of it, as the token-major, pair and expert
+// kernels do with 194 KB and more. That is said of this library's kernels: a clustered
+// kernel of another one that takes more than half of the TMEM with 113 KB at most can
+// meet a split CTA on an SM, and neither the allocation nor a cluster barrier has a time
+// limit. (78 KB where that is enough, which leaves other kernels 148, measured no faster.)
+constexpr int kSplitSmem = 113 * 1024;
+constexpr bool alone(int smem) { return smem + kSplitSmem + 2 * 1024 > 228 * 1024; }
+static_assert(2 * (kSplitSmem + 1024) <= 228 * 1024 && alone(kSplitSmem + 1), "two split CTAs fill an SM");
 static_assert(alone(DenseTokCfg<256>::SMEM_BYTES) && alone(DenseTokCfg<128>::SMEM_BYTES) &&
                   alone(DensePairCfg<DENSE_OUT>::SMEM_BYTES) && alone(DensePairCfg<DENSE_SILU>::SMEM_BYTES) &&
                   alone(GemmCfg<32, 1>::SMEM_BYTES) && alone(GemmCfg<64, 1>::SMEM_BYTES) &&
@@ -124,8 +123,6 @@ cudaError_t launch_split_dense(const DensePlan& pl, const CUtensorMap& tm_x, con
   const int nkb = ((p.K >> 7) + pl.splits - 1) / pl.splits;
   const int nstage = split_stages<T>(nkb, pl.tokens, QX);
   if (nstage == 0) return cudaErrorInvalidValue;
-  int smem = C::smem_bytes(nstage, nkb, pl.tokens, QX);
-  if (smem < kSplitSmemMin) smem = kSplitSmemMin;
   cudaError_t err = allow_smem(kernel, kSplitSmem, current_device(), done);
   if (err != cudaSuccess) return err;
   const int R = HALVES * pl.splits;
@@ -134,7 +131,7 @@ cudaError_t launch_split_dense(const DensePlan& pl, const CUtensorMap& tm_x, con
   cluster_launch(cfg, attr, R,
                  dim3((unsigned)((p.N + 128 * HALVES - 1) / (128 * HALVES) * R),
                       (unsigned)((p.M + pl.tokens - 1) / pl.tokens), 1),
-                 C::THREADS, smem, stream);
+                 C::THREADS, kSplitSmem, stream);
   return cudaLaunchKernelEx(&cfg, kernel, tm_x, tm_w, p, pl.splits, pl.tokens, nstage,
                             early_w && B200MOE_PDL ? 1 : 0);
 }
