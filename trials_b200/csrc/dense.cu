@@ -219,10 +219,15 @@ DensePlan split_plan(int epi, int64_t M, int64_t N, int nkb, bool x_bf16) {
   const int T = tt <= 16 ? 16 : (tt <= 32 ? 32 : 64);
   const int64_t units = (N + 128 * halves - 1) / (128 * halves) * n_tt;
   const int sms = sm_count_of(current_device());
-  // CTAs along K, at least two K blocks each, four where 8 CTAs would exchange the sums of
-  // more than 32 tokens (64 of 2304 x 2048: 6.4 us with 4 CTAs, 7.7 with 8).
+  // CTAs along K, at least two K blocks each. Where 8 would exchange the sums of more than
+  // 32 tokens they have an SM each, or at least four: two of them on an SM measured slower
+  // than 4 with twice the K blocks (64 tokens of K = 2048, 8 and 4 CTAs along it: N = 512
+  // 5.1 us and 5.8, 1536 5.6 and 6.0, 1920 6.0 and 6.3, then 2048 7.0 and 6.4, 2304 7.7
+  // and 6.6; of K = 3584: 1536 6.9 and 7.5, 1920 7.1 and 7.6, 2048 8.5
+  // and 7.7; 40 tokens of 1920 x 2048 5.3 and 5.8, of 2048 x 2048 6.0 and 5.8).
   int s = 8 / halves;
-  while (s > 1 && s * (T == 64 && M <= 64 && s == 8 ? 4 : 2) > nkb) s /= 2;
+  auto fewest = [&](int k) { return T == 64 && M <= 64 && k == 8 && units > resident_tok(8) ? 4 : 2; };
+  while (s > 1 && s * fewest(s) > nkb) s /= 2;
   if (M > 64) {
     // More than 64 tokens read the weights more than once, which pays while the tiles'
     // clusters run in one wave, two CTAs an SM less what clusters cannot use (gate/up of
