@@ -35,6 +35,21 @@ def test_rows_across_batch_sizes(cuda_device, N, K):
             assert ((part - whole[first:first + m]).abs() <= bound[first:first + m]).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(300, 12544, 512), (600, 15104, 256), (1100, 32768, 256), (1100, 16381, 384)])
+def test_odd_numbers_of_token_tiles(cuda_device, M, N, K):
+    """From one round of tiles to many, with half of a pair's last tile empty."""
+    g = torch.Generator(device=cuda_device).manual_seed(M + N + K)
+    x = torch.randn(M, K, generator=g, device=cuda_device).to(torch.bfloat16)
+    w, ws = per_block_quant_fp8((torch.randn(N, K, generator=g, device=cuda_device) * K ** -0.5).to(torch.bfloat16))
+    xq, xs = per_token_group_quant_fp8(x)
+    a, b = values(xq, xs, 1), values(w, ws, 128)
+    bound = (256 + 2 * (K // 128) + 2) * U * (a.abs() @ b.abs().t())
+    got = fp8_block_linear(x, w, ws, out_dtype=torch.float32)
+    assert ((got.double() - a @ b.t()).abs() <= bound).all()
+    res = torch.randn(M, N, generator=g, device=cuda_device).to(torch.bfloat16)
+    assert torch.equal(fp8_block_linear(x, w, ws, residual=res), (got + res.float()).to(torch.bfloat16))
+
+
 def test_gate_up_rows_across_batch_sizes(cuda_device):
     """Scales within the bound of both products' errors (d silu(g) <= 1.1 dg; silu good
     to 2^-20), as in tests/test_gpu_dense.py, on each side."""

@@ -303,17 +303,28 @@ DensePlan dense_plan(int epi, int64_t M, int64_t N, int64_t K, bool x_bf16) {
   // Token-major tiles of 256 columns while a cluster of two or more CTAs can share each
   // (512 x 4096 x 6144: 20.9 us against 30.7 with pairs), unless two of them share so
   // few K blocks that their exchange costs more (gate/up 300 x 1024 x 2048, 8 K blocks:
-  // 11.5 against 10.0 with pairs; 300 x 2048 x 2048, 16: 13.4 and 13.8); then whichever
-  // takes fewer rounds, a K block of either costing about the same (89 tokens leave half
-  // of a pair's tile empty), and pairs if neither does (1024 x 4096 x 6144: 31.5 against
-  // 32.9; 2048: 59.5 against 64.3).
+  // 11.5 against 10.0 with pairs; 300 x 2048 x 2048, 16: 13.4 and 13.8). Then pairs unless
+  // they take more rounds (1024 x 4096 x 6144: 31.5 and token-major 32.9; 2048: 59.5 and
+  // 64.3), and with more rounds, as an odd number of 128-token tiles leaves half of a
+  // pair's tile empty, whichever takes less time. A token-major round, whose start and end
+  // nothing hides, measured 8.7 us and 0.48 a K block, one of the persistent pairs 2.0 and
+  // 0.52 and 1.6 more a launch, for products and gate/up alike, 2.5 here as rows that are
+  // not aligned cost pairs more (us token-major and with pairs; x N, K blocks, rounds:
+  //   300 x 12544, 32, 1 and 2: 25.5, 39.7    1100 x 8192, 32, 2 and 3: 49, 57
+  //   600 x 15104, 16, 2 and 3: 34.2, 33.1    600 x 15101, 16: 42.9, 46.6
+  //   1100 x 16384, 32, 4 and 5: 98, 94       1100 x 16381, 32: 115.5, 115.8
+  //   1100 x 32768, 16, 8 and 9: 136, 94      2100 x 36864, 56, 17 and 18: 643, 598
+  //   gate/up 4160 x 36864, 56, 33 and 34: 1400, 1195
+  //   4200 x 129280, 8, 113 and 117: 1447, 752). The bits are the same either way.
   using T = DenseTokCfg<256>;
   const int64_t n_nt = (N + T::TN - 1) / T::TN;
   const int64_t units = m_tiles * n_nt, pair_units = (M + 2 * T::TM - 1) / (2 * T::TM) * n_nt;
   const int s = most_splits(units);
   const int64_t rounds = (units + resident_tok(1) - 1) / resident_tok(1);
   const int64_t pair_rounds = (pair_units + resident_pairs() - 1) / resident_pairs();
-  if ((s == 1 || (s == 2 && nkb <= 8)) && rounds >= pair_rounds) {
+  const int64_t ns_tok = rounds * (8700 + 480 * (int64_t)nkb);
+  const int64_t ns_pair = 2500 + pair_rounds * (2000 + 520 * (int64_t)nkb);
+  if ((s == 1 || (s == 2 && nkb <= 8)) && (rounds >= pair_rounds || ns_pair <= ns_tok)) {
     pl.cfg = kDensePair;
     pl.splits = 1;
     pl.x_box_rows = DensePairCfg<DENSE_OUT>::TM;
