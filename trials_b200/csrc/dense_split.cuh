@@ -30,10 +30,13 @@
 
 namespace b200moe {
 
-// Most (token, K block) groups a CTA quantises itself (QX). Up to 24 it is faster than
-// the launch that quantises every row once (one token of 6144 x 2048 6.5 us, 8.0); at 48
-// (4 of 4096 x 6144) 11.4 us on the GPU against 10.8 but 12.1 a call against 15.7, at 64
-// (16 of 6144 x 2048) 9.8 against 8.4.
+// Most (token, K block) groups a CTA quantises itself (QX): up to 48 it is faster than the
+// launch that quantises every row once (us inside a graph, here and with the launch: one
+// token of 6144 x 2048 6.5 and 8.0; 36 and 48 groups, 3 and 4 tokens of 4096 x 6144, 10.2
+// and 10.7, 10.5 and 10.7; 32, 8 of 4096 x 2048, 6.8 and 7.3; 48, 12 of 6144 x 2048, 8.0
+// and 8.2; 32, 16 of 1024 x 2048, 5.1 and 5.9; gate/up, 36, 3 of 6144 x 2048 10.7 and 11.3;
+// an eager call of 4 x 4096 x 6144 10.2 and 14.2). At 64 (16 of 6144 x 2048) it was 9.8
+// against 8.4.
 constexpr int kQuantGroups = 48;
 
 template <int T_>
