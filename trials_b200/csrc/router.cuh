@@ -168,12 +168,12 @@ __device__ __forceinline__ void route_token_warp(const RouterArgs& r, int64_t t,
 // has a power of two of lanes to itself, the last of them not always full, wherever
 // that leaves no lane more than 32 (5,580 tokens of 312 experts in 4 groups with a
 // bias: 15.9 us, 23.5 with lanes across groups). What bounds it is the number of
-// instructions a warp issues, 880 with a bias (issue slots 69% busy, the integer
+// instructions a warp issues, 889 with a bias (issue slots 69% busy, the integer
 // pipe 80%; fewer registers for more warps measured 0-8% slower): a round of the
 // selection is one redux and one ballot on the lanes' best keys, the lists behind
-// them sorted once. 8,192 tokens of 256 experts in 8 groups: 10.9 us with a bias
+// them sorted once. 8,192 tokens of 256 experts in 8 groups: 11.2 us with a bias
 // (25.7 with every value compared in turn and each close token redone in fp64),
-// 8.7 without.
+// 8.9 without.
 // ---------------------------------------------------------------------------
 constexpr int kRouterMaxGroups = 32;
 // Bound of the error of two values c together: the sigmoid's (exp 6e-8 where its
