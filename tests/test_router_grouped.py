@@ -4,7 +4,7 @@ import struct
 import pytest
 import torch
 
-from trials_b200 import _lib, moe
+from trials_b200 import _lib, moe, stages
 
 P = 256
 
@@ -64,3 +64,43 @@ def test_router_bias_covers_the_experts():
 @pytest.mark.parametrize("kw", [dict(logits=P + 2), dict(logits=P + 1), dict(bias=P + 2), dict(w=P + 1), dict(ids=P + 2)])
 def test_pointers_must_be_aligned(kw):
     assert call(**kw) == _lib.ERR_UNSUPPORTED
+
+
+class Entered(Exception):
+    pass
+
+
+class OnDevice1:
+    """Stands for a tensor on a device that is not the current one."""
+    device = torch.device("cuda", 1)
+    dtype = torch.float32
+    shape = (4, 64)
+
+    def get_device(self):
+        return 1
+
+
+@pytest.mark.parametrize("groups", [{}, dict(num_expert_group=8, topk_group=4)])
+def test_calls_go_to_the_device_of_their_tensors(monkeypatch, groups):
+    class Guard:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            raise Entered(self.device)
+
+        def __exit__(self, *a):
+            pass
+
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    for module in (moe, stages):
+        monkeypatch.setattr(module, "_require_cuda", lambda *t: torch.device("cuda", 1))
+    x = OnDevice1()
+    for call in (lambda: moe.select_experts(x, 6, "sigmoid", **groups),
+                 lambda: moe.moe_layer_from_logits(x, x, x, x, x, x, 6, **groups),
+                 lambda: stages.route_logits(x, 6, 32, **groups),
+                 lambda: moe.moe_decode_megakernel_full(x, x, x, x, x, x, x)):
+        with pytest.raises(Entered) as e:
+            call()
+        assert getattr(e.value.args[0], "index", e.value.args[0]) == 1

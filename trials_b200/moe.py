@@ -195,6 +195,10 @@ def select_experts(router_logits: torch.Tensor, top_k: int, scoring_func: str = 
     index = router_logits.get_device()
     if index < 0:
         _require_cuda(router_logits)
+    if torch.cuda.current_device() != index:  # kernels launch on the current device
+        with torch.cuda.device(index):
+            return select_experts(router_logits, top_k, scoring_func, correction_bias, renormalize,
+                                  routed_scaling_factor, num_expert_group, topk_group)
     bf16 = router_logits.dtype is torch.bfloat16
     if not bf16 and router_logits.dtype is not torch.float32:
         raise NotImplementedError("router logits must be float32 or bfloat16")
@@ -208,10 +212,6 @@ def select_experts(router_logits: torch.Tensor, top_k: int, scoring_func: str = 
     w = torch.empty(M, top_k, dtype=torch.float32, device=dev)
     ids = torch.empty(M, top_k, dtype=torch.int32, device=dev)
     if grouped:
-        if torch.cuda.current_device() != index:
-            with torch.cuda.device(index):
-                return select_experts(logits, top_k, scoring_func, bias, renormalize, routed_scaling_factor,
-                                      num_expert_group, topk_group)
         # one packed struct: fourteen converted arguments cost 1.3 us more
         status = _lib.lib().b200moe_router_topk_grouped(_PACK_GROUPED(
             logits.data_ptr(), bf16, M, E, num_expert_group, topk_group, top_k, scoring,
@@ -308,6 +308,11 @@ def _layer_call(where: str, dev: torch.device, ws_bytes: int, rows, sizes, route
 
 def _run_layer(hidden, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids, expert_map, num_experts, out=None,
                a1_scale=None):
+    dev = _require_cuda(hidden)
+    if torch.cuda.current_device() != dev.index:  # kernels launch on the current device
+        with torch.cuda.device(dev):
+            return _run_layer(hidden, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids, expert_map, num_experts,
+                              out, a1_scale)
     dev, M, H, I, E_w = _check_layer_args(hidden, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids, a1_scale)
     topk = topk_ids.shape[1]
     if out is None:
@@ -439,6 +444,11 @@ def moe_layer_from_logits(hidden_states: torch.Tensor, router_logits: torch.Tens
     select_experts. shared_expert: (w13, w13_scale, w2, w2_scale) of a dense
     expert that every token passes through; dense.fp8_mlp adds it to out."""
     dev = _require_cuda(hidden_states, router_logits, w13_fp8, w2_fp8)
+    if torch.cuda.current_device() != dev.index:  # kernels launch on the current device
+        with torch.cuda.device(dev):
+            return moe_layer_from_logits(hidden_states, router_logits, w13_fp8, w13_scale, w2_fp8, w2_scale, top_k,
+                                         scoring_func, correction_bias, renormalize, routed_scaling_factor,
+                                         expert_map, num_expert_group, topk_group, shared_expert)
     grouped = _check_groups(num_expert_group, topk_group)
     if hidden_states.dtype != torch.bfloat16:
         raise NotImplementedError("moe_layer_from_logits takes bf16 hidden_states")

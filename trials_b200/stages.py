@@ -89,6 +89,11 @@ def route_logits(logits: torch.Tensor, top_k: int, tile_tokens: int, scoring_fun
     b200moe_route_logits_grouped) -> (Routing, topk_weights (M, k) f32, topk_ids
     (M, k) int32), equal to select_experts followed by route()."""
     dev = _require_cuda(logits)
+    if torch.cuda.current_device() != dev.index:  # kernels launch on the current device
+        with torch.cuda.device(dev):
+            return route_logits(logits, top_k, tile_tokens, scoring_func, correction_bias, renormalize,
+                                routed_scaling_factor, expert_map, num_local_experts, err, num_expert_group,
+                                topk_group)
     logits = logits.contiguous()
     M, E_router = logits.shape
     E = num_local_experts if expert_map is not None else E_router
