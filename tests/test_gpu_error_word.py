@@ -127,3 +127,23 @@ def test_word_under_capture(cuda_device):
     graph.replay()
     assert torch.equal(out, want)
     assert read_device_error(word) == 0
+
+
+@pytest.mark.parametrize("bit,left", [(_lib.DEVERR_TIMEOUT, 0), (_lib.DEVERR_BAD_EXPERT_ID, 5)])
+def test_counters_after_a_timeout(cuda_device, bit, left):
+    """Reading a timeout puts the counters behind the word back to zero; they are
+    nobody else's to touch, so other errors leave them alone."""
+    with torch.cuda.stream(torch.cuda.Stream()):
+        word = layer_error_word(cuda_device)
+        header = torch.as_tensor(moe._DeviceInts(word.data_ptr(), 64), device=cuda_device)
+        header[1:4] = 5
+        word.fill_(bit)
+        assert read_device_error(word, clear=False) == bit and (header[1:4] == 5).all()
+        assert read_device_error(word) == bit
+        assert header[0] == 0 and (header[1:4] == left).all()
+        header.zero_()
+        own = torch.full((8,), bit, dtype=torch.int32, device=cuda_device)  # a caller's own word
+        assert read_device_error(own[:1]) == bit and (own[1:] == bit).all()
+        call = layer(cuda_device, 8, logits=True)
+        want = call()
+        assert torch.equal(call(), want) and read_device_error(word) == 0

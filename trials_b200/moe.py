@@ -90,6 +90,10 @@ class _Workspaces:
         ptr = self._headers.get((index, stream))
         return self._new_header(index, stream) if ptr is None else ptr
 
+    def is_header(self, ptr: int) -> bool:
+        with self._lock:
+            return ptr in self._headers.values()
+
     def _new_header(self, index: int, stream: int) -> int:
         with self._lock:
             if (index, stream) not in self._headers:
@@ -114,10 +118,14 @@ _PACK_LAYER = struct.Struct("15qd13q").pack  # b200moe_layer_args
 
 
 def read_device_error(err_word: torch.Tensor, clear: bool = True) -> int:
-    """Returns the device error word (B200MOE_DEVERR_* bits) after the stream ran."""
+    """Returns the device error word (B200MOE_DEVERR_* bits) after the stream ran. When
+    layer_error_word() reports a timeout, clearing it puts the counters behind it back
+    to zero too, which a call that gave up may have left in between."""
     val = ctypes.c_int32()
     _lib.check(_lib.lib().b200moe_read_error(err_word.data_ptr(), ctypes.byref(val), int(clear),
                                              _stream(err_word.device)), "read_error")
+    if clear and val.value & _lib.DEVERR_TIMEOUT and _workspaces.is_header(err_word.data_ptr()):
+        torch.as_tensor(_DeviceInts(err_word.data_ptr(), 64), device=err_word.device).zero_()
     return int(val.value)
 
 
